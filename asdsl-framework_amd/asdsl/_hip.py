@@ -103,6 +103,17 @@ SIGNATURES: dict[str, list] = {
     "asdsl_decode_verify": [_P, _P, _I, _P, _P, _P, _P, _P],
     "asdsl_decode_prefill_work_bytes": [_P, _I],
     "asdsl_decode_prefill": [_P, _P, _I, _I, _P, _P, _P, _P, _P],
+    "asdsl_kv_append_f16": [_P] * 7 + [_I] * 9 + [_P],
+    "asdsl_kv_append_q8": [_P] * 9 + [_I] * 9 + [_P],
+    "asdsl_attention_window_work_bytes": [_I] * 8,
+    "asdsl_attention_window_f16kv": [_P] * 5 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_window_q8kv": [_P] * 7 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_prefix_work_bytes": [_I] * 6,
+    "asdsl_attention_prefix_f16kv": [_P] * 7 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_prefix_q8kv": [_P] * 11 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
+    "asdsl_logits_control_work_bytes": [_I, _I],
+    "asdsl_logits_control": [_P] * 6 + [_I] + [_P] * 4 + [ctypes.c_longlong, _P, ctypes.c_longlong, _I, _I, _P,
+                                                         ctypes.c_size_t, _P],
     "asdsl_kv_zero_from": [_P, _P, _I, _I, _I, _I, _P],
     "asdsl_kv_zero_from_q8": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "asdsl_repack_preq_to_preq2": [_P, _P, _P, _I, _I, _I, _P],
@@ -120,7 +131,10 @@ _RESTYPE = {"asdsl_last_error": ctypes.c_char_p, "asdsl_attention_work_floats": 
             "asdsl_sparse_down_work_bytes_n": ctypes.c_size_t, "asdsl_grid_sync_probe_work_bytes": ctypes.c_size_t,
             "asdsl_gemv_preq2_fused_batch_work_bytes": ctypes.c_size_t,
             "asdsl_gemv_preq2_fused_batch_work_bytes_n": ctypes.c_size_t,
-            "asdsl_affine_batch_work_bytes": ctypes.c_size_t}
+            "asdsl_affine_batch_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_window_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_prefix_work_bytes": ctypes.c_size_t,
+            "asdsl_logits_control_work_bytes": ctypes.c_size_t}
 
 
 class HipLibraryMissing(ImportError):

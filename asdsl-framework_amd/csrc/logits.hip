@@ -1,0 +1,165 @@
+// Control of the next token: penalties for tokens that occurred, biases and a
+// grammar's mask on logits, and the greedy token of what is left.
+//
+// Per row, with seen(v) = token v is in the row's history, n(v) = its
+// occurrences past the prompt, each step rounded to fp32:
+//   y = seen ? (x > 0 ? x / repetition : x * repetition) : x
+//   y = y - frequency * n;  y = n > 0 ? y - presence : y;  y = y + bias
+//   out = allowed ? y : -inf;  token = the first largest allowed y (-1: none)
+#include <climits>
+
+#include "abi_util.hpp"
+#include "device_common.hpp"
+
+namespace asdsl {
+namespace {
+
+constexpr int kSlice = 4096;    // tokens of one workgroup
+constexpr int kThreads = 256;
+constexpr uint32_t kSeen = 0x80000000u;  // a slice's word per token: seen, and the count past the prompt
+
+struct ControlArgs {
+    const float* logits;
+    float* out;
+    unsigned long long* keys;  // [rows][slices], null without tokens
+    const int* history;
+    const int* prompt_len;
+    const int* history_len;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const float* bias;
+    const uint32_t* allowed;
+    int cap, vocab, slices;
+    long long bias_stride, allowed_stride;
+};
+
+// The slice's words are counted in LDS from the row's whole history (integer
+// atomics: any order gives the same), then its logits pass through once.
+__global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlArgs a) {
+#pragma clang fp contract(off)  // each step of the definition rounds by itself
+    __shared__ uint32_t word[kSlice];
+    __shared__ unsigned long long red[kThreads / kWave];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int row = static_cast<int>(blockIdx.x / a.slices);
+    const int slice = static_cast<int>(blockIdx.x % a.slices);
+    const int v0 = slice * kSlice;
+    const int n = min(kSlice, a.vocab - v0);
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.history) {
+        for (int i = tid; i < kSlice; i += kThreads) word[i] = 0u;
+        __syncthreads();
+        const int told = min(max(a.history_len ? a.history_len[row] : a.cap, 0), a.cap);
+        const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
+        const int* ids = a.history + static_cast<long long>(row) * a.cap;
+        for (int i = tid; i < told; i += kThreads) {
+            const uint32_t at = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(v0);
+            if (ids[i] >= 0 && at < static_cast<uint32_t>(n)) {
+                atomicOr(&word[at], kSeen);
+                if (i >= prompt) atomicAdd(&word[at], 1u);
+            }
+        }
+        if (a.repetition) rep = a.repetition[row];
+        if (a.frequency) freq = a.frequency[row];
+        if (a.presence) pres = a.presence[row];
+        __syncthreads();
+    }
+    const long long base = static_cast<long long>(row) * a.vocab + v0;
+    const float* bias = a.bias ? a.bias + row * a.bias_stride + v0 : nullptr;
+    const uint32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+    unsigned long long best = 0ull;
+    for (int i = tid; i < n; i += kThreads) {
+        float y = a.logits[base + i];
+        const uint32_t w = a.history ? word[i] : 0u;
+        if (w != 0u) {
+            y = y > 0.0f ? y / rep : y * rep;
+            const uint32_t c = w & ~kSeen;
+            y = y - freq * static_cast<float>(c);
+            if (c != 0u) y = y - pres;
+        }
+        if (bias) y = y + bias[i];
+        const int v = v0 + i;
+        const bool ok = !allowed || ((allowed[v >> 5] >> (v & 31)) & 1u) != 0u;
+        a.out[base + i] = ok ? y : -INFINITY;
+        if (ok && y == y) {
+            const unsigned long long k = argmax_key(y == 0.0f ? 0.0f : y, v);
+            best = k > best ? k : best;
+        }
+    }
+    if (!a.keys) return;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const unsigned long long other = __shfl_xor(best, o, kWave);
+        best = other > best ? other : best;
+    }
+    if ((tid & (kWave - 1)) == 0) red[tid / kWave] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int q = 1; q < kThreads / kWave; ++q) best = red[q] > best ? red[q] : best;
+        a.keys[blockIdx.x] = best;
+    }
+}
+
+// One wave per row: the largest of its slices' keys (0: nothing was allowed).
+__global__ __launch_bounds__(kWave) void logits_token_kernel(const unsigned long long* __restrict__ keys, int slices,
+                                                             int* __restrict__ tokens) {
+    unsigned long long best = 0ull;
+    for (int i = static_cast<int>(threadIdx.x); i < slices; i += kWave) {
+        const unsigned long long k = keys[static_cast<long long>(blockIdx.x) * slices + i];
+        best = k > best ? k : best;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const unsigned long long other = __shfl_xor(best, o, kWave);
+        best = other > best ? other : best;
+    }
+    if (threadIdx.x == 0)
+        tokens[blockIdx.x] = best != 0ull ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
+}
+
+int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+
+}  // namespace
+}  // namespace asdsl
+
+using namespace asdsl;
+
+extern "C" size_t asdsl_logits_control_work_bytes(int n_rows, int vocab) {
+    if (n_rows <= 0 || vocab <= 0) return 0;
+    return (static_cast<size_t>(n_rows) * slices_of(vocab) * sizeof(unsigned long long) + 255) / 256 * 256;
+}
+
+extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, const int* history,
+                                             const int* prompt_len, const int* history_len, int history_cap,
+                                             const float* repetition, const float* frequency, const float* presence,
+                                             const float* bias, long long bias_stride, const uint32_t* allowed,
+                                             long long allowed_stride, int n_rows, int vocab, void* work,
+                                             size_t work_bytes, asdsl_stream_t stream) {
+    const char* what = "logits_control";
+    ASDSL_CHECK_ARG(logits && out, "%s: null pointer", what);
+    ASDSL_CHECK_ARG(n_rows > 0 && vocab > 0, "%s: n_rows and vocab must be positive", what);
+    ASDSL_CHECK_ARG(history_cap >= 0, "%s: history_cap must not be negative", what);
+    ASDSL_CHECK_ARG(history || (!prompt_len && !history_len && !repetition && !frequency && !presence),
+                    "%s: lengths or penalties without a history", what);
+    ASDSL_CHECK_ARG(!bias || bias_stride == 0 || bias_stride >= vocab,
+                    "%s: bias_stride must be 0 or at least vocab", what);
+    ASDSL_CHECK_ARG(!allowed || allowed_stride == 0 || allowed_stride >= (vocab + 31LL) / 32,
+                    "%s: allowed_stride must be 0 or at least (vocab + 31) / 32", what);
+    ASDSL_CHECK_ARG(static_cast<long long>(n_rows) * slices_of(vocab) <= INT_MAX, "%s: too many rows", what);
+    void* ws = nullptr;
+    if (tokens) {
+        ASDSL_CHECK_ARG(work, "%s: tokens need a work buffer", what);
+        const asdsl_status st = work_buffer(as_hip(stream), work, work_bytes,
+                                            asdsl_logits_control_work_bytes(n_rows, vocab), &ws, what);
+        if (st != ASDSL_OK) return st;
+    }
+    const int slices = slices_of(vocab);
+    const ControlArgs a{logits, out, static_cast<unsigned long long*>(ws), history_cap > 0 ? history : nullptr,
+                        prompt_len, history_len, repetition, frequency, presence, bias, allowed, history_cap, vocab,
+                        slices, bias_stride, allowed_stride};
+    asdsl_status st = launch("logits_control_kernel", logits_control_kernel, dim3(static_cast<unsigned>(n_rows * slices)),
+                             dim3(kThreads), 0, as_hip(stream), a);
+    if (st != ASDSL_OK || !tokens) return st;
+    return launch("logits_token_kernel", logits_token_kernel, dim3(n_rows), dim3(kWave), 0, as_hip(stream),
+                  static_cast<const unsigned long long*>(ws), slices, tokens);
+}

@@ -632,6 +632,100 @@ size_t asdsl_decode_prefill_work_bytes(const asdsl_decode_model* model, int max_
 asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, const int* tokens, int n_tokens, int start_pos,
                                   int* token, int* pos, float* logits, void* work, asdsl_stream_t stream);
 
+/* ------------------------------------------- many tokens, many sequences
+ * Operators beside the single-sequence decode step.  Caches are
+ * [n_seq][n_kv_heads][rows][head_dim], fp16, or int8 codes with fp32 scales
+ * [n_seq][n_kv_heads][rows][head_dim / 64] (the decode step's two forms; its
+ * caches are such caches with n_seq = 1); queries and outputs are fp32
+ * [n_seq * n_tokens][n_heads][head_dim], token t of sequence s in row
+ * s * n_tokens + t.  head_dim is 64 or 128, n_heads any multiple of n_kv_heads.
+ * qkv, q, out, q_out and the caches are 16-byte aligned.  Work buffers are the
+ * caller's (256-byte aligned, the size from the *_work_bytes query, contents
+ * afterwards unspecified; null where the query gives 0): calls that may
+ * overlap, two captured graphs among them, take one each.  Nothing is
+ * allocated, and a captured call replays with the positions that the device
+ * then holds.  No reference counterpart (the reference decodes one sequence). */
+
+/* RoPE and the new cache rows.  qkv [n_seq * n_tokens][(n_heads + 2 *
+ * n_kv_heads) * head_dim] = [q | k | v] per token.  Token t of sequence s goes
+ * to cache row r = pos[s] + t and is rotated for position r + pos_offset
+ * (rope_cos/rope_sin [rope_rows][rotary_dim / 2], half split, as in
+ * asdsl_attention_f16kv): q_out = the rotated queries, the cache row = the
+ * rotated key and the value, rounded to fp16 or quantized as
+ * asdsl_attention_q8kv does, with the same bits.  A token whose row is outside
+ * [0, rows), or whose position is outside the tables, writes no cache row, and
+ * its q_out is zero.  q_out must not overlap qkv. */
+asdsl_status asdsl_kv_append_f16(const float* qkv, uint16_t* k_cache, uint16_t* v_cache, const float* rope_cos,
+                                 const float* rope_sin, const int* pos, float* q_out, int n_seq, int n_tokens,
+                                 int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int rows, int pos_offset,
+                                 int rope_rows, asdsl_stream_t stream);
+asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, int8_t* v_cache, float* k_scale, float* v_scale,
+                                const float* rope_cos, const float* rope_sin, const int* pos, float* q_out, int n_seq,
+                                int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int rows,
+                                int pos_offset, int rope_rows, asdsl_stream_t stream);
+
+/* Attention with a sliding window and first tokens that stay visible: token t
+ * of sequence s, at position p = pos[s] + t, sees cache rows j <= p with
+ * j < sinks or j > p - window (window 0: all j <= p), and
+ * out = softmax(q.K / sqrt(head_dim)) V over them.  A token whose position is
+ * outside [0, rows) sees nothing: its out is zero (a padded sequence has pos
+ * -n_tokens or less).  Rows that no token sees are not looked at, whatever
+ * they hold; a row that is not finite reaches only the tokens that see it. */
+size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
+                                         int window, int sinks);
+asdsl_status asdsl_attention_window_f16kv(const float* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                                          const int* pos, float* out, int n_seq, int n_tokens, int n_heads,
+                                          int n_kv_heads, int head_dim, int rows, int window, int sinks, void* work,
+                                          size_t work_bytes, asdsl_stream_t stream);
+asdsl_status asdsl_attention_window_q8kv(const float* q, const int8_t* k_cache, const int8_t* v_cache,
+                                         const float* k_scale, const float* v_scale, const int* pos, float* out,
+                                         int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
+                                         int window, int sinks, void* work, size_t work_bytes, asdsl_stream_t stream);
+
+/* Attention of one token each of n_seq sequences that share a prefix, whose
+ * rows are read once for all: sequence s sees rows [0, prefix_len) of the
+ * prefix caches [n_kv_heads][prefix_rows][head_dim] and rows [0, own_pos[s]] of
+ * its own caches [n_seq][n_kv_heads][own_rows][head_dim] (own_pos[s] = -1:
+ * none); its token follows them all.  A sequence that sees nothing, or whose
+ * own_pos is outside [-1, own_rows), gets zero.  With prefix_len 0 the prefix
+ * pointers may be null. */
+size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
+                                         int own_rows);
+asdsl_status asdsl_attention_prefix_f16kv(const float* q, const uint16_t* k_prefix, const uint16_t* v_prefix,
+                                          const uint16_t* k_own, const uint16_t* v_own, const int* own_pos, float* out,
+                                          int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
+                                          int prefix_rows, int own_rows, void* work, size_t work_bytes,
+                                          asdsl_stream_t stream);
+asdsl_status asdsl_attention_prefix_q8kv(const float* q, const int8_t* k_prefix, const int8_t* v_prefix,
+                                         const float* k_prefix_scale, const float* v_prefix_scale, const int8_t* k_own,
+                                         const int8_t* v_own, const float* k_own_scale, const float* v_own_scale,
+                                         const int* own_pos, float* out, int n_seq, int n_heads, int n_kv_heads,
+                                         int head_dim, int prefix_len, int prefix_rows, int own_rows, void* work,
+                                         size_t work_bytes, asdsl_stream_t stream);
+
+/* Control of the next token: logits [n_rows][vocab] -> out (may be logits
+ * itself) and tokens[n_rows] (may be null), per row, each step rounded to fp32:
+ *   y = x > 0 ? x / repetition : x * repetition   for tokens of the history
+ *   y -= frequency * n, then y -= presence        for tokens that occur n > 0
+ *                                                 times past the prompt
+ *   y += bias;  out = allowed ? y : -inf
+ * history [n_rows][history_cap] holds token ids, of which the row's first
+ * history_len[row] count (null: all; clamped to [0, history_cap]) and the first
+ * prompt_len[row] of those are the prompt (null: none); ids outside [0, vocab)
+ * are skipped.  repetition (positive), frequency and presence [n_rows] may each
+ * be null: none.  bias: null, or vocab values a row, bias_stride apart (0: one
+ * row for all).  allowed: null, or bit v % 32 of word v / 32 per row,
+ * allowed_stride words apart (0: one row for all).  tokens[row] = the first
+ * largest allowed y, -1 where none is allowed; a NaN is never taken.  work is
+ * needed for tokens only. */
+size_t asdsl_logits_control_work_bytes(int n_rows, int vocab);
+asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, const int* history,
+                                  const int* prompt_len, const int* history_len, int history_cap,
+                                  const float* repetition, const float* frequency, const float* presence,
+                                  const float* bias, long long bias_stride, const uint32_t* allowed,
+                                  long long allowed_stride, int n_rows, int vocab, void* work, size_t work_bytes,
+                                  asdsl_stream_t stream);
+
 /* The int8 cache's form of asdsl_kv_zero_from: codes 0 and scales 1.0 in rows
  * [from_pos, max_seq), as zero_kv_from leaves them
  * (asdsl/kernels/native/unified_engine.cpp:1263-1283). */
