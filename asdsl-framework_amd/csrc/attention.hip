@@ -9,6 +9,7 @@
 #include <hip/hip_fp16.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "abi_util.hpp"
 #include "device_common.hpp"
@@ -29,11 +30,12 @@ struct Cache {
 };
 
 // ------------------------------------------------------------------ append
-// Eight dims of one head of one token per lane.  A rotated pair is
-// (fmaf(a, c, -(b * s)), fmaf(a, s, b * c)), as in the decode step's
-// attention, and the stored forms are its too: fp16 rounded to nearest, or
-// per 64 dims scale = amax * (1/127) (1e-12 when amax <= 1e-12) and code =
-// round-half-even(x * (1 / scale)) clamped to [-127, 127].
+// Four dims of one head of one token per lane, so that loads and stores are 16
+// neighbouring bytes a lane (8 of an fp16 row).  A rotated pair is (fmaf(a, c,
+// -(b * s)), fmaf(a, s, b * c)), as in the decode step's attention, and the
+// stored forms are its too: fp16 rounded to nearest, or per 64 dims scale =
+// amax * (1/127) (1e-12 when amax <= 1e-12) and code = round-half-even(x * (1 /
+// scale)) clamped to [-127, 127].
 struct AppendArgs {
     const float* qkv;
     void* k;
@@ -45,71 +47,80 @@ struct AppendArgs {
     const int* pos;
     float* q_out;
     int n_tokens, n_heads, n_kv, rot_half, rows, offset, rope_rows;
-    long long units;  // 8-dim units of the call
+    int chunks;  // workgroups a token
 };
+constexpr int kAppendThreads = 256;
 
-template <int D, bool Q8>
-__global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
-    constexpr int kUnits = D / 8;  // per head
-    const long long e = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-    if (e >= a.units) return;  // units are a multiple of 8: the lanes of a 64-dim block leave together
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+
+// kVec: rotary pairs and table rows lie in whole 16-byte units.
+template <int D, bool Q8, bool kVec>
+__global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendArgs a) {
+    constexpr int kUnits = D / 4;  // per head
     const int heads = a.n_heads + 2 * a.n_kv;
-    const int dc = static_cast<int>(e % kUnits);
-    const long long hr = e / kUnits;
-    const int head = static_cast<int>(hr % heads);
-    const long long row = hr / heads;  // token row of the call
-    const int seq = static_cast<int>(row / a.n_tokens);
+    const int row = static_cast<int>(blockIdx.x) / a.chunks;  // token row of the call
+    const int u = static_cast<int>(blockIdx.x) % a.chunks * kAppendThreads + static_cast<int>(threadIdx.x);
+    const int head = u / kUnits, d = u % kUnits * 4;
+    if (head >= heads) return;  // whole heads: the lanes of a 64-dim block leave together
+    const int seq = row / a.n_tokens;
+    const float* src = a.qkv + (static_cast<size_t>(row) * heads + head) * D;
+    const float4 own = load4(src + d);
     const long long r = static_cast<long long>(a.pos[seq]) + row % a.n_tokens;  // cache row
     const long long p = r + a.offset;                                           // rotary position
     const bool inside = r >= 0 && r < a.rows && p >= 0 && p < a.rope_rows;
     if (!inside && head >= a.n_heads) return;
-    const float* src = a.qkv + (row * heads + head) * D;
-    float x[8];
+    float x[4] = {own.x, own.y, own.z, own.w};
+    const int half = a.rot_half;
+    if (!inside) {
+        x[0] = x[1] = x[2] = x[3] = 0.0f;
+    } else if (head < a.n_heads + a.n_kv && d < 2 * half) {
+        const float* cs = a.cos + p * half;
+        const float* sn = a.sin + p * half;
+        if constexpr (kVec) {
+            const bool first = d < half;
+            const int j = first ? d : d - half;
+            const float4 o = load4(src + (first ? d + half : j)), c4 = load4(cs + j), s4 = load4(sn + j);
+            const float y[4] = {o.x, o.y, o.z, o.w}, c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = 8 * dc + i;
-        if (!inside) {
-            x[i] = 0.0f;
-        } else if (head >= a.n_heads + a.n_kv || d >= 2 * a.rot_half) {
-            x[i] = src[d];
+            for (int i = 0; i < 4; ++i)
+                x[i] = first ? fmaf(x[i], c[i], -(y[i] * s[i])) : fmaf(y[i], s[i], x[i] * c[i]);
         } else {
-            const int j = d < a.rot_half ? d : d - a.rot_half;
-            const float lo = src[j], hi = src[j + a.rot_half];
-            const float c = a.cos[p * a.rot_half + j], s = a.sin[p * a.rot_half + j];
-            x[i] = d < a.rot_half ? fmaf(lo, c, -(hi * s)) : fmaf(lo, s, hi * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (d + i >= 2 * half) continue;
+                const bool first = d + i < half;
+                const int j = first ? d + i : d + i - half;
+                const float lo = src[j], hi = src[j + half];
+                x[i] = first ? fmaf(lo, cs[j], -(hi * sn[j])) : fmaf(lo, sn[j], hi * cs[j]);
+            }
         }
     }
     if (head < a.n_heads) {
-        float4* dst = reinterpret_cast<float4*>(a.q_out + (row * a.n_heads + head) * D + 8 * dc);
-        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+        *reinterpret_cast<float4*>(a.q_out + (static_cast<size_t>(row) * a.n_heads + head) * D + d) =
+            make_float4(x[0], x[1], x[2], x[3]);
         return;
     }
     const bool key = head < a.n_heads + a.n_kv;
     const int kvh = head - a.n_heads - (key ? 0 : a.n_kv);
-    const long long crow = (static_cast<long long>(seq) * a.n_kv + kvh) * a.rows + r;
+    const size_t crow = (static_cast<size_t>(seq) * a.n_kv + kvh) * a.rows + static_cast<size_t>(r);
     void* base = key ? a.k : a.v;
     if constexpr (Q8) {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-        m = group_max<8>(m);
+        const float m = group_max<16>(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
         const float scale = m > 1e-12f ? m * kInv127 : 1e-12f;
         const float inv = 1.0f / scale;
-        int q[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            q[i] = static_cast<int>(fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.0f), 127.0f));
-        *reinterpret_cast<uint2*>(static_cast<int8_t*>(base) + crow * D + 8 * dc) =
-            make_uint2(pack4_i8(q[0], q[1], q[2], q[3]), pack4_i8(q[4], q[5], q[6], q[7]));
-        if ((dc & 7) == 0) (key ? a.ks : a.vs)[crow * (D / kBlockDims) + (dc >> 3)] = scale;
-    } else {
-        uint32_t w[4];
+        int q[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
+            q[i] = static_cast<int>(fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.0f), 127.0f));
+        *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(base) + crow * D + d) = pack4_i8(q[0], q[1], q[2], q[3]);
+        if (d % kBlockDims == 0) (key ? a.ks : a.vs)[crow * (D / kBlockDims) + d / kBlockDims] = scale;
+    } else {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
             w[i] = static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x[2 * i]))) |
                    (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x[2 * i + 1]))) << 16);
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + crow * D + 8 * dc) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + crow * D + d) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -120,9 +131,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 // a first part of 11 bits and the rest (2^-22 off at most), at twice the
 // products.  One part alone would leave 2^-12 a weight, 1e-4 of an output.
 // The parts keep clear of fp16's small numbers: a query row is scaled by a power
-// of two to 2^12..2^13, the weights are 2^kShift times theirs (the first part is
-// then whole down to 2^-22 of the largest weight, the second to 2^-11 of it, and
-// off by 2^-33 of it below; a larger shift costs the exponent's argument bits).
+// of two to 2^12..2^13, the weights are 2^kShift times theirs or more (the first
+// part is then whole down to 2^-22 of the largest weight, the second to 2^-11 of
+// it, and off by 2^-33 of it below; more costs bits of the exponent's argument).
 //
 // A wave takes 16 query rows (the columns of its tiles) and 32 keys a step:
 //   S' = K Q'  two 16x16 tiles; a lane gets 8 scores of the one row it holds, so
@@ -132,11 +143,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const AppendArgs a) {
 //              keys and turns the block in registers; no transposition in memory.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kRows = 16;      // query rows of a wave's tile
 constexpr int kKeys = 32;      // keys of a wave's step
 constexpr float kShift = 8.0f;
+constexpr float kMost = 14.0f;  // and 2 more for an int8 cache's scales: below fp16's 2^16
 constexpr int kFewWaves = 4;
 
 // The keys of one KV head that a workgroup's rows see between them: rows [0, na)
@@ -175,28 +189,33 @@ struct AttnArgs {
     float scale;        // log2(e) / sqrt(D)
 };
 
-// The other operand's value from lane ^ 32 and lane ^ 16: the swap exchanges one
-// half (rows of 16) of a register with the other half of a second one, so with
-// two copies of v the results hold both lanes' values.  The copy is kept
-// apart from v: given one register twice, the swap leaves it as it is.
-template <typename F>
-__device__ __forceinline__ float lanes16(float v, F f) {
+// f over the lanes that hold one row: lane % kStep is the same (16: four lanes,
+// 32: two).  A swap exchanges one half (or odd rows of 16) of a register with
+// the other half of a second one, so with two copies of v the results hold
+// both lanes' values.  The copy is kept apart from v: given one register twice,
+// the swap leaves it as it is.
+template <int kStep, typename F>
+__device__ __forceinline__ float lanes(float v, F f) {
     uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
     asm("" : "+v"(b));
     auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
     v = f(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
-    a = b = __builtin_bit_cast(uint32_t, v);
-    asm("" : "+v"(b));
-    r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    return f(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+    if constexpr (kStep == 16) {
+        a = b = __builtin_bit_cast(uint32_t, v);
+        asm("" : "+v"(b));
+        r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+        v = f(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
+              __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+    }
+    return v;
 }
-
-// Over the four lanes of equal lane % 16.
-__device__ __forceinline__ float lanes16_max(float v) {
-    return lanes16(v, [](float x, float y) { return fmaxf(x, y); });
+template <int kStep>
+__device__ __forceinline__ float lanes_max(float v) {
+    return lanes<kStep>(v, [](float x, float y) { return fmaxf(x, y); });
 }
-__device__ __forceinline__ float lanes16_sum(float v) {
-    return lanes16(v, [](float x, float y) { return x + y; });
+template <int kStep>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return lanes<kStep>(v, [](float x, float y) { return x + y; });
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -211,29 +230,28 @@ __device__ __forceinline__ int exponent(float x) {
 
 // x = hi + lo with fp16 parts, two at a time.
 __device__ __forceinline__ void two_parts(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const half2v h = {static_cast<_Float16>(x0), static_cast<_Float16>(x1)};
-    const half2v l = {static_cast<_Float16>(x0 - static_cast<float>(h.x)),
-                      static_cast<_Float16>(x1 - static_cast<float>(h.y))};
+    const half2v h = __builtin_convertvector((f32x2{x0, x1}), half2v);
     hi = __builtin_bit_cast(uint32_t, h);
-    lo = __builtin_bit_cast(uint32_t, l);
+    f32x2 d;  // x - h, exactly; the compiler converts h back in an instruction of its own
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(d.x) : "v"(hi), "v"(x0));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d.y) : "v"(hi), "v"(x1));
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(d, half2v));
 }
 
 __device__ __forceinline__ half8 as_half8(const uint32_t (&w)[4]) {
     return __builtin_bit_cast(half8, make_uint4(w[0], w[1], w[2], w[3]));
 }
 
-// Two bytes c0 at bits 0-7 and c1 at bits 16-23 of w, int8 codes with their top
-// bit flipped, as fp16 numbers: 0x6400 | u is 1024 + u, exactly.
+// Two int8 codes at bits 0-7 and 16-23 of w as fp16 numbers: with the top bit
+// flipped a code is u = code + 128, and 0x6400 | u is 1024 + u, exactly.
 __device__ __forceinline__ uint32_t codes_half2(uint32_t w) {
-    const half2v h = __builtin_bit_cast(half2v, w | 0x64006400u) - half2v{_Float16(1152.0f), _Float16(1152.0f)};
+    const half2v h = __builtin_bit_cast(half2v, w ^ 0x64806480u) - half2v{_Float16(1152.0f), _Float16(1152.0f)};
     return __builtin_bit_cast(uint32_t, h);
 }
 
 // Eight int8 codes as the K operand's eight fp16 numbers.
 __device__ __forceinline__ half8 codes_half8(uint2 c) {
     uint32_t w[4];
-    c.x ^= 0x80808080u;
-    c.y ^= 0x80808080u;
     w[0] = codes_half2(__builtin_amdgcn_perm(0u, c.x, 0x0C010C00u));
     w[1] = codes_half2(__builtin_amdgcn_perm(0u, c.x, 0x0C030C02u));
     w[2] = codes_half2(__builtin_amdgcn_perm(0u, c.y, 0x0C010C00u));
@@ -241,20 +259,27 @@ __device__ __forceinline__ half8 codes_half8(uint2 c) {
     return as_half8(w);
 }
 
-// A query row's operands: dims 32 * s + 8 * (lane / 16) .. + 8 in step s.
-template <int D>
+// All ones in each half of w that is an infinity or NaN (an exponent of all ones).
+__device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
+    const uint32_t t = (w & 0x7C007C00u) + 0x04000400u;
+    return (t & 0x8000u ? 0xFFFFu : 0u) | (t & 0x80000000u ? 0xFFFF0000u : 0u);
+}
+
+// A query row's operands: dims kDims * s + 8 * part .. + 8 in step s, part =
+// lane / (512 / kDims): kDims 32 for 16x16 tiles, 16 for 32x32 tiles.
+template <int D, int kDims>
 struct Query {
-    half8 hi[D / 32], lo[D / 32];
+    half8 hi[D / kDims], lo[D / kDims];
     float c;  // score = product * c, in powers of two
 
-    __device__ __forceinline__ void load(const float* row, int gq, float scale) {
-        float x[D / 32][8];
+    __device__ __forceinline__ void load(const float* row, int part, float scale) {
+        float x[D / kDims][8];
         float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
+        for (int s = 0; s < D / kDims; ++s) {
             if (row) {
-                const float4 a = *reinterpret_cast<const float4*>(row + 32 * s + 8 * gq);
-                const float4 b = *reinterpret_cast<const float4*>(row + 32 * s + 8 * gq + 4);
+                const float4 a = *reinterpret_cast<const float4*>(row + kDims * s + 8 * part);
+                const float4 b = *reinterpret_cast<const float4*>(row + kDims * s + 8 * part + 4);
                 x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
                 x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
             } else {
@@ -264,13 +289,13 @@ struct Query {
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[s][i]));
         }
-        top = lanes16_max(top);
+        top = lanes_max<512 / kDims>(top);
         int e = 12 - exponent(top);  // a query that is not finite stays as it is
         e = e < -115 ? 0 : (e > 120 ? 120 : e);
         const float f = pow2(e);
         c = scale * pow2(-e);
 #pragma unroll
-        for (int s = 0; s < D / 32; ++s) {
+        for (int s = 0; s < D / kDims; ++s) {
             uint32_t h[4], l[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) two_parts(x[s][2 * i] * f, x[s][2 * i + 1] * f, h[i], l[i]);
@@ -291,8 +316,8 @@ struct VRaw;
 template <int D>
 struct VRaw<D, false> {
     uint32_t w[8][D / 32];
-    __device__ __forceinline__ void load(const void* v, int key, size_t row, int r) {
-        const uint16_t* src = static_cast<const uint16_t*>(v) + row * D + D / 16 * r;
+    __device__ __forceinline__ void load(const char* row, int key, int r) {
+        const char* src = row + D / 8 * r;
         if constexpr (D == 128) {
             const uint4 x = *reinterpret_cast<const uint4*>(src);
             w[key][0] = x.x; w[key][1] = x.y; w[key][2] = x.z; w[key][3] = x.w;
@@ -321,73 +346,119 @@ struct VRaw<D, false> {
 template <int D>
 struct VRaw<D, true> {
     uint32_t w[8][D / 64];
-    __device__ __forceinline__ void load(const void* v, int key, size_t row, int r) {
-        const int8_t* src = static_cast<const int8_t*>(v) + row * D + 4 * r;
+    __device__ __forceinline__ void load(const char* row, int key, int r) {
+        const char* src = row + 4 * r;
 #pragma unroll
         for (int b = 0; b < D / 64; ++b)
-            w[key][b] = *reinterpret_cast<const uint32_t*>(src + 64 * b) ^ 0x80808080u;
+            w[key][b] = *reinterpret_cast<const uint32_t*>(src + 64 * b);
     }
     __device__ __forceinline__ half8 operand(int j) const {
         uint32_t o[4];
         const uint32_t sel = 0x0C040C00u + 0x00010001u * static_cast<uint32_t>(j & 3);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) o[p] = codes_half2(__builtin_amdgcn_perm(w[2 * p + 1][j >> 2], w[2 * p][j >> 2], sel));
+        for (int p = 0; p < 4; ++p)
+            o[p] = codes_half2(__builtin_amdgcn_perm(w[2 * p + 1][j >> 2], w[2 * p][j >> 2], sel));
         return as_half8(o);
     }
 };
 
-// Running state of one query row (column lane % 16): the base m of its weights
-// exp2(score - m), kShift below the largest score so far, their sum over the
-// lane's share of the keys, and O' with element i of acc[j] at dim
-// *_dim(4 * (lane / 16) + i, j).  An int8 cache's value scales go into the
+// Running state of one query row, held by the lanes of equal lane % kStep: the
+// base m of its weights exp2(score - m) and their sum over the lane's share of
+// the keys.  A base is set kShift below the row's largest score so far and
+// stays while the scores keep kMost above it at most: nearly always after a
+// row's first keys, so that a step then needs no exchange between lanes and no
+// scaling of what was accumulated.  An int8 cache's value scales go into the
 // weights before they are cut; ev is the power of two that keeps those in
-// fp16's range (the accumulator is 2^-ev times O').
-template <int D, bool Q8>
-struct State {
+// fp16's range (the row's accumulators are 2^-ev times O').
+template <bool Q8, int kStep>
+struct Softmax {
     float m = -INFINITY, l = 0.0f;
     int ev = -126;
+
+    // Whether a step's products (score = s * c) or its seen value scales ask for a
+    // new base, in any lane of the wave; then the base and the factor of what
+    // the row has accumulated.
+    template <int N>
+    __device__ __forceinline__ bool rises(const float (&s)[N], float c, float vs_max, float& top) const {
+        top = s[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
+        top *= c;
+        bool up = top - m > kMost;
+        if constexpr (Q8) up |= exponent(vs_max) > ev;
+        return __builtin_amdgcn_ballot_w64(up) != 0ull;
+    }
+    __device__ __forceinline__ float rebase(float top, float vs_max) {
+        top = lanes_max<kStep>(top);
+        const float m1 = top - m > kMost ? top - kShift : m;
+        float alpha = m == m1 ? 1.0f : exp2_fast(m - m1);
+        m = m1;
+        l *= alpha;
+        if constexpr (Q8) {
+            const int e1 = max(ev, exponent(lanes_max<kStep>(vs_max)));
+            alpha *= pow2(max(ev - e1, -126));
+            ev = e1;
+        }
+        return alpha;
+    }
+    // The weights of N keys from their products, in place.
+    template <int N>
+    __device__ __forceinline__ void weigh(float (&s)[N], float c) {
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum[4] = {};
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[i] = exp2_fast(fmaf(s[i], c, -base));
+            sum[i & 3] += s[i];
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    }
+    __device__ __forceinline__ float out_scale() const {
+        if constexpr (Q8) return pow2(max(ev, -126));
+        return 1.0f;
+    }
+};
+
+// O' of 16 rows: element i of acc[j] at dim *_dim(4 * (lane / 16) + i, j).
+template <int D, bool Q8>
+struct State : Softmax<Q8, 16> {
     f32x4 acc[D / 16];
 
     __device__ __forceinline__ State() {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
-    // The weights of N keys from their products s (score = s * c; -inf where not
-    // seen), in place.  vs_max: the largest finite value scale among the keys
-    // of this step that the row sees.
     template <int N>
-    __device__ __forceinline__ void weigh(float (&s)[N], float c, float vs_max) {
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
-        const float m1 = fmaxf(m, lanes16_max(top) * c - kShift);
-        const float base = m1 == -INFINITY ? 0.0f : m1;
-        float alpha = exp2_fast(m - base);
-        l *= alpha;
-        if constexpr (Q8) {
-            const int e1 = max(ev, exponent(lanes16_max(vs_max)));
-            alpha *= pow2(max(ev - e1, -126));
-            ev = e1;
-        }
-        m = m1;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            s[i] = exp2_fast(fmaf(s[i], c, -base));
-            l += s[i];
-        }
-        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0ull) {
+    __device__ __forceinline__ void step(float (&s)[N], float c, float vs_max) {
+        float top;
+        if (this->rises(s, c, vs_max, top)) {
+            const float alpha = this->rebase(top, vs_max);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
         }
+        this->weigh(s, c);
     }
 };
+
+// A value that is the same in every lane, in a scalar register.  Every condition
+// around a matrix instruction has to be one: the instruction writes all lanes,
+// also where the compiler has masked them off for the other side of a branch.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
 __device__ __forceinline__ int cache_row(const Keys& K, int i) { return i < K.na ? i : i + K.db; }
+
+// Whether the rows of keys [i0, i0 + kKeys) follow each other in the cache.
+__device__ __forceinline__ bool rows_follow(const Keys& K, int i0) {
+    return i0 + kKeys <= K.n && (i0 >= K.na || i0 + kKeys <= K.na);
+}
 
 // Whether every one of the workgroup's tokens sees all the keys [i0, i0 + n).
 __device__ __forceinline__ bool all_seen(const Keys& K, int i0, int n) {
@@ -396,68 +467,88 @@ __device__ __forceinline__ bool all_seen(const Keys& K, int i0, int n) {
     return cache_row(K, i0 + n - 1) <= K.p_first && (i0 + n <= K.na || cache_row(K, max(i0, K.na)) >= K.lo_last);
 }
 
-// P' of 8 keys (s) as two fp16 operands, and O' += V' P'.
+// P' of 8 keys as two fp16 operands per scale block (one without scales).
 template <int D, bool Q8>
-__device__ __forceinline__ void add_values(State<D, Q8>& st, const VRaw<D, Q8>& v, const float (&s)[8],
-                                           const float (&vs)[8][D / 64], uint32_t seen, bool all) {
-    if constexpr (Q8) {
-        const float f = pow2(min(max(-st.ev, -126), 126));
+struct Weights {
+    static constexpr int kBlocks = Q8 ? D / 64 : 1;
+    uint32_t h[kBlocks][4], l[kBlocks][4];
+
+    // vs: the keys' value scales; a scale of a key that the row does not see
+    // may be anything.  ev: the row's State::ev.
+    __device__ __forceinline__ void cut(const float* s, const float (*vs)[D / 64], uint32_t seen, int ev) {
+        if constexpr (Q8) {
+            const float f = pow2(min(-ev, 126));
 #pragma unroll
-        for (int b = 0; b < D / 64; ++b) {
-            uint32_t h[4], l[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // a scale of a key that the row does not see may be anything
-                const float x0 = (seen >> (2 * i)) & 1u ? s[2 * i] * (vs[2 * i][b] * f) : 0.0f;
-                const float x1 = (seen >> (2 * i + 1)) & 1u ? s[2 * i + 1] * (vs[2 * i + 1][b] * f) : 0.0f;
-                two_parts(x0, x1, h[i], l[i]);
-            }
-#pragma unroll
-            for (int j = 4 * b; j < 4 * b + 4; ++j) {
-                const half8 o = v.operand(j);
-                st.acc[j] = mfma(o, as_half8(h), st.acc[j]);
-                st.acc[j] = mfma(o, as_half8(l), st.acc[j]);
-            }
-        }
-    } else {
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) two_parts(s[2 * i], s[2 * i + 1], h[i], l[i]);
-        // Infinities and NaN among the values of keys that not every row sees:
-        // a weight of zero would make them NaN in every row.  They are taken
-        // out, and NaN goes to the outputs of the rows that see them.
-        if (!all && __builtin_amdgcn_ballot_w64(v.odd()) != 0ull) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[i] = ((seen >> (2 * i)) & 1u ? 0x3C00u : 0u) | ((seen >> (2 * i + 1)) & 1u ? 0x3C000000u : 0u);
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) {
-                const uint4 o = __builtin_bit_cast(uint4, v.operand(j));
-                uint32_t clean[4] = {o.x, o.y, o.z, o.w}, bad[4];
+            for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t t = ((clean[i] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
-                    const uint32_t mask = (t & 0x8000u ? 0xFFFFu : 0u) | (t & 0x80000000u ? 0xFFFF0000u : 0u);
-                    bad[i] = mask & 0x3C003C00u;
-                    clean[i] &= ~mask;
+                    const float x0 = (seen >> (2 * i)) & 1u ? s[2 * i] * (vs[2 * i][b] * f) : 0.0f;
+                    const float x1 = (seen >> (2 * i + 1)) & 1u ? s[2 * i + 1] * (vs[2 * i + 1][b] * f) : 0.0f;
+                    two_parts(x0, x1, h[b][i], l[b][i]);
                 }
-                const f32x4 hit = mfma(as_half8(bad), as_half8(w), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                st.acc[j] = mfma(as_half8(clean), as_half8(h), st.acc[j]);
-                st.acc[j] = mfma(as_half8(clean), as_half8(l), st.acc[j]);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (hit[i] > 0.0f) st.acc[j][i] = __builtin_nanf("");
-            }
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-            const half8 o = v.operand(j);
-            st.acc[j] = mfma(o, as_half8(h), st.acc[j]);
-            st.acc[j] = mfma(o, as_half8(l), st.acc[j]);
+            for (int i = 0; i < 4; ++i) two_parts(s[2 * i], s[2 * i + 1], h[0][i], l[0][i]);
         }
     }
+    __device__ __forceinline__ half8 first(int b) const { return as_half8(h[Q8 ? b : 0]); }
+    __device__ __forceinline__ half8 rest(int b) const { return as_half8(l[Q8 ? b : 0]); }
+    // acc += V' P' for an operand of V in scale block b
+    template <typename T>
+    __device__ __forceinline__ T add(half8 o, int b, T acc) const {
+        b = Q8 ? b : 0;
+        return mfma(o, as_half8(l[b]), mfma(o, as_half8(h[b]), acc));
+    }
+    // The same where V may hold infinities or NaN at keys that not every row
+    // sees: a weight of zero would make them NaN in every row.  They are taken
+    // out, and NaN goes to the outputs of the rows that see them.
+    __device__ __forceinline__ f32x4 add_odd(half8 o, uint32_t seen, f32x4 acc) const {
+        const uint4 v = __builtin_bit_cast(uint4, o);
+        uint32_t w[4], clean[4] = {v.x, v.y, v.z, v.w}, bad[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t mask = odd_mask(clean[i]);
+            bad[i] = mask & 0x3C003C00u;
+            clean[i] &= ~mask;
+            w[i] = ((seen >> (2 * i)) & 1u ? 0x3C00u : 0u) | ((seen >> (2 * i + 1)) & 1u ? 0x3C000000u : 0u);
+        }
+        const f32x4 hit = mfma(as_half8(bad), as_half8(w), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        acc = add(as_half8(clean), 0, acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = hit[i] == 0.0f ? acc[i] : __builtin_nanf("");
+        return acc;
+    }
+};
+
+// Which of N keys a row sees (bit i: the key with index at(i)); the products of
+// the others become -inf.
+template <int N, typename F>
+__device__ __forceinline__ uint32_t mask_keys(const Keys& K, const RowSight& see, float* s, F at) {
+    uint32_t seen = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int k = at(i);
+        const int row = cache_row(K, k);
+        const bool ok = (k < K.n) & ((row <= see.p) & ((row >= see.lo) | (row < K.sinks)));
+        s[i] = ok ? s[i] : -INFINITY;
+        seen |= ok ? 1u << i : 0u;
+    }
+    return seen;
+}
+
+// The largest value scale of the N keys that the row sees (those that are no
+// number of any use, infinite ones among them, make their weights infinite).
+template <int N, int D>
+__device__ __forceinline__ float top_scale(const float (&vs)[N][D / 64], uint32_t seen) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b) {
+            const float a = fabsf(vs[i][b]);
+            top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
+        }
+    return top;
 }
 
 // ------------------------------------------------- few rows: waves over keys
@@ -471,41 +562,79 @@ struct Step {
     VRaw<D, Q8> v;
     float ks[8][D / 64], vs[8][D / 64];
 
-    __device__ __forceinline__ void load_k(const Keys& K, int t, int lane) {
+    // Key i's row is at(i) rows past `first`; kFollow: at(i) = i, so that the
+    // addresses are one scalar and constants, and a lane's scales lie together.
+    template <bool kFollow, typename F>
+    __device__ __forceinline__ void k_rows(const Keys& K, size_t first, F at, int lane) {
+        constexpr int kBytes = Q8 ? 1 : 2;
         const int r = lane & 15, gq = lane >> 4;
+        const char* src = static_cast<const char*>(K.k) + first * (D * kBytes);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const size_t row = cache_row(K, min(t * kKeys + 16 * kt + r, K.n - 1));
+            const char* x = src + (at(16 * kt + r) * (D * kBytes) + 8 * gq * kBytes);
 #pragma unroll
             for (int s = 0; s < D / 32; ++s) {
                 if constexpr (Q8)
-                    k8[kt][s] = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(K.k) + row * D + 32 * s + 8 * gq);
+                    k8[kt][s] = *reinterpret_cast<const uint2*>(x + 32 * s);
                 else
-                    k16[kt][s] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(K.k) + row * D + 32 * s + 8 * gq);
+                    k16[kt][s] = *reinterpret_cast<const uint4*>(x + 64 * s);
             }
         }
-        if constexpr (Q8) {
+        if constexpr (Q8) scale_rows<kFollow>(K.ks, first, at, gq, ks);
+    }
+    template <bool kFollow, typename F>
+    __device__ __forceinline__ void v_rows(const Keys& K, size_t first, F at, int lane) {
+        constexpr int kBytes = Q8 ? 1 : 2;
+        const int r = lane & 15, gq = lane >> 4;
+        const char* src = static_cast<const char*>(K.v) + first * (D * kBytes);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const size_t row = cache_row(K, min(t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3), K.n - 1));
+        for (int i = 0; i < 8; ++i) v.load(src + at((i & 4) * 4 + 4 * gq + (i & 3)) * (D * kBytes), i, r);
+        if constexpr (Q8) scale_rows<kFollow>(K.vs, first, at, gq, vs);
+    }
+    // The scales of the lane's 8 keys.
+    template <bool kFollow, typename F>
+    __device__ __forceinline__ void scale_rows(const float* src, size_t first, F at, int gq, float (&dst)[8][D / 64]) {
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // a row's scales start anywhere
+        src += first * (D / 64);
+        if constexpr (kFollow) {
 #pragma unroll
-                for (int b = 0; b < D / 64; ++b) ks[i][b] = K.ks[row * (D / 64) + b];
-            }
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4 * (D / 64); i += 4) {
+                    const f4 x = *reinterpret_cast<const f4*>(src + (16 * h + 4 * gq) * (D / 64) + i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) dst[4 * h + (i + e) / (D / 64)][(i + e) % (D / 64)] = x[e];
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b) dst[i][b] = src[at((i & 4) * 4 + 4 * gq + (i & 3)) * (D / 64) + b];
         }
+    }
+    // Step t: where its rows do not follow each other (at a range's end) every
+    // row is looked up by itself.
+    __device__ __forceinline__ void load_k(const Keys& K, int t, int lane) {
+        const int i0 = t * kKeys;
+        if (rows_follow(K, i0))
+            k_rows<true>(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, lane);
+        else
+            k_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
     }
     __device__ __forceinline__ void load_v(const Keys& K, int t, int lane) {
-        const int r = lane & 15, gq = lane >> 4;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const size_t row = cache_row(K, min(t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3), K.n - 1));
-            v.load(K.v, i, row, r);
-            if constexpr (Q8) {
-#pragma unroll
-                for (int b = 0; b < D / 64; ++b) vs[i][b] = K.vs[row * (D / 64) + b];
-            }
-        }
+        const int i0 = t * kKeys;
+        if (rows_follow(K, i0))
+            v_rows<true>(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, lane);
+        else
+            v_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
     }
-    __device__ __forceinline__ void scores(const Query<D>& q, float (&s)[8]) const {
+    __device__ __forceinline__ half8 k_operand(int kt, int s) const {
+        if constexpr (Q8)
+            return codes_half8(k8[kt][s]);
+        else
+            return __builtin_bit_cast(half8, k16[kt][s]);
+    }
+    __device__ __forceinline__ void scores(const Query<D, 32>& q, float (&s)[8]) const {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             if constexpr (Q8) {
@@ -515,7 +644,7 @@ struct Step {
                     f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int x = 2 * b; x < 2 * b + 2; ++x) {
-                        const half8 k = codes_half8(k8[kt][x]);
+                        const half8 k = k_operand(kt, x);
                         a = mfma(k, q.hi[x], a);
                         a = mfma(k, q.lo[x], a);
                     }
@@ -528,7 +657,7 @@ struct Step {
                 f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int x = 0; x < D / 32; ++x) {
-                    const half8 k = __builtin_bit_cast(half8, k16[kt][x]);
+                    const half8 k = k_operand(kt, x);
                     a = mfma(k, q.hi[x], a);
                     a = mfma(k, q.lo[x], a);
                 }
@@ -540,7 +669,7 @@ struct Step {
 };
 
 template <int D, bool Q8>
-__device__ __forceinline__ void few_rows(const Keys& K, const Query<D>& q, const RowSight& see, int t0, int t1,
+__device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, const RowSight& see, int t0, int t1,
                                          int stride, int lane, State<D, Q8>& st) {
     if (t0 >= t1) return;
     const int gq = lane >> 4;
@@ -554,29 +683,21 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D>& q, const
         if (next < t1) x.load_k(K, next, lane);
         const bool all = all_seen(K, t * kKeys, kKeys);  // the same in every lane
         uint32_t seen = 0xFFu;
-        if (!all) {
-            seen = 0u;
+        if (!all) seen = mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
+        float top = 0.0f;
+        if constexpr (Q8) top = top_scale<8, D>(x.vs, seen);
+        st.step(s, q.c, top);
+        Weights<D, Q8> w;
+        w.cut(s, x.vs, seen, st.ev);
+        bool odd = false;
+        if constexpr (!Q8) odd = !all && __builtin_amdgcn_ballot_w64(x.v.odd()) != 0ull;
+        if (__builtin_expect(!odd, 1)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int at = t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3);
-                const int row = cache_row(K, at);
-                const bool ok = at < K.n && (!K.masked || (row <= see.p && (row >= see.lo || row < K.sinks)));
-                s[i] = ok ? s[i] : -INFINITY;
-                seen |= ok ? 1u << i : 0u;
-            }
+            for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add_odd(x.v.operand(j), seen, st.acc[j]);
         }
-        float vs_max = 0.0f;
-        if constexpr (Q8) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int b = 0; b < D / 64; ++b) {
-                    const float a = fabsf(x.vs[i][b]);
-                    vs_max = (seen >> i) & 1u && a < 1e30f ? fmaxf(vs_max, a) : vs_max;
-                }
-        }
-        st.weigh(s, q.c, vs_max);
-        add_values<D, Q8>(st, x.v, s, x.vs, seen, all);
         if (next < t1) x.load_v(K, next, lane);
     }
 }
@@ -596,22 +717,17 @@ __device__ __forceinline__ float share(float2 ml, float m) {
     return ml.y == 0.0f ? 0.0f : ml.y == ml.y ? exp2_fast(ml.x - m) : ml.y;
 }
 
-template <int D, bool Q8>
-__device__ __forceinline__ float out_scale(const State<D, Q8>& st) {
-    if constexpr (Q8) return pow2(min(max(st.ev, -126), 127));
-    return 1.0f;
-}
-
-template <int D, bool Q8>
-__device__ __forceinline__ void store_row(float* dst, const State<D, Q8>& st, int gq, float f) {
+// O' times f to a row of D floats; kBlocks: operand j's dims are code_dim's.
+template <int D, bool kBlocks>
+__device__ __forceinline__ void store_row(float* dst, const f32x4 (&acc)[D / 16], int gq, float f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = 4 * gq + i;
 #pragma unroll
         for (int j = 0; j < D / 16; j += 4) {
-            const int d = Q8 ? code_dim(r, j) : fp16_dim<D>(r, j);
+            const int d = kBlocks ? code_dim(r, j) : fp16_dim<D>(r, j);
             *reinterpret_cast<float4*>(dst + d) =
-                make_float4(st.acc[j][i] * f, st.acc[j + 1][i] * f, st.acc[j + 2][i] * f, st.acc[j + 3][i] * f);
+                make_float4(acc[j][i] * f, acc[j + 1][i] * f, acc[j + 2][i] * f, acc[j + 3][i] * f);
         }
     }
 }
@@ -630,18 +746,18 @@ struct RowMap {
 __device__ __forceinline__ RowSight sight(const Keys& K, long long p, int rows, int window) {
     RowSight s;
     s.any = !K.masked || (p >= 0 && p < rows);
-    s.p = s.any ? static_cast<int>(p) : -1;
-    s.lo = window > 0 ? s.p - window + 1 : 0;
+    s.p = !K.masked ? INT_MAX : s.any ? static_cast<int>(p) : -1;
+    s.lo = K.masked && window > 0 ? s.p - window + 1 : 0;
     return s;
 }
 
 template <int D, bool Q8>
 __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const RowMap& map, int row0, long long p0,
                                         int rows, int split, int splits, int slot, JoinArea<D, kFewWaves>& area) {
-    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
     const int n = row0 + (lane & 15), gq = lane >> 4;
     const bool real = n < map.total;
-    Query<D> q;
+    Query<D, 32> q;
     q.load(real ? g.q + map.at(n) * D : nullptr, gq, g.scale);
     const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
     State<D, Q8> st;
@@ -649,8 +765,8 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
     // a split's steps, a multiple of the waves'
     const int per = ((steps + splits - 1) / splits + kFewWaves - 1) / kFewWaves * kFewWaves;
     few_rows<D, Q8>(K, q, see, split * per + wave, min(steps, (split + 1) * per), kFewWaves, lane, st);
-    st.l = lanes16_sum(st.l);
-    store_row<D, Q8>(area.acc[wave][lane & 15], st, gq, out_scale(st));
+    st.l = lanes_sum<16>(st.l);
+    store_row<D, Q8>(area.acc[wave][lane & 15], st.acc, gq, st.out_scale());
     if (gq == 0) area.ml[wave][lane & 15] = make_float2(st.m, st.l);
     __syncthreads();
     constexpr int kPer = kRows * D / (kFewWaves * 64);  // values a thread: 8 (D 128) or 4
@@ -722,10 +838,373 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
     return K;
 }
 
+// ---------------------------------------------- many rows: waves over rows
+// A wave takes 32 query rows (columns of 32x32 tiles: half the operand reads a
+// product of 16x16 ones, and one lane exchange a step), the workgroup's four
+// waves share each 32 keys through LDS, where K and V lie as the operands are
+// read, 16 bytes a lane; int8 codes are turned into fp16 on the way.  Waves 0 and
+// 1 bring 64 dims of V each (turned in registers), waves 2 and 3 16 keys of K.
+// Two buffers: the next keys' loads run during a tile's products and are
+// written to the other buffer after them, one barrier a tile.
+//
+// A lane holds one row n = lane % 32 and, with h = lane / 32, the keys
+// wide_key(i, h) of a tile's score registers i = 0..15; operand step s of the
+// weighted values takes i = 8 s .. 8 s + 7.
+constexpr int kManyWaves = 4;
+constexpr int kWideRows = 32;
+
+__device__ __forceinline__ int wide_key(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// Operand row m of V's dim tile u is dim 64 (u / 2) + 4 (m % 16) + 2 (u % 2) + m / 16:
+// a lane that brings 4 neighbouring dims of 8 keys writes beside its neighbours.
+template <int D, bool Q8>
+struct Stage {
+    half8 k[D / 8][kKeys + 1];     // [8 dims][key]: the odd stride spreads a key's dims over the banks
+    half8 v[D / 32][2][2][32];     // [dim tile][step][h][m]
+    float ks[Q8 ? D / 64 : 1][Q8 ? kKeys : 4], vs[Q8 ? D / 64 : 1][Q8 ? kKeys : 4];
+    uint32_t odd[2];                             // fp16: the wave brought infinities or NaN, as bits j
+    uint8_t bad[Q8 ? 1 : kKeys][Q8 ? 4 : D / 4];  // of byte r of a key: dims 4 r + j, zero in v
+};
+
+// A wave's share of a tile on its way, 8 or 16 dwords.
+template <int D, bool Q8>
+struct Bring {
+    static constexpr int kV = Q8 ? 1 : 2;   // dwords of 4 dims of V
+    static constexpr int kK = Q8 ? 2 : 4;   // dwords of 8 dims of K
+    static constexpr int kLoads = D / 32;   // 16 keys of K
+    uint32_t w[8 * kV];
+    float scale;
+
+    // Key i of the 8 that lane group q = lane / 16 brings of V.
+    static __device__ __forceinline__ int v_key(int i, int q) {
+        return 16 * (q >> 1) + 4 * (q & 1) + 8 * (i >> 2) + (i & 3);
+    }
+    static __device__ __forceinline__ int k_key(int i, int wave, int lane) {
+        return 16 * (wave - 2) + (16 / kLoads) * i + lane / (D / 8);
+    }
+    // Key i's row is at(i) rows past `first`.
+    template <typename F>
+    __device__ __forceinline__ void load_rows(const Keys& K, size_t first, F at, int wave, int lane) {
+        constexpr int kBytes = Q8 ? 1 : 2;
+        if (wave < 2) {
+            if (wave < D / 64) {
+                const char* src = static_cast<const char*>(K.v) + first * (D * kBytes);
+                const int lane_at = (64 * wave + 4 * (lane & 15)) * kBytes;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const char* x = src + (at(v_key(i, lane >> 4)) * (D * kBytes) + lane_at);
+                    if constexpr (Q8) {
+                        w[i] = *reinterpret_cast<const uint32_t*>(x);
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(x);
+                        w[2 * i] = v.x;
+                        w[2 * i + 1] = v.y;
+                    }
+                }
+            }
+        } else {
+            const char* src = static_cast<const char*>(K.k) + first * (D * kBytes);
+            const int lane_at = 8 * (lane % (D / 8)) * kBytes;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const char* x = src + (at(k_key(i, wave, lane)) * (D * kBytes) + lane_at);
+                if constexpr (Q8) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(x);
+                    w[2 * i] = v.x;
+                    w[2 * i + 1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4*>(x);
+                    w[4 * i] = v.x;
+                    w[4 * i + 1] = v.y;
+                    w[4 * i + 2] = v.z;
+                    w[4 * i + 3] = v.w;
+                }
+            }
+        }
+        if constexpr (Q8) {
+            const int e = wave * 64 + lane;
+            if (e < 2 * kKeys * (D / 64)) {
+                const int i = e % (kKeys * (D / 64));
+                const float* src = (e < kKeys * (D / 64) ? K.ks : K.vs) + first * (D / 64);
+                scale = src[at(i / (D / 64)) * (D / 64) + i % (D / 64)];
+            }
+        }
+    }
+    // Tile t.  Where its rows follow each other its addresses are one scalar and
+    // constants; at a range's end every row is looked up by itself.
+    __device__ __forceinline__ void load(const Keys& K, int t, int wave, int lane) {
+        const int i0 = t * kKeys;
+        if (rows_follow(K, i0))
+            load_rows(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, wave, lane);
+        else
+            load_rows(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, wave, lane);
+    }
+    __device__ __forceinline__ void store(Stage<D, Q8>& s, int wave, int lane) {
+        if (wave < 2) {
+            if (wave < D / 64) {
+                const int q = lane >> 4;
+                if constexpr (!Q8) {
+                    uint32_t any = 0u;  // an exponent of all ones
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) any |= (w[i] & 0x7C007C00u) + 0x04000400u;
+                    const bool odd = __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0u) != 0ull;
+                    if (lane == 0) s.odd[wave] = odd ? 1u : 0u;
+                    if (odd) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t m0 = odd_mask(w[2 * i]), m1 = odd_mask(w[2 * i + 1]);
+                            s.bad[v_key(i, q)][16 * wave + (lane & 15)] =
+                                static_cast<uint8_t>((m0 & 1u) | (m0 >> 16 & 2u) | (m1 & 4u) | (m1 >> 16 & 8u));
+                            w[2 * i] &= ~m0;
+                            w[2 * i + 1] &= ~m1;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        if constexpr (Q8)
+                            o[p] = codes_half2(__builtin_amdgcn_perm(w[2 * p + 1], w[2 * p],
+                                                                     0x0C040C00u + 0x00010001u * static_cast<uint32_t>(j)));
+                        else
+                            o[p] = __builtin_amdgcn_perm(w[2 * (2 * p + 1) + (j >> 1)], w[2 * (2 * p) + (j >> 1)],
+                                                         (j & 1) ? 0x07060302u : 0x05040100u);
+                    }
+                    s.v[2 * wave + (j >> 1)][q >> 1][q & 1][16 * (j & 1) + (lane & 15)] = as_half8(o);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                half8 x;
+                if constexpr (Q8)
+                    x = codes_half8(make_uint2(w[2 * i], w[2 * i + 1]));
+                else
+                    x = __builtin_bit_cast(half8, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+                s.k[lane % (D / 8)][k_key(i, wave, lane)] = x;
+            }
+        }
+        if constexpr (Q8) {
+            const int e = wave * 64 + lane;
+            if (e < 2 * kKeys * (D / 64)) {
+                const int at = e % (kKeys * (D / 64));
+                (e < kKeys * (D / 64) ? s.ks : s.vs)[at % (D / 64)][at / (D / 64)] = scale;
+            }
+        }
+    }
+};
+
+template <int D, bool Q8>
+__device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const RowMap& map, int row0, long long p0,
+                                         int rows, int split, int splits, int slot, Stage<D, Q8> (&stage)[2]) {
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
+    const int n = row0 + wave * kWideRows + (lane & 31), h = lane >> 5;
+    const int tiles = (K.n + kKeys - 1) / kKeys;
+    const int per = (tiles + splits - 1) / splits;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
+    Query<D, 16> q;
+    q.load(n < map.total ? g.q + map.at(n) * D : nullptr, h, g.scale);
+    const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
+    Softmax<false, 32> st;
+    f32x16 acc[D / 32];
+    // int8: the power of two that keeps the wave's weights times value scales in
+    // fp16's range (acc is 2^-ev times O'), and the rows that any of its rows sees
+    int ev = -126, p_top = INT_MAX, lo_low = 0;
+    if (Q8 && K.masked) {
+        p_top = n < map.total ? see.p : -1;
+        lo_low = n < map.total && see.any ? see.lo : INT_MAX;
+#pragma unroll
+        for (int x = 16; x >= 1; x >>= 1) {
+            p_top = max(p_top, __shfl_xor(p_top, x, kWave));
+            lo_low = min(lo_low, __shfl_xor(lo_low, x, kWave));
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
+    // Values that are infinite or NaN are zero in the products (times the zero
+    // weight of a row that does not see them they would be NaN); the dims
+    // where the row sees one are kept here and become NaN at the end.
+    uint32_t bad[Q8 ? 1 : D / 16] = {};
+    Bring<D, Q8> next;
+    if (t0 < t1) {
+        next.load(K, t0, wave, lane);
+        next.store(stage[0], wave, lane);
+    }
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        const Stage<D, Q8>& s = stage[(t - t0) & 1];
+        half8 o[D / 16];  // the tile's K operands, then V's
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x) o[x] = s.k[2 * x + h][lane & 31];
+        if (t + 1 < t1) next.load(K, t + 1, wave, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        float p[16];
+#pragma unroll
+        for (int b = 0; b < (Q8 ? D / 64 : 1); ++b) {
+            f32x16 a;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a[i] = 0.0f;
+#pragma unroll
+            for (int x = b * 4; x < (Q8 ? b * 4 + 4 : D / 16); ++x) {
+                a = mfma(o[x], q.hi[x], a);
+                a = mfma(o[x], q.lo[x], a);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                if constexpr (Q8) {
+                    const float4 sc = *reinterpret_cast<const float4*>(&s.ks[b][wide_key(i, h)]);
+                    p[i] = b ? fmaf(a[i], sc.x, p[i]) : a[i] * sc.x;
+                    p[i + 1] = b ? fmaf(a[i + 1], sc.y, p[i + 1]) : a[i + 1] * sc.y;
+                    p[i + 2] = b ? fmaf(a[i + 2], sc.z, p[i + 2]) : a[i + 2] * sc.z;
+                    p[i + 3] = b ? fmaf(a[i + 3], sc.w, p[i + 3]) : a[i + 3] * sc.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) p[i + e] = a[i + e];
+                }
+            }
+        }
+        constexpr bool kBoth = !Q8 || D == 64;  // registers for both of V's steps
+#pragma unroll
+        for (int u = 0; u < (kBoth ? D / 16 : D / 32); ++u) o[u] = s.v[u % (D / 32)][u / (D / 32)][h][lane & 31];
+        __builtin_amdgcn_sched_barrier(0);
+        const bool all = all_seen(K, t * kKeys, kKeys);
+        uint32_t seen = 0xFFFFu;
+        if (!all) seen = mask_keys<16>(K, see, p, [&](int i) { return t * kKeys + wide_key(i, h); });
+        float high;
+        if (st.rises(p, q.c, 0.0f, high)) {
+            const float alpha = st.rebase(high, 0.0f);
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) acc[u] *= alpha;
+        }
+        if constexpr (Q8) {
+            // A value scale a lane.  One that no row of the wave sees may be anything;
+            // one that is no number of any use makes its weights infinite.
+            const int key = lane / (D / 64) % kKeys, i = t * kKeys + key, row = cache_row(K, i);
+            const float a = fabsf(s.vs[lane % (D / 64)][key]);
+            const bool ok = (i < K.n) & (a < 1e30f) & (row <= p_top) & ((row >= lo_low) | (row < K.sinks));
+            if (__builtin_amdgcn_ballot_w64(ok & (exponent(a) > ev)) != 0ull) {
+                float top = ok ? a : 0.0f;
+#pragma unroll
+                for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
+                const int e1 = max(ev, uniform(exponent(top)));
+                const float f = pow2(max(ev - e1, -126));
+#pragma unroll
+                for (int u = 0; u < D / 32; ++u) acc[u] *= f;
+                ev = e1;
+            }
+        }
+        st.weigh(p, q.c);
+        Weights<D, Q8> w;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (!kBoth && e) {
+#pragma unroll
+                for (int u = 0; u < D / 32; ++u) o[u] = s.v[u][1][h][lane & 31];
+            }
+            float vs[8][D / 64];
+            if constexpr (Q8) {
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 4) {
+                        const float4 sc = *reinterpret_cast<const float4*>(&s.vs[b][wide_key(8 * e + i, h)]);
+                        vs[i][b] = sc.x;
+                        vs[i + 1][b] = sc.y;
+                        vs[i + 2][b] = sc.z;
+                        vs[i + 3][b] = sc.w;
+                    }
+            }
+            w.cut(p + 8 * e, vs, seen >> (8 * e), ev);
+            const half8* v = &o[kBoth ? e * (D / 32) : 0];
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) acc[u] = mfma(v[u], w.first(u >> 1), acc[u]);
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u) acc[u] = mfma(v[u], w.rest(u >> 1), acc[u]);
+        }
+        if constexpr (!Q8) {
+            if (uniform(static_cast<int>(s.odd[0] | s.odd[D / 64 - 1])) != 0) {
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b)
+                    if (s.odd[b] != 0u) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i)
+#pragma unroll
+                            for (int e = 4 * b; e < 4 * b + 4; ++e)
+                                bad[e] |= (seen >> i) & 1u
+                                              ? *reinterpret_cast<const uint32_t*>(&s.bad[wide_key(i, h)][4 * e]) : 0u;
+                    }
+            }
+        }
+        if (t + 1 < t1) next.store(stage[(t + 1 - t0) & 1], wave, lane);
+    }
+    const float l = lanes_sum<32>(st.l);
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) bad[e] |= __shfl_xor(bad[e], 32, kWave);
+    }
+    if (n >= map.total) return;
+    const long long at = map.at(n);
+    float f = Q8 ? pow2(max(ev, -126)) : 1.0f;
+    float* dst;
+    if (g.slots == 1) {
+        const bool any = see.any && l != 0.0f;
+        f = any ? f / l : 0.0f;
+        if (!any) {
+#pragma unroll
+            for (int u = 0; u < D / 32; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
+        }
+        dst = g.out + at * D;
+    } else {
+        if (h == 0) g.ml[at * g.slots + slot] = make_float2(st.m, l);
+        if (l == 0.0f) return;
+        dst = g.part + (at * g.slots + slot) * D;
+    }
+#pragma unroll
+    for (int u = 0; u < D / 32; u += 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float4 o = make_float4(acc[u][i] * f, acc[u][i + 8] * f, acc[u + 1][i] * f, acc[u + 1][i + 8] * f);
+            if constexpr (!Q8) {
+                const uint32_t x = (h ? bad[2 * u + 2 * (i >> 2) + 1] : bad[2 * u + 2 * (i >> 2)]) >> (8 * (i & 3));
+                const float nan = __builtin_nanf("");
+                o = make_float4(x & 1u ? nan : o.x, x & 2u ? nan : o.y, x & 4u ? nan : o.z, x & 8u ? nan : o.w);
+            }
+            *reinterpret_cast<float4*>(dst + 32 * u + 4 * wide_key(i, h)) = o;
+        }
+}
+
+// Row tiles from the last one down: with no window its tokens see the most.
+template <int D, bool Q8>
+__global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const AttnArgs g) {
+    __shared__ Stage<D, Q8> stage[2];
+    constexpr int kWgRows = kManyWaves * kWideRows;
+    const int group = g.n_heads / g.n_kv;
+    const int total = g.n_tokens * group;
+    const int tiles = (total + kWgRows - 1) / kWgRows;
+    int b = static_cast<int>(blockIdx.x);
+    const int kvh = b % g.n_kv;
+    b /= g.n_kv;
+    const int split = b % g.splits;
+    b /= g.splits;
+    const int row0 = (tiles - 1 - b % tiles) * kWgRows;
+    const int seq = b / tiles;
+    const RowMap map{static_cast<long long>(seq) * g.n_tokens * g.n_heads + static_cast<long long>(kvh) * group, group,
+                     g.n_heads, total};
+    const Keys K = window_keys<D, Q8>(g, seq, kvh, row0 / group, (min(row0 + kWgRows, total) - 1) / group + 1);
+    many_job<D, Q8>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, stage);
+}
+
+// ------------------------------------------------------- few rows: kernels
 // blockIdx.x = ((sequence * row tiles + tile) * splits + split) * n_kv + kv head:
 // with 8 KV heads one head's workgroups share an XCD's L2.
 template <int D, bool Q8>
-__global__ __launch_bounds__(kFewWaves * 64) void window_few_kernel(const AttnArgs g) {
+__global__ __launch_bounds__(kFewWaves * 64, 2) void window_few_kernel(const AttnArgs g) {
     __shared__ JoinArea<D, kFewWaves> area;
     const int group = g.n_heads / g.n_kv;
     const int total = g.n_tokens * group;
@@ -743,24 +1222,34 @@ __global__ __launch_bounds__(kFewWaves * 64) void window_few_kernel(const AttnAr
     few_job<D, Q8>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, area);
 }
 
-// Shared prefix: the first jobs take 16 (sequence, head) rows of a KV head and a
-// split of the prefix, the others a sequence's own keys.
-template <int D, bool Q8>
-__global__ __launch_bounds__(kFewWaves * 64) void prefix_few_kernel(const AttnArgs g, int prefix_splits, int jobs) {
-    __shared__ JoinArea<D, kFewWaves> area;
+// Shared prefix: the first `jobs` workgroups take rows of a KV head, 16 or 128
+// of all sequences' (sequence, head) rows, and a split of the prefix, the others
+// a sequence's own keys.
+template <int D, bool Q8, bool kMany>
+__global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArgs g, int prefix_splits, int jobs) {
+    static_assert(kFewWaves == kManyWaves, "one workgroup size");
+    constexpr int kWgRows = kMany ? kManyWaves * kWideRows : kRows;
+    __shared__ union Lds {
+        JoinArea<D, kFewWaves> area;
+        Stage<D, Q8> stage[kMany ? 2 : 1];
+        __device__ Lds() {}
+    } lds;
     const int group = g.n_heads / g.n_kv;
     int b = static_cast<int>(blockIdx.x);
     if (b < jobs) {
         const int total = g.n_seq * group;
-        const int tiles = (total + kRows - 1) / kRows;
+        const int tiles = (total + kWgRows - 1) / kWgRows;
         const int kvh = b % g.n_kv;
         b /= g.n_kv;
-        const int row0 = b % tiles * kRows;
+        const int row0 = b % tiles * kWgRows;
         const int split = b / tiles;
         const RowMap map{static_cast<long long>(kvh) * group, group, g.n_heads, total};
         Keys K = head_keys<D, Q8>(g.a, kvh, g.rows_a);
         K.n = g.prefix;
-        few_job<D, Q8>(g, K, map, row0, 0, 0, split, prefix_splits, split, area);
+        if constexpr (kMany)
+            many_job<D, Q8>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.stage);
+        else
+            few_job<D, Q8>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.area);
         return;
     }
     b -= jobs;
@@ -777,7 +1266,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void prefix_few_kernel(const AttnAr
     Keys K = head_keys<D, Q8>(g.b, static_cast<long long>(seq) * g.n_kv + kvh, g.rows_b);
     const int p = g.pos[seq];
     K.n = p >= 0 && p < g.rows_b ? p + 1 : 0;
-    few_job<D, Q8>(g, K, map, row0, 0, 0, split, own_splits, prefix_splits + split, area);
+    few_job<D, Q8>(g, K, map, row0, 0, 0, split, own_splits, prefix_splits + split, lds.area);
 }
 
 // One wave per query row: its partials in slot order.
@@ -800,19 +1289,42 @@ __global__ __launch_bounds__(kJoinRows * 64) void attention_join_kernel(const At
     float l = ml.y * w;
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, kWave);
+    // Slots with keys, four at a time: their loads are independent.
     float acc[D / 64] = {};
     const float* part = g.part + row * g.slots * D + lane * (D / 64);
-    for (int s = 0; s < g.slots; ++s) {
-        const float ws = __shfl(w, s, kWave);
-        if (ws == 0.0f) continue;  // the same in every lane
+    uint64_t left = __builtin_amdgcn_ballot_w64(w != 0.0f);
+    while (left != 0ull) {
+        int s[4];
+        float ws[4], x[4][D / 64];
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) acc[i] = fmaf(part[s * D + i], ws, acc[i]);
+        for (int i = 0; i < 4; ++i) {
+            s[i] = left != 0ull ? __builtin_ctzll(left) : s[0];
+            ws[i] = left != 0ull ? __shfl(w, s[i], kWave) : 0.0f;
+            left &= left - 1;
+#pragma unroll
+            for (int e = 0; e < D / 64; ++e) x[i][e] = part[s[i] * D + e];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (ws[i] != 0.0f) {
+#pragma unroll
+                for (int e = 0; e < D / 64; ++e) acc[e] = fmaf(x[i][e], ws[i], acc[e]);
+            }
     }
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) g.out[row * D + lane * (D / 64) + i] = any && l != 0.0f ? acc[i] / l : 0.0f;
 }
 
 // ------------------------------------------------------------- host checks
+// f(head_dim, int8) as compile-time constants.
+template <typename F>
+asdsl_status with_form(int head_dim, bool q8, F f) {
+    using std::integral_constant;
+    if (head_dim == 128)
+        return q8 ? f(integral_constant<int, 128>{}, std::true_type{}) : f(integral_constant<int, 128>{}, std::false_type{});
+    return q8 ? f(integral_constant<int, 64>{}, std::true_type{}) : f(integral_constant<int, 64>{}, std::false_type{});
+}
+
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 asdsl_status check_heads(const char* what, int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
@@ -841,32 +1353,66 @@ asdsl_status append(const char* what, bool q8, const float* qkv, void* k, void* 
                     "%s: rows and rope_rows must be positive, pos_offset not negative", what);
     ASDSL_CHECK_ARG(aligned16(qkv) && aligned16(k) && aligned16(v) && aligned16(q_out),
                     "%s: qkv, caches and q_out must be 16-byte aligned", what);
-    AppendArgs a{qkv, k, v, ks, vs, rope_cos, rope_sin, pos, q_out, n_tokens, n_heads, n_kv_heads, rotary_dim / 2,
-                 rows, pos_offset, rope_rows, 0};
-    a.units = static_cast<long long>(n_seq) * n_tokens * (n_heads + 2 * n_kv_heads) * (head_dim / 8);
-    auto kern = head_dim == 128 ? (q8 ? kv_append_kernel<128, true> : kv_append_kernel<128, false>)
-                                : (q8 ? kv_append_kernel<64, true> : kv_append_kernel<64, false>);
-    return launch("kv_append_kernel", kern, dim3(static_cast<unsigned>((a.units + 255) / 256)), dim3(256), 0,
-                  as_hip(stream), a);
+    const int chunks = ((n_heads + 2 * n_kv_heads) * (head_dim / 4) + kAppendThreads - 1) / kAppendThreads;
+    const long long grid = static_cast<long long>(n_seq) * n_tokens * chunks;
+    ASDSL_CHECK_ARG(grid <= INT_MAX, "%s: n_seq * n_tokens * heads exceeds 2^31", what);
+    const AppendArgs a{qkv, k, v, ks, vs, rope_cos, rope_sin, pos, q_out, n_tokens, n_heads, n_kv_heads,
+                       rotary_dim / 2, rows, pos_offset, rope_rows, chunks};
+    const bool vec = rotary_dim % 8 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
+    return with_form(head_dim, q8, [&](auto dim, auto codes) {
+        constexpr int kD = decltype(dim)::value;
+        constexpr bool kQ8 = decltype(codes)::value;
+        return launch("kv_append_kernel", vec ? kv_append_kernel<kD, kQ8, true> : kv_append_kernel<kD, kQ8, false>,
+                      dim3(static_cast<unsigned>(grid)), dim3(kAppendThreads), 0, as_hip(stream), a);
+    });
 }
 
-// Workgroups that fill the device (256 compute units), and how many key splits
-// get a launch of `jobs` workgroups there when each split keeps at least
-// `least` of at most n keys.
-constexpr long long kFill = 512;
+// How many key splits get a launch of `jobs` workgroups to `fill` of them when
+// each split keeps at least kLeastKeys of at most n keys.
+constexpr int kLeastKeys = kFewWaves * kKeys;
 
-int splits_for(long long jobs, long long n, int least, int most) {
-    long long s = (kFill + jobs - 1) / jobs;
-    const long long by_keys = (n + least - 1) / least;
+int splits_for(long long fill, long long jobs, long long n, int most) {
+    long long s = (fill + jobs - 1) / jobs;
+    const long long by_keys = (n + kLeastKeys - 1) / kLeastKeys;
     s = s < by_keys ? s : by_keys;
     s = s < most ? s : most;
     return s > 1 ? static_cast<int>(s) : 1;
 }
 
+// Which form takes `total` rows of each of `heads` KV heads over at most n keys.
+// The few-rows form reads the keys once per 16 rows and streams better, the
+// many-rows form once per 128.  us a call in a graph, few / many rows, 8 KV
+// heads of 128 dims, by total x keys: 12 x 1000 10.2 / 13.5, 96 x 1000 14.2 /
+// 17.1, 24 x 8000 20.5 / 23.0, 33 x 8000 28.5 / 24.2, 66 x 8000 31.7 / 29.2; of
+// 16 sequences 12 x 2000 27.2 / 35.5, 18 x 2000 42.4 / 35.8.  64 dims, where
+// more of its waves fit a compute unit: 192 x 1000 11.8 / 14.9, 129 x 8000 27.4 /
+// 28.6, 192 x 8000 34.8 / 31.4.  So it goes by the few-rows form's steps.
+bool takes_many(long long total, long long heads, long long n, int head_dim) {
+    if (total <= kRows) return false;
+    const long long tiles = (total + kRows - 1) / kRows;
+    return tiles * heads * ((n + kLeastKeys - 1) / kLeastKeys) > (head_dim == 128 ? 1024 : 6144);
+}
+
+// Workgroups a launch is split up to: two a compute unit.  The many-rows form's
+// partials are 16 times as large a job, so it is split to one a compute unit
+// where those of two would come to a quarter of the keys' bytes (2068 rows over
+// 1000 keys, 4 KV heads: 31 us, 41 with two; 16 sequences of 18 rows over 2000
+// keys, 8 KV heads: 48 us, 36 with two).
+constexpr long long kFillFew = 512;
+
+long long fill_many(long long jobs, long long rows, long long heads, long long n) {
+    const long long splits = splits_for(kFillFew, jobs, n, kMaxSlots);
+    return rows * splits * 4 <= heads * n ? kFillFew : kFillFew / 2;
+}
+
 // How a call is laid out; the same for the work buffer's size and the launch.
 struct Plan {
+    bool many;          // the many-rows form
     int splits;         // of the window's keys, or of the prefix
     int slots;          // partials a query row (1: none kept)
+    int wg_rows;        // query rows of a workgroup
+    long long jobs;     // workgroups
+    long long own_jobs; // and those of the sequences' own keys behind a prefix
     size_t rows, work;  // query rows, bytes
 };
 
@@ -885,8 +1431,13 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, i
     long long n = rows;
     if (window > 0 && static_cast<long long>(window) + sinks + n_tokens - 1 < n)
         n = static_cast<long long>(window) + sinks + n_tokens - 1;
-    const long long tiles = (static_cast<long long>(n_tokens) * (n_heads / n_kv) + kRows - 1) / kRows;
-    p.splits = p.slots = splits_for(n_seq * tiles * n_kv, n, kFewWaves * kKeys, kMaxSlots);
+    const long long total = static_cast<long long>(n_tokens) * (n_heads / n_kv);
+    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, n, head_dim);
+    p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
+    p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
+    p.splits = p.slots = splits_for(
+        p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n) : kFillFew, p.jobs, n, kMaxSlots);
+    p.jobs *= p.splits;
     return finish(p, head_dim);
 }
 
@@ -894,10 +1445,18 @@ Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, int prefix_len,
     Plan p{};
     p.rows = static_cast<size_t>(n_seq) * n_heads;
     const int group = n_heads / n_kv;
-    const long long tiles = (static_cast<long long>(n_seq) * group + kRows - 1) / kRows;
-    const long long own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
-    p.splits = prefix_len > 0 ? splits_for(tiles * n_kv, prefix_len, kFewWaves * kKeys, kMaxSlots / 2) : 0;
-    p.slots = p.splits + splits_for(own_jobs, own_rows, kFewWaves * kKeys, kMaxSlots / 2);
+    const long long total = static_cast<long long>(n_seq) * group;
+    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim);
+    p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
+    p.own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
+    const int own_splits = splits_for(kFillFew, p.own_jobs, own_rows, kMaxSlots / 4);
+    const long long jobs = (total + p.wg_rows - 1) / p.wg_rows * n_kv;
+    if (prefix_len > 0)
+        p.splits = splits_for(p.many ? fill_many(jobs, p.rows, n_kv, prefix_len) : kFillFew, jobs, prefix_len,
+                              kMaxSlots - own_splits);
+    p.jobs = jobs * p.splits;
+    p.own_jobs *= own_splits;
+    p.slots = p.splits + own_splits;
     return finish(p, head_dim);
 }
 
@@ -939,13 +1498,18 @@ asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, c
     AttnArgs g{q, out, nullptr, nullptr, c, c, pos, n_seq, n_tokens, n_heads, n_kv_heads, rows, rows, -1, window,
                sinks, p.splits, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    const long long tiles = (static_cast<long long>(n_tokens) * (n_heads / n_kv_heads) + kRows - 1) / kRows;
-    const long long grid = n_seq * tiles * p.splits * n_kv_heads;
-    ASDSL_CHECK_ARG(grid <= INT_MAX, "%s: too many query rows", what);
-    auto kern = head_dim == 128 ? (q8 ? window_few_kernel<128, true> : window_few_kernel<128, false>)
-                                : (q8 ? window_few_kernel<64, true> : window_few_kernel<64, false>);
-    st = launch("window_few_kernel", kern, dim3(static_cast<unsigned>(grid)), dim3(kFewWaves * 64), 0, as_hip(stream),
-                g);
+    ASDSL_CHECK_ARG(p.jobs <= INT_MAX, "%s: too many query rows", what);
+    const dim3 grid(static_cast<unsigned>(p.jobs));
+    auto with = [&](auto dim, auto codes) {
+        constexpr int kD = decltype(dim)::value;
+        constexpr bool kQ8 = decltype(codes)::value;
+        if (!p.many)
+            return launch("window_few_kernel", window_few_kernel<kD, kQ8>, grid, dim3(kFewWaves * 64), 0,
+                          as_hip(stream), g);
+        return launch("window_many_kernel", window_many_kernel<kD, kQ8>, grid, dim3(kManyWaves * 64), 0,
+                      as_hip(stream), g);
+    };
+    st = with_form(head_dim, q8, with);
     return st != ASDSL_OK ? st : join(g, p, head_dim, stream);
 }
 
@@ -971,15 +1535,14 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
     AttnArgs g{q, out, nullptr, nullptr, shared, own, own_pos, n_seq, 1, n_heads, n_kv_heads, prefix_rows, own_rows,
                prefix_len, 0, 0, 0, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    const int group = n_heads / n_kv_heads;
-    const long long jobs = (static_cast<long long>(n_seq) * group + kRows - 1) / kRows * p.splits * n_kv_heads;
-    const long long own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * (p.slots - p.splits) *
-                               n_kv_heads;
-    ASDSL_CHECK_ARG(jobs + own_jobs <= INT_MAX, "%s: too many query rows", what);
-    auto kern = head_dim == 128 ? (q8 ? prefix_few_kernel<128, true> : prefix_few_kernel<128, false>)
-                                : (q8 ? prefix_few_kernel<64, true> : prefix_few_kernel<64, false>);
-    st = launch("prefix_few_kernel", kern, dim3(static_cast<unsigned>(jobs + own_jobs)), dim3(kFewWaves * 64), 0,
-                as_hip(stream), g, p.splits, static_cast<int>(jobs));
+    ASDSL_CHECK_ARG(p.jobs + p.own_jobs <= INT_MAX, "%s: too many query rows", what);
+    st = with_form(head_dim, q8, [&](auto dim, auto codes) {
+        constexpr int kD = decltype(dim)::value;
+        constexpr bool kQ8 = decltype(codes)::value;
+        return launch("prefix_kernel", p.many ? prefix_kernel<kD, kQ8, true> : prefix_kernel<kD, kQ8, false>,
+                      dim3(static_cast<unsigned>(p.jobs + p.own_jobs)), dim3(kFewWaves * 64), 0, as_hip(stream), g,
+                      p.splits, static_cast<int>(p.jobs));
+    });
     return st != ASDSL_OK ? st : join(g, p, head_dim, stream);
 }
 

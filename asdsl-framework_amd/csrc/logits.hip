@@ -14,7 +14,6 @@
 namespace asdsl {
 namespace {
 
-constexpr int kSlice = 4096;    // tokens of one workgroup
 constexpr int kThreads = 256;
 constexpr uint32_t kSeen = 0x80000000u;  // a slice's word per token: seen, and the count past the prompt
 
@@ -34,27 +33,57 @@ struct ControlArgs {
     long long bias_stride, allowed_stride;
 };
 
-// The slice's words are counted in LDS from the row's whole history (integer
-// atomics: any order gives the same), then its logits pass through once.
+// A workgroup takes kPer tokens a thread of one row.  Their logits are requested
+// first; while they come, the slice's words are counted in LDS from the row's
+// whole history (integer atomics: any order gives the same).  kVec: the rows of
+// logits, out and bias lie in whole 16-byte units.
+template <int kPer, bool kVec>
 __global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlArgs a) {
 #pragma clang fp contract(off)  // each step of the definition rounds by itself
-    __shared__ uint32_t word[kSlice];
+    constexpr int kSlice = kThreads * kPer;
+    constexpr int kWide = kVec ? 4 : 1;  // tokens of one load
+    __shared__ __align__(16) uint32_t word[kSlice];
     __shared__ unsigned long long red[kThreads / kWave];
     const int tid = static_cast<int>(threadIdx.x);
     const int row = static_cast<int>(blockIdx.x / a.slices);
-    const int slice = static_cast<int>(blockIdx.x % a.slices);
-    const int v0 = slice * kSlice;
+    const int v0 = static_cast<int>(blockIdx.x % a.slices) * kSlice;
     const int n = min(kSlice, a.vocab - v0);
+    const long long base = static_cast<long long>(row) * a.vocab + v0;
+    const float* bias = a.bias ? a.bias + row * a.bias_stride + v0 : nullptr;
+    const uint32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
+    float y[kPer], b[kPer];
+    uint32_t mask[kPer / kWide];
+#pragma unroll
+    for (int i = 0; i < kPer / kWide; ++i) {
+        const int at = (i * kThreads + tid) * kWide;
+        mask[i] = ~0u;
+        if (at >= n) continue;
+        if constexpr (kVec) {
+            const float4 x = *reinterpret_cast<const float4*>(a.logits + base + at);
+            y[4 * i] = x.x; y[4 * i + 1] = x.y; y[4 * i + 2] = x.z; y[4 * i + 3] = x.w;
+            if (bias) {
+                const float4 z = *reinterpret_cast<const float4*>(bias + at);
+                b[4 * i] = z.x; b[4 * i + 1] = z.y; b[4 * i + 2] = z.z; b[4 * i + 3] = z.w;
+            }
+        } else {
+            y[i] = a.logits[base + at];
+            if (bias) b[i] = bias[at];
+        }
+        if (allowed) mask[i] = allowed[(v0 + at) >> 5] >> ((v0 + at) & 31);
+    }
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (a.history) {
-        for (int i = tid; i < kSlice; i += kThreads) word[i] = 0u;
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4)
+            *reinterpret_cast<uint4*>(word + (i * kThreads + 4 * tid)) = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
         const int told = min(max(a.history_len ? a.history_len[row] : a.cap, 0), a.cap);
         const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
         const int* ids = a.history + static_cast<long long>(row) * a.cap;
         for (int i = tid; i < told; i += kThreads) {
-            const uint32_t at = static_cast<uint32_t>(ids[i]) - static_cast<uint32_t>(v0);
-            if (ids[i] >= 0 && at < static_cast<uint32_t>(n)) {
+            const int id = ids[i];
+            const uint32_t at = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
+            if (id >= 0 && at < static_cast<uint32_t>(n)) {
                 atomicOr(&word[at], kSeen);
                 if (i >= prompt) atomicAdd(&word[at], 1u);
             }
@@ -64,29 +93,42 @@ __global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlA
         if (a.presence) pres = a.presence[row];
         __syncthreads();
     }
-    const long long base = static_cast<long long>(row) * a.vocab + v0;
-    const float* bias = a.bias ? a.bias + row * a.bias_stride + v0 : nullptr;
-    const uint32_t* allowed = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-    unsigned long long best = 0ull;
-    for (int i = tid; i < n; i += kThreads) {
-        float y = a.logits[base + i];
-        const uint32_t w = a.history ? word[i] : 0u;
-        if (w != 0u) {
-            y = y > 0.0f ? y / rep : y * rep;
-            const uint32_t c = w & ~kSeen;
-            y = y - freq * static_cast<float>(c);
-            if (c != 0u) y = y - pres;
+    // A thread meets its tokens in rising order: only a larger one replaces the best.
+    float top = -INFINITY;
+    int top_at = -1;
+#pragma unroll
+    for (int i = 0; i < kPer / kWide; ++i) {
+        const int at = (i * kThreads + tid) * kWide;
+        if (at >= n) continue;
+        uint32_t w[kWide];
+#pragma unroll
+        for (int e = 0; e < kWide; ++e) w[e] = a.history ? word[at + e] : 0u;
+#pragma unroll
+        for (int e = 0; e < kWide; ++e) {
+            float x = y[kWide * i + e];
+            if (w[e] != 0u) {
+                x = x > 0.0f ? x / rep : x * rep;
+                const uint32_t c = w[e] & ~kSeen;
+                x = x - freq * static_cast<float>(c);
+                if (c != 0u) x = x - pres;
+            }
+            if (bias) x = x + b[kWide * i + e];
+            const bool ok = ((mask[i] >> e) & 1u) != 0u;
+            y[kWide * i + e] = ok ? x : -INFINITY;
+            if (ok & ((x > top) | ((top_at < 0) & (x == x)))) {
+                top = x;
+                top_at = at + e;
+            }
         }
-        if (bias) y = y + bias[i];
-        const int v = v0 + i;
-        const bool ok = !allowed || ((allowed[v >> 5] >> (v & 31)) & 1u) != 0u;
-        a.out[base + i] = ok ? y : -INFINITY;
-        if (ok && y == y) {
-            const unsigned long long k = argmax_key(y == 0.0f ? 0.0f : y, v);
-            best = k > best ? k : best;
-        }
+        if constexpr (kVec)
+            *reinterpret_cast<float4*>(a.out + base + at) =
+                make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        else
+            a.out[base + at] = y[i];
     }
     if (!a.keys) return;
+    // equal values of either sign of zero are one
+    unsigned long long best = top_at < 0 ? 0ull : argmax_key(top == 0.0f ? 0.0f : top, v0 + top_at);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) {
         const unsigned long long other = __shfl_xor(best, o, kWave);
@@ -117,7 +159,15 @@ __global__ __launch_bounds__(kWave) void logits_token_kernel(const unsigned long
         tokens[blockIdx.x] = best != 0ull ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
 }
 
-int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+// Tokens a thread: 16, or 4 where 16 leave compute units without a workgroup.
+int per_thread(int n_rows, int vocab) {
+    const long long slices = (vocab + 16LL * kThreads - 1) / (16 * kThreads);
+    return n_rows * slices < 256 ? 4 : 16;
+}
+long long slices_of(int n_rows, int vocab) {
+    const long long slice = static_cast<long long>(per_thread(n_rows, vocab)) * kThreads;
+    return (vocab + slice - 1) / slice;
+}
 
 }  // namespace
 }  // namespace asdsl
@@ -126,7 +176,7 @@ using namespace asdsl;
 
 extern "C" size_t asdsl_logits_control_work_bytes(int n_rows, int vocab) {
     if (n_rows <= 0 || vocab <= 0) return 0;
-    return (static_cast<size_t>(n_rows) * slices_of(vocab) * sizeof(unsigned long long) + 255) / 256 * 256;
+    return (static_cast<size_t>(n_rows) * slices_of(n_rows, vocab) * sizeof(unsigned long long) + 255) / 256 * 256;
 }
 
 extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, const int* history,
@@ -145,7 +195,7 @@ extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, in
                     "%s: bias_stride must be 0 or at least vocab", what);
     ASDSL_CHECK_ARG(!allowed || allowed_stride == 0 || allowed_stride >= (vocab + 31LL) / 32,
                     "%s: allowed_stride must be 0 or at least (vocab + 31) / 32", what);
-    ASDSL_CHECK_ARG(static_cast<long long>(n_rows) * slices_of(vocab) <= INT_MAX, "%s: too many rows", what);
+    ASDSL_CHECK_ARG(n_rows * slices_of(n_rows, vocab) <= INT_MAX, "%s: too many rows", what);
     void* ws = nullptr;
     if (tokens) {
         ASDSL_CHECK_ARG(work, "%s: tokens need a work buffer", what);
@@ -153,12 +203,17 @@ extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, in
                                             asdsl_logits_control_work_bytes(n_rows, vocab), &ws, what);
         if (st != ASDSL_OK) return st;
     }
-    const int slices = slices_of(vocab);
+    const int slices = static_cast<int>(slices_of(n_rows, vocab));
     const ControlArgs a{logits, out, static_cast<unsigned long long*>(ws), history_cap > 0 ? history : nullptr,
                         prompt_len, history_len, repetition, frequency, presence, bias, allowed, history_cap, vocab,
                         slices, bias_stride, allowed_stride};
-    asdsl_status st = launch("logits_control_kernel", logits_control_kernel, dim3(static_cast<unsigned>(n_rows * slices)),
-                             dim3(kThreads), 0, as_hip(stream), a);
+    auto whole = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool vec = vocab % 4 == 0 && whole(logits) && whole(out) && whole(bias) && bias_stride % 4 == 0;
+    const bool four = per_thread(n_rows, vocab) == 4;
+    asdsl_status st = launch("logits_control_kernel",
+                             four ? (vec ? logits_control_kernel<4, true> : logits_control_kernel<4, false>)
+                                  : (vec ? logits_control_kernel<16, true> : logits_control_kernel<16, false>),
+                             dim3(static_cast<unsigned>(n_rows * slices)), dim3(kThreads), 0, as_hip(stream), a);
     if (st != ASDSL_OK || !tokens) return st;
     return launch("logits_token_kernel", logits_token_kernel, dim3(n_rows), dim3(kWave), 0, as_hip(stream),
                   static_cast<const unsigned long long*>(ws), slices, tokens);
