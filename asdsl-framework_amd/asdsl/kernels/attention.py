@@ -12,25 +12,42 @@ reference, which decodes one sequence (asdsl/kernels/native/unified_engine.cpp:1
 
 from __future__ import annotations
 
+import functools
+
 from asdsl import _hip
 from asdsl.kernels._buffers import _Tensor
 
 try:
     from torch import cuda as _cuda
-    from torch import empty as _empty
+    from torch import empty_like as _empty_like
     from torch import float16 as _f16
     from torch import float32 as _f32
     from torch import int8 as _i8
     from torch import int32 as _i32
     from torch import uint8 as _u8
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream  # without a Stream object
 except ImportError:  # no tensors without torch: every call is refused
-    _cuda = _empty = _f16 = _f32 = _i8 = _i32 = _u8 = None
+    _cuda = _empty_like = _f16 = _f32 = _i8 = _i32 = _u8 = _raw_stream = None
 
 KV_BLOCK = 64  # dims per scale of an int8 cache
 
 
-def _addr(fn: str, name: str, t, dtype, n: int) -> int:
-    """The address of a contiguous tensor of n elements on the current device."""
+def _stream(dev: int) -> int:
+    """The current stream of the current device dev."""
+    return _raw_stream(dev) if _raw_stream is not None else _hip.stream_handle()
+
+
+def _device(t) -> int:
+    """The current device, which the call's tensors have to be on (no device where t, one of them, is on none)."""
+    return _cuda.current_device() if isinstance(t, _Tensor) and t.is_cuda else -2
+
+
+def _addr(fn: str, dev: int, name: str, t, dtype, n: int) -> int:
+    """The address of a contiguous tensor of n elements on device dev.  A call
+    of small sizes is bound by its host time, most of which is these checks:
+    the good case is one expression."""
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.numel() == n and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, _Tensor):
         raise ValueError(f"{fn}: {name} must be a device tensor")
     if t.dtype is not dtype:
@@ -39,11 +56,9 @@ def _addr(fn: str, name: str, t, dtype, n: int) -> int:
         raise ValueError(f"{fn}: {name} has {t.numel()} elements, needs {n}")
     if not t.is_cuda:
         raise ValueError(f"{fn}: {name} must be a device tensor")
-    if t.get_device() != _cuda.current_device():
-        raise ValueError(f"{fn}: {name} is on device {t.get_device()}, the current one is {_cuda.current_device()}")
-    if not t.is_contiguous():
-        raise ValueError(f"{fn}: {name} must be contiguous")
-    return t.data_ptr()
+    if t.get_device() != dev:
+        raise ValueError(f"{fn}: {name} is on device {t.get_device()}, the current one is {dev}")
+    raise ValueError(f"{fn}: {name} must be contiguous")
 
 
 def _cache_dims(fn: str, name: str, k, v, dims: int = 4) -> tuple:
@@ -53,7 +68,7 @@ def _cache_dims(fn: str, name: str, k, v, dims: int = 4) -> tuple:
     shape = tuple(k.shape)
     if tuple(v.shape) != shape or v.dtype is not k.dtype:
         raise ValueError(f"{fn}: the {name} caches differ in shape or type")
-    if len(shape) not in (3, dims):
+    if len(shape) != dims and len(shape) != 3:
         raise ValueError(f"{fn}: a {name} cache has {len(shape)} dimensions, {3 if dims == 3 else '3 or 4'} are wanted")
     if k.dtype is not _f16 and k.dtype is not _i8:
         raise ValueError(f"{fn}: a {name} cache is fp16 or int8, got {k.dtype}")
@@ -62,16 +77,19 @@ def _cache_dims(fn: str, name: str, k, v, dims: int = 4) -> tuple:
     return shape if len(shape) == 4 else (1, *shape)
 
 
-def _caches(fn: str, name: str, k, v, k_scale, v_scale, n: int, head_dim: int) -> tuple:
+def _caches(fn: str, dev: int, name: str, k, v, k_scale, v_scale, head_dim: int) -> tuple:
     """Addresses of a pair of caches (k, v), and of their scales for the int8 form (k, v, k_scale, v_scale)."""
-    int8 = k.dtype is _i8
-    if int8 != (k_scale is not None) or int8 != (v_scale is not None):
+    dtype, n = k.dtype, k.numel()
+    if dtype is not _i8:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"{fn}: {name} caches take scales exactly where they are int8")
+        return _addr(fn, dev, f"{name} keys", k, dtype, n), _addr(fn, dev, f"{name} values", v, dtype, n)
+    if k_scale is None or v_scale is None:
         raise ValueError(f"{fn}: {name} caches take scales exactly where they are int8")
-    at = (_addr(fn, f"{name} keys", k, k.dtype, n), _addr(fn, f"{name} values", v, v.dtype, n))
-    if int8:
-        m = n // head_dim * (head_dim // KV_BLOCK)
-        at += (_addr(fn, f"{name} key scales", k_scale, _f32, m), _addr(fn, f"{name} value scales", v_scale, _f32, m))
-    return at
+    m = n // KV_BLOCK
+    return (_addr(fn, dev, f"{name} keys", k, dtype, n), _addr(fn, dev, f"{name} values", v, dtype, n),
+            _addr(fn, dev, f"{name} key scales", k_scale, _f32, m),
+            _addr(fn, dev, f"{name} value scales", v_scale, _f32, m))
 
 
 def _heads(fn: str, q, head_dim: int, n_rows: int, what: str = "q") -> int:
@@ -84,15 +102,19 @@ def _heads(fn: str, q, head_dim: int, n_rows: int, what: str = "q") -> int:
     return n // (n_rows * head_dim)
 
 
-def _out(fn: str, name: str, out, like, shape):
-    if out is None:
-        return _empty(shape, dtype=_f32, device=like.device)
-    return out
-
-
 def _work(nbytes: int, like):
     """A work buffer of this call on its stream (None where it needs none)."""
-    return _empty(nbytes, dtype=_u8, device=like.device) if nbytes else None
+    return like.new_empty(nbytes, dtype=_u8) if nbytes else None
+
+
+@functools.lru_cache(maxsize=4096)
+def _window_bytes(*dims) -> int:
+    return _hip.LIB.asdsl_attention_window_work_bytes(*dims)
+
+
+@functools.lru_cache(maxsize=4096)
+def _prefix_bytes(*dims) -> int:
+    return _hip.LIB.asdsl_attention_prefix_work_bytes(*dims)
 
 
 def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, pos_offset: int = 0, k_scale=None,
@@ -121,14 +143,15 @@ def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, p
             or rope_cos.shape != rope_sin.shape:
         raise ValueError(f"{fn}: rope_cos and rope_sin must be tensors [positions, rotary_dim / 2] of one shape")
     rope_rows, half = rope_cos.shape
-    at = (_addr(fn, "qkv", qkv, _f32, qkv.numel()), *_caches(fn, "kv", k_cache, v_cache, k_scale, v_scale,
-                                                           k_cache.numel(), d),
-          _addr(fn, "rope_cos", rope_cos, _f32, rope_rows * half), _addr(fn, "rope_sin", rope_sin, _f32, rope_rows * half),
-          _addr(fn, "pos", pos, _i32, n_seq))
-    q_out = _out(fn, "q_out", q_out, qkv, (tokens, n_heads * d))
-    _hip.call("asdsl_kv_append_q8" if k_scale is not None else "asdsl_kv_append_f16", *at,
-              _addr(fn, "q_out", q_out, _f32, tokens * n_heads * d), n_seq, tokens // n_seq, n_heads, n_kv, d, 2 * half,
-              rows, int(pos_offset), rope_rows, _hip.stream_handle())
+    dev = _device(qkv)
+    at = (_addr(fn, dev, "qkv", qkv, _f32, qkv.numel()), *_caches(fn, dev, "kv", k_cache, v_cache, k_scale, v_scale, d),
+          _addr(fn, dev, "rope_cos", rope_cos, _f32, rope_rows * half),
+          _addr(fn, dev, "rope_sin", rope_sin, _f32, rope_rows * half), _addr(fn, dev, "pos", pos, _i32, n_seq))
+    if q_out is None:
+        q_out = qkv.new_empty((tokens, n_heads * d))
+    _hip.call("asdsl_kv_append_f16" if k_scale is None else "asdsl_kv_append_q8", *at,
+              _addr(fn, dev, "q_out", q_out, _f32, tokens * n_heads * d), n_seq, tokens // n_seq, n_heads, n_kv, d,
+              2 * half, rows, int(pos_offset), rope_rows, _stream(dev))
     return q_out
 
 
@@ -150,16 +173,17 @@ def attention_window(q, k_cache, v_cache, pos, *, window: int = 0, sinks: int = 
         raise ValueError(f"{fn}: q must be [..., n_heads, {d}] or [tokens, n_heads * {d}], n_heads a multiple of {n_kv}")
     n = q.numel()
     tokens = per_seq // n_heads
-    window, sinks = int(window), int(sinks)
-    dims = (n_seq, tokens, n_heads, n_kv, d, rows, window, sinks)
-    at = (_addr(fn, "q", q, _f32, n), *_caches(fn, "kv", k_cache, v_cache, k_scale, v_scale, k_cache.numel(), d),
-          _addr(fn, "pos", pos, _i32, n_seq))
-    out = _out(fn, "out", out, q, q.shape)
-    nbytes = _hip.LIB.asdsl_attention_window_work_bytes(*dims)
+    dims = (n_seq, tokens, n_heads, n_kv, d, rows, int(window), int(sinks))
+    dev = _device(q)
+    at = (_addr(fn, dev, "q", q, _f32, n), *_caches(fn, dev, "kv", k_cache, v_cache, k_scale, v_scale, d),
+          _addr(fn, dev, "pos", pos, _i32, n_seq))
+    if out is None:
+        out = _empty_like(q)
+    nbytes = _window_bytes(*dims)
     work = _work(nbytes, q)
-    _hip.call("asdsl_attention_window_q8kv" if k_scale is not None else "asdsl_attention_window_f16kv", *at,
-              _addr(fn, "out", out, _f32, n), *dims, None if work is None else work.data_ptr(), nbytes,
-              _hip.stream_handle())
+    _hip.call("asdsl_attention_window_f16kv" if k_scale is None else "asdsl_attention_window_q8kv", *at,
+              _addr(fn, dev, "out", out, _f32, n), *dims, None if work is None else work.data_ptr(), nbytes,
+              _stream(dev))
     return out
 
 
@@ -187,14 +211,15 @@ def attention_prefix(q, k_prefix, v_prefix, k_own, v_own, own_pos, *, prefix_len
     if not 0 <= prefix_len <= prefix_rows:
         raise ValueError(f"{fn}: prefix_len must be in [0, {prefix_rows}], got {prefix_len}")
     n = q.numel()
-    at = (_addr(fn, "q", q, _f32, n), *_caches(fn, "prefix", k_prefix, v_prefix, k_prefix_scale, v_prefix_scale,
-                                               k_prefix.numel(), d),
-          *_caches(fn, "own", k_own, v_own, k_scale, v_scale, k_own.numel(), d),
-          _addr(fn, "own_pos", own_pos, _i32, n_seq))
-    out = _out(fn, "out", out, q, q.shape)
-    nbytes = _hip.LIB.asdsl_attention_prefix_work_bytes(n_seq, n_heads, n_kv, d, prefix_len, rows)
+    dev = _device(q)
+    at = (_addr(fn, dev, "q", q, _f32, n),
+          *_caches(fn, dev, "prefix", k_prefix, v_prefix, k_prefix_scale, v_prefix_scale, d),
+          *_caches(fn, dev, "own", k_own, v_own, k_scale, v_scale, d), _addr(fn, dev, "own_pos", own_pos, _i32, n_seq))
+    if out is None:
+        out = _empty_like(q)
+    nbytes = _prefix_bytes(n_seq, n_heads, n_kv, d, prefix_len, rows)
     work = _work(nbytes, q)
-    _hip.call("asdsl_attention_prefix_q8kv" if k_scale is not None else "asdsl_attention_prefix_f16kv", *at,
-              _addr(fn, "out", out, _f32, n), n_seq, n_heads, n_kv, d, prefix_len, prefix_rows, rows,
-              None if work is None else work.data_ptr(), nbytes, _hip.stream_handle())
+    _hip.call("asdsl_attention_prefix_f16kv" if k_scale is None else "asdsl_attention_prefix_q8kv", *at,
+              _addr(fn, dev, "out", out, _f32, n), n_seq, n_heads, n_kv, d, prefix_len, prefix_rows, rows,
+              None if work is None else work.data_ptr(), nbytes, _stream(dev))
     return out

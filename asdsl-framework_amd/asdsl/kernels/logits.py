@@ -5,9 +5,16 @@ counterpart in the reference, whose decoding is plain greedy
 
 from __future__ import annotations
 
+import functools
+
 from asdsl import _hip
 from asdsl.kernels._buffers import _Tensor
-from asdsl.kernels.attention import _addr, _empty, _f32, _i32, _work
+from asdsl.kernels.attention import _addr, _device, _empty_like, _f32, _i32, _stream, _work
+
+
+@functools.lru_cache(maxsize=4096)
+def _control_bytes(rows: int, vocab: int) -> int:
+    return _hip.LIB.asdsl_logits_control_work_bytes(rows, vocab)
 
 
 def control_logits(logits, *, history=None, prompt_len=None, history_len=None, repetition=None, frequency=None,
@@ -59,28 +66,33 @@ def control_logits(logits, *, history=None, prompt_len=None, history_len=None, r
         else:
             raise ValueError(f"{fn}: {name} must be a device tensor [{width}] or [{rows}, {width}]")
 
-    def opt(name, t, dtype, count):
-        return None if t is None else _addr(fn, name, t, dtype, count)
-
-    a_logits = _addr(fn, "logits", logits, _f32, n)
-    a_history = opt("history", history, _i32, rows * cap) if cap else None
-    a_prompt = opt("prompt_len", prompt_len, _i32, rows) if cap else None
-    a_len = opt("history_len", history_len, _i32, rows) if cap else None
-    a_rep = opt("repetition", repetition, _f32, rows) if cap else None
-    a_freq = opt("frequency", frequency, _f32, rows) if cap else None
-    a_pres = opt("presence", presence, _f32, rows) if cap else None
-    a_bias = None if bias is None else _addr(fn, "bias", bias, _f32, bias.numel())
-    a_allowed = None if allowed is None else _addr(fn, "allowed", allowed, _i32, allowed.numel())
+    dev = _device(logits)
+    a_logits = _addr(fn, dev, "logits", logits, _f32, n)
+    a_history = a_prompt = a_len = a_rep = a_freq = a_pres = None
+    if cap:
+        a_history = _addr(fn, dev, "history", history, _i32, rows * cap)
+        if prompt_len is not None:
+            a_prompt = _addr(fn, dev, "prompt_len", prompt_len, _i32, rows)
+        if history_len is not None:
+            a_len = _addr(fn, dev, "history_len", history_len, _i32, rows)
+        if repetition is not None:
+            a_rep = _addr(fn, dev, "repetition", repetition, _f32, rows)
+        if frequency is not None:
+            a_freq = _addr(fn, dev, "frequency", frequency, _f32, rows)
+        if presence is not None:
+            a_pres = _addr(fn, dev, "presence", presence, _f32, rows)
+    a_bias = None if bias is None else _addr(fn, dev, "bias", bias, _f32, bias.numel())
+    a_allowed = None if allowed is None else _addr(fn, dev, "allowed", allowed, _i32, allowed.numel())
     if out is None:
-        out = _empty(logits.shape, dtype=_f32, device=logits.device)
-    a_out = _addr(fn, "out", out, _f32, n)
+        out = _empty_like(logits)
+    a_out = _addr(fn, dev, "out", out, _f32, n)
     tokens = work = None
     nbytes = 0
     if pick:
-        tokens = _empty(rows, dtype=_i32, device=logits.device)
-        nbytes = _hip.LIB.asdsl_logits_control_work_bytes(rows, vocab)
+        tokens = logits.new_empty(rows, dtype=_i32)
+        nbytes = _control_bytes(rows, vocab)
         work = _work(nbytes, logits)
     _hip.call("asdsl_logits_control", a_logits, a_out, None if tokens is None else tokens.data_ptr(), a_history,
               a_prompt, a_len, cap, a_rep, a_freq, a_pres, a_bias, strides[0], a_allowed, strides[1], rows, vocab,
-              None if work is None else work.data_ptr(), nbytes, _hip.stream_handle())
+              None if work is None else work.data_ptr(), nbytes, _stream(dev))
     return out, tokens
