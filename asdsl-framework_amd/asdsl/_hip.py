@@ -114,6 +114,8 @@ SIGNATURES: dict[str, list] = {
     "asdsl_logits_control_work_bytes": [_I, _I],
     "asdsl_logits_control": [_P] * 6 + [_I] + [_P] * 4 + [ctypes.c_longlong, _P, ctypes.c_longlong, _I, _I, _P,
                                                          ctypes.c_size_t, _P],
+    "asdsl_decode_branches_work_bytes": [_P, _I, _I, _I],
+    "asdsl_decode_branches": [_P, _P, _I, _I, _I, _P, _P, _P, _P, ctypes.c_size_t, _P],
     "asdsl_kv_zero_from": [_P, _P, _I, _I, _I, _I, _P],
     "asdsl_kv_zero_from_q8": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
     "asdsl_repack_preq_to_preq2": [_P, _P, _P, _I, _I, _I, _P],
@@ -132,6 +134,7 @@ _RESTYPE = {"asdsl_last_error": ctypes.c_char_p, "asdsl_attention_work_floats": 
             "asdsl_gemv_preq2_fused_batch_work_bytes": ctypes.c_size_t,
             "asdsl_gemv_preq2_fused_batch_work_bytes_n": ctypes.c_size_t,
             "asdsl_affine_batch_work_bytes": ctypes.c_size_t,
+            "asdsl_decode_branches_work_bytes": ctypes.c_size_t,
             "asdsl_attention_window_work_bytes": ctypes.c_size_t,
             "asdsl_attention_prefix_work_bytes": ctypes.c_size_t,
             "asdsl_logits_control_work_bytes": ctypes.c_size_t}

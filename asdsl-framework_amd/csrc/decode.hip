@@ -1543,6 +1543,60 @@ asdsl_status launch_prefill_attention(const float* Q, const KvCache& kv, bool q8
     return ASDSL_OK;
 }
 
+// ---------------------------------------------------------------- branches
+// A step of n continuations of one prompt: the prompt chunk's projections (each
+// column with the single-token step's arithmetic), every column's K/V rows in
+// its own cache, and attention over the prompt's rows, shared, and its own.
+
+// The int8 image of X [n][K] (verify_add_norm_kernel's CHUNK form of images).
+template <int GS>
+__global__ __launch_bounds__(256) void branch_image_kernel(const float* __restrict__ X, int K, uint2* __restrict__ img,
+                                                           float2* __restrict__ fac, float* __restrict__ us) {
+    const int col = static_cast<int>(blockIdx.y);
+    const size_t at = image_at(col, K);
+    const int nchunk = K >> 3;
+    const int ch = static_cast<int>(blockIdx.x * blockDim.x + threadIdx.x);
+    const float4* x = reinterpret_cast<const float4*>(X + static_cast<size_t>(col) * K) + 2 * min(ch, nchunk - 1);
+    const float4 a = x[0], b = x[1];
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    image_store8<GS>(v, ch, col % kImageCols, ch < nchunk, img + at / sizeof(uint2), fac + at / sizeof(float2),
+                     us + at / sizeof(float));
+}
+
+constexpr int kMaxBranches = 256;
+
+// Work buffer layout of a step of n branches (offsets in floats).
+struct BranchWork {
+    size_t H, QKV, Q, att, O, GU, img, attn, attn_bytes, total;
+};
+
+BranchWork branch_work(const asdsl_decode_model& m, int n, int prefix_len, int own_rows) {
+    BranchWork w{};
+    size_t at = 0;
+    auto take = [&](size_t cnt) {
+        const size_t here = at;
+        at += align64(cnt);
+        return here;
+    };
+    const size_t N = static_cast<size_t>(n);
+    const int wide = m.hidden > m.ffn ? m.hidden : m.ffn;
+    w.H = take(N * m.hidden);
+    w.QKV = take(N * (m.n_heads + 2 * m.n_kv_heads) * m.head_dim);
+    w.Q = take(N * m.n_heads * m.head_dim);
+    w.att = take(N * m.n_heads * m.head_dim);
+    w.O = take(N * m.hidden);
+    w.GU = take(N * 2 * m.ffn);
+    w.img = take((N + kImageCols - 1) / kImageCols * image_bytes(wide) / sizeof(float));
+    w.attn_bytes = asdsl_attention_prefix_work_bytes(n, m.n_heads, m.n_kv_heads, m.head_dim, prefix_len, own_rows);
+    w.attn = take(w.attn_bytes / sizeof(float));
+    w.total = at;
+    return w;
+}
+
+bool branch_sizes_ok(const asdsl_decode_model& m, int n, int prefix_len, int own_rows) {
+    return n >= 1 && n <= kMaxBranches && prefix_len >= 0 && own_rows >= 1 && prefix_len <= m.max_seq - own_rows;
+}
+
 // Work buffer layout of a verify pass of up to n tokens (offsets in floats).
 struct VerifyWork {
     size_t H, X, QKV, part, att, O, GU, S, keys, inv, mimg, mimg_bytes, total;
@@ -2078,6 +2132,117 @@ extern "C" asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, co
     }
     return launch("prefill_finish_kernel", prefill_finish_kernel, dim3(1), dim3(kWave), 0, s,
                   static_cast<const unsigned long long*>(logits ? key : nullptr), token, pos, start_pos + n);
+}
+
+extern "C" size_t asdsl_decode_branches_work_bytes(const asdsl_decode_model* model, int n_branches, int prefix_len,
+                                                   int own_rows) {
+    if (check_model(model) != ASDSL_OK || !branch_sizes_ok(*model, n_branches, prefix_len, own_rows)) return 0;
+    return branch_work(*model, n_branches, prefix_len, own_rows).total * sizeof(float);
+}
+
+extern "C" asdsl_status asdsl_decode_branches(const asdsl_decode_model* model, const asdsl_branch_layer* own,
+                                              int n_branches, int prefix_len, int own_rows, const int* tokens,
+                                              const int* own_pos, float* logits, void* work, size_t work_bytes,
+                                              asdsl_stream_t stream) {
+    const asdsl_status cs = check_model(model);
+    if (cs != ASDSL_OK) return cs;
+    const asdsl_decode_model& m = *model;
+    ASDSL_CHECK_ARG(own && tokens && own_pos && logits && work, "decode_branches: null pointer");
+    ASDSL_CHECK_ARG(branch_sizes_ok(m, n_branches, prefix_len, own_rows),
+                    "decode_branches: 1..%d branches, prefix_len + own_rows within the model's max_seq", kMaxBranches);
+    const bool q8 = m.kv_format == ASDSL_KV_INT8;
+    for (int l = 0; l < m.n_layers; ++l)
+        ASDSL_CHECK_ARG(own[l].k && own[l].v && reinterpret_cast<uintptr_t>(own[l].k) % 16 == 0 &&
+                            reinterpret_cast<uintptr_t>(own[l].v) % 16 == 0 && (!q8 || (own[l].k_scale && own[l].v_scale)),
+                        "decode_branches: layer %d: own caches must be non-null, 16-byte aligned, with scales for int8", l);
+    ASDSL_CHECK_ARG(reinterpret_cast<uintptr_t>(logits) % 16 == 0, "decode_branches: logits must be 16-byte aligned");
+    if (preq2_norm_factored()) {  // the step's other arithmetic, as in a prompt chunk
+        set_error("decode_branches: not with the factored norm");
+        return ASDSL_ERR_UNSUPPORTED;
+    }
+    const int n = n_branches;
+    const BranchWork w = branch_work(m, n, prefix_len, own_rows);
+    hipStream_t s = as_hip(stream);
+    void* ws = nullptr;
+    asdsl_status st = work_buffer(s, work, work_bytes, w.total * sizeof(float), &ws, "decode_branches");
+    if (st != ASDSL_OK) return st;
+    float* base = static_cast<float*>(ws);
+    float* H = base + w.H;
+    float* QKV = base + w.QKV;
+    float* Q = base + w.Q;
+    float* att = base + w.att;
+    float* O = base + w.O;
+    float* GU = base + w.GU;
+    void* image = base + w.img;
+    void* attn = w.attn_bytes ? base + w.attn : nullptr;
+    auto* img = reinterpret_cast<uint2*>(base + w.img);
+    const int qkv_dim = (m.n_heads + 2 * m.n_kv_heads) * m.head_dim;
+    const int q_dim = m.n_heads * m.head_dim;
+    auto fac_of = [&](int K) { return reinterpret_cast<float2*>(static_cast<uint8_t*>(image) + image_fac_offset(K)); };
+    auto us_of = [&](int K) { return reinterpret_cast<float*>(static_cast<uint8_t*>(image) + image_us_offset(K)); };
+    auto gemm = [&](const uint8_t* meta, const uint8_t* quant, float* Y, int M, int K, int gs) -> asdsl_status {
+        return n <= kImageCols && preq2_batch_exact_mfma_applies(M, K, gs, n)
+                   ? preq2_batch_exact_mfma_image(meta, quant, image, Y, M, K, gs, n, stream)
+                   : preq2_gemm_exact(meta, quant, image, Y, M, K, gs, n, stream);
+    };
+    auto norm_then_gemm = [&](const float* D, const float* nw, const uint8_t* meta, const uint8_t* quant, float* Y,
+                              int M, int gs) -> asdsl_status {
+        const int K = m.hidden;
+        const asdsl_status r = launch("verify_add_norm_kernel",
+                                      gs == 32 ? verify_add_norm_kernel<32, true> : verify_add_norm_kernel<128, true>,
+                                      dim3(n), dim3(kNormThreads), 0, s, H, D, nw, static_cast<float*>(nullptr), K,
+                                      m.rms_eps, n, img, fac_of(K), us_of(K), static_cast<float*>(nullptr));
+        return r != ASDSL_OK ? r : gemm(meta, quant, Y, M, K, gs);
+    };
+    st = launch("verify_embed_kernel", verify_embed_kernel, dim3((m.hidden + 1023) / 1024, n), dim3(256), 0, s, m.embed,
+                tokens, H, m.hidden, m.vocab, static_cast<unsigned long long*>(nullptr));
+    if (st != ASDSL_OK) return st;
+    const float* pending = nullptr;
+    for (int l = 0; l < m.n_layers; ++l) {
+        const asdsl_decode_layer& L = m.layers[l];
+        const asdsl_branch_layer& B = own[l];
+        st = norm_then_gemm(pending, L.rms_att, L.qkv_meta, L.qkv_quant, QKV, qkv_dim, m.gs_attn);
+        if (st != ASDSL_OK) return st;
+        if (q8) {
+            auto* k = static_cast<int8_t*>(B.k);
+            auto* v = static_cast<int8_t*>(B.v);
+            st = asdsl_kv_append_q8(QKV, k, v, B.k_scale, B.v_scale, m.rope_cos, m.rope_sin, own_pos, Q, n, 1,
+                                    m.n_heads, m.n_kv_heads, m.head_dim, m.rotary_dim, own_rows, prefix_len, m.max_seq,
+                                    stream);
+            if (st != ASDSL_OK) return st;
+            st = asdsl_attention_prefix_q8kv(Q, static_cast<const int8_t*>(L.k_cache),
+                                             static_cast<const int8_t*>(L.v_cache), L.k_scale, L.v_scale, k, v,
+                                             B.k_scale, B.v_scale, own_pos, att, n, m.n_heads, m.n_kv_heads,
+                                             m.head_dim, prefix_len, m.max_seq, own_rows, attn, w.attn_bytes, stream);
+        } else {
+            auto* k = static_cast<uint16_t*>(B.k);
+            auto* v = static_cast<uint16_t*>(B.v);
+            st = asdsl_kv_append_f16(QKV, k, v, m.rope_cos, m.rope_sin, own_pos, Q, n, 1, m.n_heads, m.n_kv_heads,
+                                     m.head_dim, m.rotary_dim, own_rows, prefix_len, m.max_seq, stream);
+            if (st != ASDSL_OK) return st;
+            st = asdsl_attention_prefix_f16kv(Q, static_cast<const uint16_t*>(L.k_cache),
+                                              static_cast<const uint16_t*>(L.v_cache), k, v, own_pos, att, n,
+                                              m.n_heads, m.n_kv_heads, m.head_dim, prefix_len, m.max_seq, own_rows,
+                                              attn, w.attn_bytes, stream);
+        }
+        if (st != ASDSL_OK) return st;
+        st = launch("branch_image_kernel", m.gs_attn == 32 ? branch_image_kernel<32> : branch_image_kernel<128>,
+                    dim3((q_dim / 8 + 255) / 256, n), dim3(256), 0, s, static_cast<const float*>(att), q_dim, img,
+                    fac_of(q_dim), us_of(q_dim));
+        if (st != ASDSL_OK) return st;
+        st = gemm(L.o_meta, L.o_quant, O, m.hidden, q_dim, m.gs_attn);
+        if (st != ASDSL_OK) return st;
+        st = norm_then_gemm(O, L.rms_ffn, L.gu_meta, L.gu_quant, GU, 2 * m.ffn, m.gs_ffn);
+        if (st != ASDSL_OK) return st;
+        st = launch("verify_swiglu_kernel", m.gs_ffn == 32 ? verify_swiglu_kernel<32, true> : verify_swiglu_kernel<128, true>,
+                    dim3((m.ffn / 8 + 255) / 256, n), dim3(256), 0, s, static_cast<const float*>(GU),
+                    static_cast<float*>(nullptr), m.ffn, L.fatrelu_threshold, n, img, fac_of(m.ffn), us_of(m.ffn));
+        if (st != ASDSL_OK) return st;
+        st = gemm(L.down_meta, L.down_quant, O, m.hidden, m.ffn, m.gs_ffn);
+        if (st != ASDSL_OK) return st;
+        pending = O;
+    }
+    return norm_then_gemm(pending, m.rms_out, m.lm_meta, m.lm_quant, logits, m.vocab, m.gs_lm);
 }
 
 extern "C" asdsl_status asdsl_kv_zero_from(uint16_t* k_cache, uint16_t* v_cache, int n_kv_heads, int head_dim,

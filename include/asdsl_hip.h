@@ -726,6 +726,38 @@ asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, 
                                   long long allowed_stride, int n_rows, int vocab, void* work, size_t work_bytes,
                                   asdsl_stream_t stream);
 
+/* One layer's caches of the branches' own rows (device pointers):
+ * [n_branches][n_kv_heads][own_rows][128], fp16 or int8 as the model's
+ * kv_format, int8 with scales [n_branches][n_kv_heads][own_rows][2]. */
+typedef struct asdsl_branch_layer {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+} asdsl_branch_layer;
+
+/* Bytes of device work buffer asdsl_decode_branches needs; 0 for an invalid
+ * model or sizes it refuses. */
+size_t asdsl_decode_branches_work_bytes(const asdsl_decode_model* model, int n_branches, int prefix_len, int own_rows);
+
+/* Queues one step of n_branches (1..256) continuations of one prompt, whose
+ * rows [0, prefix_len) the model's caches hold and are only read: branch b's
+ * tokens[b] (device) runs through every layer at position prefix_len +
+ * own_pos[b] (device; not advanced), its K/V rows go to row own_pos[b] of its
+ * own caches (own: a HOST array of n_layers entries), and its attention covers
+ * the prompt's rows and its own up to there; logits[n_branches][vocab] (16-byte
+ * aligned).  A branch whose own_pos is outside [0, own_rows) writes no row and
+ * attends to nothing (to the prompt alone at -1), so its logits are not the
+ * model's.  prefix_len + own_rows <= max_seq.  The projections are the
+ * single-token step's column by column; the attention sums in another order, so
+ * a branch follows asdsl_decode_token up to fp32 rounding (which int8
+ * activation codes can carry on).  work: 256-byte aligned.  ASDSL_ERR_UNSUPPORTED
+ * under ASDSL_HIP_NORM_FACTORED.  No reference counterpart (the reference
+ * decodes one sequence, asdsl/kernels/native/unified_engine.cpp:1339-1688). */
+asdsl_status asdsl_decode_branches(const asdsl_decode_model* model, const asdsl_branch_layer* own, int n_branches,
+                                   int prefix_len, int own_rows, const int* tokens, const int* own_pos, float* logits,
+                                   void* work, size_t work_bytes, asdsl_stream_t stream);
+
 /* The int8 cache's form of asdsl_kv_zero_from: codes 0 and scales 1.0 in rows
  * [from_pos, max_seq), as zero_kv_from leaves them
  * (asdsl/kernels/native/unified_engine.cpp:1263-1283). */
