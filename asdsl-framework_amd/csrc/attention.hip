@@ -369,15 +369,19 @@ struct VRaw<D, true> {
 // row's first keys, so that a step then needs no exchange between lanes and no
 // scaling of what was accumulated.  An int8 cache's value scales go into the
 // weights before they are cut; ev is the power of two that keeps those in
-// fp16's range (the row's accumulators are 2^-ev times O').
+// fp16's range (the row's accumulators are 2^-ev times O'), at least kEvLow,
+// below which scales leave no trace in a sum (2^-ev and 2^kMost have room
+// in fp32 together).
+constexpr int kEvLow = -100;
 template <bool Q8, int kStep>
 struct Softmax {
     float m = -INFINITY, l = 0.0f;
-    int ev = -126;
+    int ev = kEvLow;
 
-    // Whether a step's products (score = s * c) or its seen value scales ask for a
-    // new base, in any lane of the wave; then the base and the factor of what
-    // the row has accumulated.
+    // Whether a step's products (score = s * c) or its value scales (vs_max, the
+    // largest, seen or not) may ask for a new base, in any lane of the wave;
+    // then the base and the factor of what the row has accumulated (vs_max: the
+    // largest of use that the row sees).
     template <int N>
     __device__ __forceinline__ bool rises(const float (&s)[N], float c, float vs_max, float& top) const {
         top = s[0];
@@ -414,10 +418,24 @@ struct Softmax {
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
     __device__ __forceinline__ float out_scale() const {
-        if constexpr (Q8) return pow2(max(ev, -126));
-        return 1.0f;
+        return Q8 ? pow2(ev) : 1.0f;
     }
 };
+
+// The largest value scale of the N keys that the row sees (those that are no
+// number of any use, infinite ones among them, make their weights infinite).
+template <int N, int D>
+__device__ __forceinline__ float top_scale(const float (&vs)[N][D / 64], uint32_t seen) {
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b) {
+            const float a = fabsf(vs[i][b]);
+            top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
+        }
+    return top;
+}
 
 // O' of 16 rows: element i of acc[j] at dim *_dim(4 * (lane / 16) + i, j).
 template <int D, bool Q8>
@@ -428,11 +446,16 @@ struct State : Softmax<Q8, 16> {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    template <int N>
-    __device__ __forceinline__ void step(float (&s)[N], float c, float vs_max) {
-        float top;
-        if (this->rises(s, c, vs_max, top)) {
-            const float alpha = this->rebase(top, vs_max);
+    __device__ __forceinline__ void step(float (&s)[8], float c, const float (&vs)[8][D / 64], uint32_t seen) {
+        float top, any = 0.0f;
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b) any = fmaxf(any, fabsf(vs[i][b]));
+        }
+        if (this->rises(s, c, any, top)) {
+            const float alpha = this->rebase(top, Q8 ? top_scale<8, D>(vs, seen) : 0.0f);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
         }
@@ -473,19 +496,28 @@ struct Weights {
     static constexpr int kBlocks = Q8 ? D / 64 : 1;
     uint32_t h[kBlocks][4], l[kBlocks][4];
 
-    // vs: the keys' value scales; a scale of a key that the row does not see
-    // may be anything.  ev: the row's State::ev.
-    __device__ __forceinline__ void cut(const float* s, const float (*vs)[D / 64], uint32_t seen, int ev) {
+    // vs: the keys' value scales; one of a key that the row does not see may be
+    // anything (all: the row sees them all).  ev: the row's Softmax::ev.
+    __device__ __forceinline__ void cut(const float* s, const float (*vs)[D / 64], bool all, uint32_t seen, int ev) {
         if constexpr (Q8) {
-            const float f = pow2(min(-ev, 126));
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b)
+            const float f = pow2(-ev);
+            if (all) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x0 = (seen >> (2 * i)) & 1u ? s[2 * i] * (vs[2 * i][b] * f) : 0.0f;
-                    const float x1 = (seen >> (2 * i + 1)) & 1u ? s[2 * i + 1] * (vs[2 * i + 1][b] * f) : 0.0f;
-                    two_parts(x0, x1, h[b][i], l[b][i]);
+                    const float s0 = s[2 * i] * f, s1 = s[2 * i + 1] * f;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b) two_parts(s0 * vs[2 * i][b], s1 * vs[2 * i + 1][b], h[b][i], l[b][i]);
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s0 = s[2 * i] * f, s1 = s[2 * i + 1] * f;
+#pragma unroll
+                    for (int b = 0; b < kBlocks; ++b)
+                        two_parts((seen >> (2 * i)) & 1u ? s0 * vs[2 * i][b] : 0.0f,
+                                  (seen >> (2 * i + 1)) & 1u ? s1 * vs[2 * i + 1][b] : 0.0f, h[b][i], l[b][i]);
+                }
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) two_parts(s[2 * i], s[2 * i + 1], h[0][i], l[0][i]);
@@ -534,21 +566,6 @@ __device__ __forceinline__ uint32_t mask_keys(const Keys& K, const RowSight& see
         seen |= ok ? 1u << i : 0u;
     }
     return seen;
-}
-
-// The largest value scale of the N keys that the row sees (those that are no
-// number of any use, infinite ones among them, make their weights infinite).
-template <int N, int D>
-__device__ __forceinline__ float top_scale(const float (&vs)[N][D / 64], uint32_t seen) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int b = 0; b < D / 64; ++b) {
-            const float a = fabsf(vs[i][b]);
-            top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
-        }
-    return top;
 }
 
 // ------------------------------------------------- few rows: waves over keys
@@ -684,11 +701,9 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, c
         const bool all = all_seen(K, t * kKeys, kKeys);  // the same in every lane
         uint32_t seen = 0xFFu;
         if (!all) seen = mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
-        float top = 0.0f;
-        if constexpr (Q8) top = top_scale<8, D>(x.vs, seen);
-        st.step(s, q.c, top);
+        st.step(s, q.c, x.vs, seen);
         Weights<D, Q8> w;
-        w.cut(s, x.vs, seen, st.ev);
+        w.cut(s, x.vs, all, seen, st.ev);
         bool odd = false;
         if constexpr (!Q8) odd = !all && __builtin_amdgcn_ballot_w64(x.v.odd()) != 0ull;
         if (__builtin_expect(!odd, 1)) {
@@ -852,6 +867,7 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
 // weighted values takes i = 8 s .. 8 s + 7.
 constexpr int kManyWaves = 4;
 constexpr int kWideRows = 32;
+constexpr int kStages = 4;
 
 __device__ __forceinline__ int wide_key(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
@@ -998,7 +1014,7 @@ struct Bring {
 
 template <int D, bool Q8>
 __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const RowMap& map, int row0, long long p0,
-                                         int rows, int split, int splits, int slot, Stage<D, Q8> (&stage)[2]) {
+                                         int rows, int split, int splits, int slot, Stage<D, Q8> (&stage)[kStages]) {
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
     const int n = row0 + wave * kWideRows + (lane & 31), h = lane >> 5;
     const int tiles = (K.n + kKeys - 1) / kKeys;
@@ -1011,7 +1027,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     f32x16 acc[D / 32];
     // int8: the power of two that keeps the wave's weights times value scales in
     // fp16's range (acc is 2^-ev times O'), and the rows that any of its rows sees
-    int ev = -126, p_top = INT_MAX, lo_low = 0;
+    int ev = kEvLow, p_top = INT_MAX, lo_low = 0;
     if (Q8 && K.masked) {
         p_top = n < map.total ? see.p : -1;
         lo_low = n < map.total && see.any ? see.lo : INT_MAX;
@@ -1033,14 +1049,19 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     if (t0 < t1) {
         next.load(K, t0, wave, lane);
         next.store(stage[0], wave, lane);
+        if (t0 + 1 < t1) {
+            next.load(K, t0 + 1, wave, lane);
+            next.store(stage[1], wave, lane);
+        }
     }
     for (int t = t0; t < t1; ++t) {
-        __syncthreads();
-        const Stage<D, Q8>& s = stage[(t - t0) & 1];
+        const int at = t - t0;
+        if (at % 2 == 0) __syncthreads();
+        const Stage<D, Q8>& s = stage[at % kStages];
         half8 o[D / 16];  // the tile's K operands, then V's
 #pragma unroll
         for (int x = 0; x < D / 16; ++x) o[x] = s.k[2 * x + h][lane & 31];
-        if (t + 1 < t1) next.load(K, t + 1, wave, lane);
+        if (t + 2 < t1) next.load(K, t + 2, wave, lane);
         __builtin_amdgcn_sched_barrier(0);
         float p[16];
 #pragma unroll
@@ -1118,7 +1139,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                         vs[i + 3][b] = sc.w;
                     }
             }
-            w.cut(p + 8 * e, vs, seen >> (8 * e), ev);
+            w.cut(p + 8 * e, vs, all, seen >> (8 * e), ev);
             const half8* v = &o[kBoth ? e * (D / 32) : 0];
 #pragma unroll
             for (int u = 0; u < D / 32; ++u) acc[u] = mfma(v[u], w.first(u >> 1), acc[u]);
@@ -1139,7 +1160,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                     }
             }
         }
-        if (t + 1 < t1) next.store(stage[(t + 1 - t0) & 1], wave, lane);
+        if (t + 2 < t1) next.store(stage[(at + 2) % kStages], wave, lane);
     }
     const float l = lanes_sum<32>(st.l);
     if constexpr (!Q8) {
@@ -1148,7 +1169,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     }
     if (n >= map.total) return;
     const long long at = map.at(n);
-    float f = Q8 ? pow2(max(ev, -126)) : 1.0f;
+    float f = Q8 ? pow2(ev) : 1.0f;
     float* dst;
     if (g.slots == 1) {
         const bool any = see.any && l != 0.0f;
@@ -1182,7 +1203,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
 // Row tiles from the last one down: with no window its tokens see the most.
 template <int D, bool Q8>
 __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const AttnArgs g) {
-    __shared__ Stage<D, Q8> stage[2];
+    __shared__ Stage<D, Q8> stage[kStages];
     constexpr int kWgRows = kManyWaves * kWideRows;
     const int group = g.n_heads / g.n_kv;
     const int total = g.n_tokens * group;
@@ -1231,7 +1252,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArg
     constexpr int kWgRows = kMany ? kManyWaves * kWideRows : kRows;
     __shared__ union Lds {
         JoinArea<D, kFewWaves> area;
-        Stage<D, Q8> stage[kMany ? 2 : 1];
+        Stage<D, Q8> stage[kMany ? kStages : 1];
         __device__ Lds() {}
     } lds;
     const int group = g.n_heads / g.n_kv;

@@ -80,12 +80,18 @@ __global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlA
         const int told = min(max(a.history_len ? a.history_len[row] : a.cap, 0), a.cap);
         const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
         const int* ids = a.history + static_cast<long long>(row) * a.cap;
-        for (int i = tid; i < told; i += kThreads) {
-            const int id = ids[i];
-            const uint32_t at = static_cast<uint32_t>(id) - static_cast<uint32_t>(v0);
-            if (id >= 0 && at < static_cast<uint32_t>(n)) {
-                atomicOr(&word[at], kSeen);
-                if (i >= prompt) atomicAdd(&word[at], 1u);
+        constexpr int kIds = 8;  // of a thread at a time, all requested before one is counted
+        for (int i0 = tid; i0 < told; i0 += kIds * kThreads) {
+            int id[kIds];
+#pragma unroll
+            for (int j = 0; j < kIds; ++j) id[j] = i0 + j * kThreads < told ? ids[i0 + j * kThreads] : -1;
+#pragma unroll
+            for (int j = 0; j < kIds; ++j) {
+                const uint32_t at = static_cast<uint32_t>(id[j]) - static_cast<uint32_t>(v0);
+                if (id[j] >= 0 && at < static_cast<uint32_t>(n)) {
+                    atomicOr(&word[at], kSeen);
+                    if (i0 + j * kThreads >= prompt) atomicAdd(&word[at], 1u);
+                }
             }
         }
         if (a.repetition) rep = a.repetition[row];
@@ -188,7 +194,7 @@ extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, in
     const char* what = "logits_control";
     ASDSL_CHECK_ARG(logits && out, "%s: null pointer", what);
     ASDSL_CHECK_ARG(n_rows > 0 && vocab > 0, "%s: n_rows and vocab must be positive", what);
-    ASDSL_CHECK_ARG(history_cap >= 0, "%s: history_cap must not be negative", what);
+    ASDSL_CHECK_ARG(history_cap >= 0 && history_cap <= 1 << 30, "%s: history_cap must be in [0, 2^30]", what);
     ASDSL_CHECK_ARG(history || (!prompt_len && !history_len && !repetition && !frequency && !presence),
                     "%s: lengths or penalties without a history", what);
     ASDSL_CHECK_ARG(!bias || bias_stride == 0 || bias_stride >= vocab,
