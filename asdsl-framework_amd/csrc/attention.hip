@@ -859,8 +859,9 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
 // waves share each 32 keys through LDS, where K and V lie as the operands are
 // read, 16 bytes a lane; int8 codes are turned into fp16 on the way.  Waves 0 and
 // 1 bring 64 dims of V each (turned in registers), waves 2 and 3 16 keys of K.
-// Two buffers: the next keys' loads run during a tile's products and are
-// written to the other buffer after them, one barrier a tile.
+// Four buffers in a ring: a tile's loads are started two tiles ahead, run during
+// its products and are written behind them, so that waves may be two tiles
+// apart and one barrier does for two tiles.
 //
 // A lane holds one row n = lane % 32 and, with h = lane / 32, the keys
 // wide_key(i, h) of a tile's score registers i = 0..15; operand step s of the
@@ -1025,18 +1026,9 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
     Softmax<false, 32> st;
     f32x16 acc[D / 32];
-    // int8: the power of two that keeps the wave's weights times value scales in
-    // fp16's range (acc is 2^-ev times O'), and the rows that any of its rows sees
-    int ev = kEvLow, p_top = INT_MAX, lo_low = 0;
-    if (Q8 && K.masked) {
-        p_top = n < map.total ? see.p : -1;
-        lo_low = n < map.total && see.any ? see.lo : INT_MAX;
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) {
-            p_top = max(p_top, __shfl_xor(p_top, x, kWave));
-            lo_low = min(lo_low, __shfl_xor(lo_low, x, kWave));
-        }
-    }
+    // int8: the power of two that keeps the row's weights times the value scales it
+    // sees in fp16's range (acc is 2^-ev times O'), and the least of the wave's
+    int ev = kEvLow, ev_low = kEvLow;
 #pragma unroll
     for (int u = 0; u < D / 32; ++u)
 #pragma unroll
@@ -1088,9 +1080,11 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                 }
             }
         }
-        constexpr bool kBoth = !Q8 || D == 64;  // registers for both of V's steps
+        constexpr bool kBoth = !Q8;  // registers for both of V's steps (with int8 codes they would spill)
+        if constexpr (kBoth) {
 #pragma unroll
-        for (int u = 0; u < (kBoth ? D / 16 : D / 32); ++u) o[u] = s.v[u % (D / 32)][u / (D / 32)][h][lane & 31];
+            for (int u = 0; u < D / 16; ++u) o[u] = s.v[u % (D / 32)][u / (D / 32)][h][lane & 31];
+        }
         __builtin_amdgcn_sched_barrier(0);
         const bool all = all_seen(K, t * kKeys, kKeys);
         uint32_t seen = 0xFFFFu;
@@ -1102,29 +1096,36 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
             for (int u = 0; u < D / 32; ++u) acc[u] *= alpha;
         }
         if constexpr (Q8) {
-            // A value scale a lane.  One that no row of the wave sees may be anything;
-            // one that is no number of any use makes its weights infinite.
-            const int key = lane / (D / 64) % kKeys, i = t * kKeys + key, row = cache_row(K, i);
-            const float a = fabsf(s.vs[lane % (D / 64)][key]);
-            const bool ok = (i < K.n) & (a < 1e30f) & (row <= p_top) & ((row >= lo_low) | (row < K.sinks));
-            if (__builtin_amdgcn_ballot_w64(ok & (exponent(a) > ev)) != 0ull) {
-                float top = ok ? a : 0.0f;
+            // A value scale a lane; then each row by the keys that it sees, whose scales
+            // may be anything else.  One of no use makes its weights infinite.
+            const float any = fabsf(s.vs[lane % (D / 64)][lane / (D / 64) % kKeys]);
+            if (__builtin_amdgcn_ballot_w64(exponent(any) > ev_low) != 0ull) {
+                float top = 0.0f;
+#pragma unroll 1
+                for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-                for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x, kWave));
-                const int e1 = max(ev, uniform(exponent(top)));
+                    for (int i = 0; i < 16; ++i) {
+                        const float a = fabsf(s.vs[b][wide_key(i, h)]);
+                        top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
+                    }
+                top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                const int e1 = max(ev, exponent(top));
                 const float f = pow2(max(ev - e1, -126));
 #pragma unroll
                 for (int u = 0; u < D / 32; ++u) acc[u] *= f;
-                ev = e1;
+                ev = ev_low = e1;
+#pragma unroll
+                for (int x = 16; x >= 1; x >>= 1) ev_low = min(ev_low, __shfl_xor(ev_low, x, kWave));
+                ev_low = uniform(ev_low);
             }
         }
         st.weigh(p, q.c);
         Weights<D, Q8> w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            if (!kBoth && e) {
+            if (!kBoth) {
 #pragma unroll
-                for (int u = 0; u < D / 32; ++u) o[u] = s.v[u][1][h][lane & 31];
+                for (int u = 0; u < D / 32; ++u) o[u] = s.v[u][e][h][lane & 31];
             }
             float vs[8][D / 64];
             if constexpr (Q8) {

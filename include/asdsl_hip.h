@@ -639,7 +639,9 @@ asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, const int* to
  * caches are such caches with n_seq = 1); queries and outputs are fp32
  * [n_seq * n_tokens][n_heads][head_dim], token t of sequence s in row
  * s * n_tokens + t.  head_dim is 64 or 128, n_heads any multiple of n_kv_heads.
- * qkv, q, out, q_out and the caches are 16-byte aligned.  Work buffers are the
+ * qkv, q, out, q_out and the caches are 16-byte aligned.  An int8 cache's value
+ * scales that a query row sees are finite and below 1e30; values whose scale is
+ * 2^-s of the largest that the row sees are held to 2^-min(22, 33 - s).  Work buffers are the
  * caller's (256-byte aligned, the size from the *_work_bytes query, contents
  * afterwards unspecified; null where the query gives 0): calls that may
  * overlap, two captured graphs among them, take one each.  Nothing is
