@@ -102,6 +102,14 @@ def _heads(fn: str, q, head_dim: int, n_rows: int, what: str = "q") -> int:
     return n // (n_rows * head_dim)
 
 
+def _count(fn: str, name: str, v) -> int:
+    """A length that the C ABI takes as an int."""
+    n = int(v)
+    if not 0 <= n < 1 << 31:
+        raise ValueError(f"{fn}: {name} must be in [0, 2^31), got {n}")
+    return n
+
+
 def _work(nbytes: int, like):
     """A work buffer of this call on its stream (None where it needs none)."""
     return like.new_empty(nbytes, dtype=_u8) if nbytes else None
@@ -133,7 +141,7 @@ def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, p
     queries are zero."""
     fn = "kv_append"
     n_seq, n_kv, rows, d = _cache_dims(fn, "kv", k_cache, v_cache)
-    n_heads = int(n_heads)
+    n_heads, pos_offset = int(n_heads), _count(fn, "pos_offset", pos_offset)
     if n_heads <= 0 or n_heads % n_kv:
         raise ValueError(f"{fn}: n_heads must be a multiple of the caches' {n_kv} heads")
     if not isinstance(qkv, _Tensor) or qkv.numel() == 0 or qkv.numel() % (n_seq * (n_heads + 2 * n_kv) * d):
@@ -151,7 +159,7 @@ def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, p
         q_out = qkv.new_empty((tokens, n_heads * d))
     _hip.call("asdsl_kv_append_f16" if k_scale is None else "asdsl_kv_append_q8", *at,
               _addr(fn, dev, "q_out", q_out, _f32, tokens * n_heads * d), n_seq, tokens // n_seq, n_heads, n_kv, d,
-              2 * half, rows, int(pos_offset), rope_rows, _stream(dev))
+              2 * half, rows, pos_offset, rope_rows, _stream(dev))
     return q_out
 
 
@@ -173,7 +181,7 @@ def attention_window(q, k_cache, v_cache, pos, *, window: int = 0, sinks: int = 
         raise ValueError(f"{fn}: q must be [..., n_heads, {d}] or [tokens, n_heads * {d}], n_heads a multiple of {n_kv}")
     n = q.numel()
     tokens = per_seq // n_heads
-    dims = (n_seq, tokens, n_heads, n_kv, d, rows, int(window), int(sinks))
+    dims = (n_seq, tokens, n_heads, n_kv, d, rows, _count(fn, "window", window), _count(fn, "sinks", sinks))
     dev = _device(q)
     at = (_addr(fn, dev, "q", q, _f32, n), *_caches(fn, dev, "kv", k_cache, v_cache, k_scale, v_scale, d),
           _addr(fn, dev, "pos", pos, _i32, n_seq))

@@ -56,6 +56,8 @@ def control_logits(logits, *, history=None, prompt_len=None, history_len=None, r
         raise ValueError(f"{fn}: history must be a device tensor [{rows}, ids]")
     else:
         cap = history.shape[-1]
+        if cap > 1 << 30:
+            raise ValueError(f"{fn}: a history of at most 2^30 ids a row")
     words = (vocab + 31) // 32
     strides = []
     for name, t, width in (("bias", bias, vocab), ("allowed", allowed, words)):

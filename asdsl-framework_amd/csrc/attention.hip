@@ -1180,6 +1180,10 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
             for (int u = 0; u < D / 32; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
+            if constexpr (!Q8) {  // a row that sees nothing meets the tile's keys where all others see them
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) bad[e] = 0u;
+            }
         }
         dst = g.out + at * D;
     } else {
@@ -1347,6 +1351,8 @@ asdsl_status with_form(int head_dim, bool q8, F f) {
     return q8 ? f(integral_constant<int, 64>{}, std::true_type{}) : f(integral_constant<int, 64>{}, std::false_type{});
 }
 
+constexpr int kMaxRows = 1 << 30;  // rows seen, so that a tile past the last of them is an int
+
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 asdsl_status check_heads(const char* what, int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
@@ -1510,7 +1516,7 @@ asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, c
     ASDSL_CHECK_ARG(!q8 || (c.ks && c.vs), "%s: null scale array", what);
     asdsl_status st = check_heads(what, n_seq, n_tokens, n_heads, n_kv_heads, head_dim);
     if (st != ASDSL_OK) return st;
-    ASDSL_CHECK_ARG(rows > 0, "%s: rows must be positive", what);
+    ASDSL_CHECK_ARG(rows > 0 && rows <= kMaxRows, "%s: rows must be positive and at most 2^30", what);
     ASDSL_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window and sinks must not be negative", what);
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(c.k) && aligned16(c.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
@@ -1540,14 +1546,14 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
                     int prefix_len, int prefix_rows, int own_rows, void* work, size_t work_bytes,
                     asdsl_stream_t stream) {
     ASDSL_CHECK_ARG(q && own.k && own.v && own_pos && out, "%s: null pointer", what);
-    ASDSL_CHECK_ARG(prefix_len >= 0 && prefix_len <= prefix_rows,
-                    "%s: prefix_len must be in [0, prefix_rows]", what);
+    ASDSL_CHECK_ARG(prefix_len >= 0 && prefix_len <= prefix_rows && prefix_len <= kMaxRows,
+                    "%s: prefix_len must be in [0, prefix_rows] and at most 2^30", what);
     ASDSL_CHECK_ARG(prefix_len == 0 || (shared.k && shared.v), "%s: null pointer", what);
     ASDSL_CHECK_ARG(!q8 || (own.ks && own.vs && (prefix_len == 0 || (shared.ks && shared.vs))),
                     "%s: null scale array", what);
     asdsl_status st = check_heads(what, n_seq, 1, n_heads, n_kv_heads, head_dim);
     if (st != ASDSL_OK) return st;
-    ASDSL_CHECK_ARG(own_rows > 0, "%s: own_rows must be positive", what);
+    ASDSL_CHECK_ARG(own_rows > 0 && own_rows <= kMaxRows, "%s: own_rows must be positive and at most 2^30", what);
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(shared.k) && aligned16(shared.v) && aligned16(own.k) &&
                         aligned16(own.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
@@ -1594,7 +1600,7 @@ extern "C" asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, in
 extern "C" size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
                                                     int rows, int window_size, int sinks) {
     if (check_heads("attention_window", n_seq, n_tokens, n_heads, n_kv_heads, head_dim) != ASDSL_OK || rows <= 0 ||
-        window_size < 0 || sinks < 0)
+        rows > kMaxRows || window_size < 0 || sinks < 0)
         return 0;
     return plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks).work;
 }
@@ -1620,7 +1626,7 @@ extern "C" asdsl_status asdsl_attention_window_q8kv(const float* q, const int8_t
 extern "C" size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim,
                                                     int prefix_len, int own_rows) {
     if (check_heads("attention_prefix", n_seq, 1, n_heads, n_kv_heads, head_dim) != ASDSL_OK || prefix_len < 0 ||
-        own_rows <= 0)
+        prefix_len > kMaxRows || own_rows <= 0 || own_rows > kMaxRows)
         return 0;
     return plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows).work;
 }

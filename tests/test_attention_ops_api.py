@@ -137,3 +137,28 @@ def test_wrappers_refuse_what_does_not_fit():
         attention_window(q, codes, codes, pos)
     with pytest.raises(ValueError):
         attention_window(q, k, k, pos, k_scale=scale, v_scale=scale)
+
+
+def test_sizes_past_the_kernels_ints():
+    import torch
+
+    from asdsl import _hip
+    from asdsl.kernels import attention_window, control_logits, kv_append
+
+    lib = _hip.LIB
+    big = (1 << 30) + 1
+    refused(lib.asdsl_attention_window_f16kv(*(ONE,) * 5, 1, 1, 8, 2, 64, big, 0, 0, ONE, 0, None), "2^30")
+    assert lib.asdsl_attention_window_work_bytes(1, 1, 8, 2, 64, big, 0, 0) == 0
+    refused(lib.asdsl_attention_prefix_f16kv(*(ONE,) * 7, 1, 8, 2, 64, big, big, 1, ONE, 0, None), "2^30")
+    refused(lib.asdsl_attention_prefix_f16kv(*(ONE,) * 7, 1, 8, 2, 64, 1, 1, big, ONE, 0, None), "2^30")
+    assert lib.asdsl_attention_prefix_work_bytes(1, 8, 2, 64, big, 1) == 0
+    assert lib.asdsl_attention_prefix_work_bytes(1, 8, 2, 64, 1, big) == 0
+    k = torch.zeros((2, 4, 8, 128), dtype=torch.float16)
+    q, pos, cs = torch.zeros((2, 1, 8, 128)), torch.zeros(2, dtype=torch.int32), torch.zeros((8, 48))
+    for call in (lambda x: attention_window(q, k, k, pos, window=x), lambda x: attention_window(q, k, k, pos, sinks=x),
+                 lambda x: kv_append(torch.zeros(2, 16 * 128), k, k, cs, cs, pos, n_heads=8, pos_offset=x)):
+        for x in (-1, 1 << 31, (1 << 32) + 5):
+            with pytest.raises(ValueError, match=r"2\^31"):
+                call(x)
+    with pytest.raises(ValueError, match=r"2\^30"):
+        control_logits(torch.zeros(1, 40), history=torch.zeros(1, dtype=torch.int32).expand((1 << 30) + 1))

@@ -96,6 +96,30 @@ def test_unseen_rows_do_not_reach_the_output(gpu, kv, d, n, rows, win, sinks):
             assert not torch.isfinite(got[:, -1]).any()
 
 
+def test_tokens_outside_the_cache_beside_infinite_rows(gpu):
+    """A padded token shares its tiles with tokens that see every key: zero all
+    the same, where theirs are not finite."""
+    import torch
+
+    from asdsl.kernels import attention_window
+
+    rng = np.random.default_rng(9)
+    n, tokens, h, kvh, d, rows = 48, 40, 8, 8, 128, 128
+    for kv in ("fp16", "int8"):
+        k, ks, _ = make_cache(rng, kv, n, kvh, rows, d)
+        v, vs, _ = make_cache(rng, kv, n, kvh, rows, d)
+        (v if vs is None else vs)[:, :, 3] = float("inf")
+        q = dev(rng.standard_normal((n, tokens, h, d)).astype(np.float32))
+        first = [rows - 7 if i % 2 else -10 for i in range(n)]
+        got = attention_window(q, k, v, dev(np.array(first, np.int32)), k_scale=ks, v_scale=vs)
+        for i, p in enumerate(first):
+            at = np.arange(tokens) + p
+            outside = torch.from_numpy((at < 0) | (at >= rows)).cuda()
+            sees = torch.from_numpy((at >= 3) & (at < rows)).cuda()
+            assert (got[i][outside] == 0).all() and not torch.isfinite(got[i][sees]).any()
+            assert torch.isfinite(got[i][~outside & ~sees]).all()
+
+
 @pytest.mark.parametrize("tokens,rows", [(5, 300), (64, 300), (64, 6000)])
 def test_window_value_scales_of_a_wide_range(gpu, tokens, rows):
     """Value scales 2^11 apart.  A key's weight times its scale is held with an
