@@ -1433,6 +1433,14 @@ long long fill_many(long long jobs, long long rows, long long heads, long long n
     return rows * splits * 4 <= heads * n ? kFillFew : kFillFew / 2;
 }
 
+// Values of a KV head's keys that few rows take in one piece: a second launch
+// for the join costs more than the pieces save.  us a call in a graph (queued
+// one by one), whole / in pieces of 128 keys, 8 KV heads of 128 dims: 200 keys
+// 8.1 (9.5) / 9.0 (13.4), 256 8.3 (9.6) / 9.0 (13.6), 400 11.7 (11.7) / 9.1
+// (13.4); a compute unit alone draws some 32 bytes a ns.  64 dims: 512 keys 7.1
+// (9.4) / 7.0 (13.4), 1024 10.2 / 7.3.
+constexpr long long kAlone = 256 * 128;
+
 // How a call is laid out; the same for the work buffer's size and the launch.
 struct Plan {
     bool many;          // the many-rows form
@@ -1463,8 +1471,12 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, i
     p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, n, head_dim);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
-    p.splits = p.slots = splits_for(
-        p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n) : kFillFew, p.jobs, n, kMaxSlots);
+    if (!p.many && n * head_dim <= kAlone)
+        p.splits = 1;
+    else
+        p.splits = splits_for(p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n) : kFillFew,
+                              p.jobs, n, kMaxSlots);
+    p.slots = p.splits;
     p.jobs *= p.splits;
     return finish(p, head_dim);
 }
