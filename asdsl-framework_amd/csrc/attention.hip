@@ -36,6 +36,11 @@ struct Cache {
 // stored forms are its too: fp16 rounded to nearest, or per 64 dims scale =
 // amax * (1/127) (1e-12 when amax <= 1e-12) and code = round-half-even(x * (1 /
 // scale)) clamped to [-127, 127].
+//
+// Bound by HBM: 2045 tokens of 24 + 2 * 8 heads of 128 dims move 76 MB in 14.3 us
+// (5.3 TB/s; a copy of 1 GiB gets 5.15), a head per workgroup of scalar lanes took
+// 47.  16 tokens take 2.9 us, of which the launch and one chain of loads
+// (position, then tables) are nearly all.
 struct AppendArgs {
     const float* qkv;
     void* k;
@@ -141,6 +146,12 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
 //   O' = V' P' the lane's 8 weights are its operand as they stand when V's is
 //              read for the same 8 keys: every lane loads its D / 16 dims of those
 //              keys and turns the block in registers; no transposition in memory.
+// This form for few rows streams: 32 sequences of one token (24 heads of 128, 8 KV
+// heads, int8 caches, about 3300 rows each seen, 232 MB) take 52.4 us and 4.7 of
+// join, 4.4 TB/s, bound by HBM and by the bytes its waves keep on the way.  For
+// small calls a workgroup's chain of position, first keys and join in LDS counts:
+// 6.3 us at 128 keys, where a compute unit then draws 32 bytes a ns.  Keys of many
+// rows, read once per 16 of them, are left to the other form.
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -863,6 +874,15 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
 // its products and are written behind them, so that waves may be two tiles
 // apart and one barrier does for two tiles.
 //
+// 4096 tokens with a window of 2048 over up to 6000 rows (24 heads of 128, 8 KV
+// heads, fp16): 225 us, 455 TFLOP/s of the definition's products and twice that
+// in the matrix cores, which are busy 43 % of the time; two products in fp16
+// parts at the rate of a large library product would take 189.  Neither the
+// loads nor the softmax alone bounds it: left out, each takes some 25 us off.  A
+// tile of 32 keys takes 1.24 us with one workgroup on a compute unit and 2.0 with
+// two.  Two buffers and a barrier a tile took 260 us, the form for few rows 462.
+// Over int8 caches 4096 tokens take 254 us with all of 4096 rows to see.
+//
 // A lane holds one row n = lane % 32 and, with h = lane / 32, the keys
 // wide_key(i, h) of a tile's score registers i = 0..15; operand step s of the
 // weighted values takes i = 8 s .. 8 s + 7.
@@ -1295,7 +1315,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArg
     few_job<D, Q8>(g, K, map, row0, 0, 0, split, own_splits, prefix_splits + split, lds.area);
 }
 
-// One wave per query row: its partials in slot order.
+// One wave per query row: its partials in slot order, so that the result does not
+// depend on the order in which the pieces end.  2.7 us at 24 rows, which is its
+// launch and two dependent loads; 5.6 us at 8272 rows of 128 dims in 4 pieces
+// (17 MB).
 constexpr int kJoinRows = 4;  // rows (waves) of a workgroup
 constexpr int kMaxSlots = 64;
 template <int D>

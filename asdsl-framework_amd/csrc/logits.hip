@@ -37,6 +37,13 @@ struct ControlArgs {
 // first; while they come, the slice's words are counted in LDS from the row's
 // whole history (integer atomics: any order gives the same).  kVec: the rows of
 // logits, out and bias lie in whole 16-byte units.
+//
+// Bound by HBM for many rows: 64 of 200064 (history 500, masks) read and write 104
+// MB in 22.2 us and 3.5 more for the tokens in a graph, 4.7 TB/s (a copy of 1 GiB
+// gets 5.15); one pass per step of the definition took 59.  Cold and alone the
+// kernel takes 27-29.  Stores past the caches save 1.3 us here and cost as much in
+// the kernel that reads the result.  One row: 4.4 us and 2.0, launches and
+// the chain of history length, ids and counts.
 template <int kPer, bool kVec>
 __global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlArgs a) {
 #pragma clang fp contract(off)  // each step of the definition rounds by itself
@@ -165,7 +172,10 @@ __global__ __launch_bounds__(kWave) void logits_token_kernel(const unsigned long
         tokens[blockIdx.x] = best != 0ull ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
 }
 
-// Tokens a thread: 16, or 4 where 16 leave compute units without a workgroup.
+// Tokens a thread: 16, or 4 where 16 leave compute units without a workgroup (every
+// workgroup reads its row's whole history).  us in a graph with 16 / 4: 64 rows of
+// 200064 26.3 / 29.5, 256 of 32000 18.8 / 20.6, 8 of 200064 8.5 / 9.0; 4 of 200064
+// 8.0 / 7.3, one 7.5 / 6.2, 16 of 32000 8.0 / 6.4, 7 of 50257 10.8 / 6.9.
 int per_thread(int n_rows, int vocab) {
     const long long slices = (vocab + 16LL * kThreads - 1) / (16 * kThreads);
     return n_rows * slices < 256 ? 4 : 16;
