@@ -82,7 +82,9 @@ class BranchDecoder:
     # ------------------------------------------------------------ one prompt
     def start(self, prompt_ids, control: TokenControl | None = None):
         """Prefill the prompt; the first tokens are the n best of its controlled
-        logits (device int32 [n], also in self.tokens)."""
+        logits (device int32 [n], also in self.tokens).  With a mask row for
+        each continuation, each in turn takes the best that its row allows
+        and no earlier one has taken."""
         import torch
 
         eng, c = self.engine, self.engine.cfg
@@ -104,12 +106,36 @@ class BranchDecoder:
         self.history = torch.full((self.n, len(prompt) + self.own_rows + 1), -1, dtype=torch.int32, device=dev)
         self.history[:, :len(prompt)] = torch.tensor(prompt, dtype=torch.int32, device=dev)
         self.history_len = torch.full((self.n,), len(prompt), dtype=torch.int32, device=dev)
-        self._set_control(control or TokenControl())
-        first, _ = control_logits(eng.logits.reshape(1, -1), pick=False, **self._control_args(1))
-        if self.n > c.vocab or int(torch.isfinite(first).sum()) < self.n:
-            raise ValueError(f"BranchDecoder.start: fewer than {self.n} tokens to begin with")
-        self._note(torch.topk(first[0], self.n).indices.to(torch.int32))
+        try:
+            self._set_control(control or TokenControl())
+            self._note(self._first_tokens())
+        except Exception:
+            self.prefix_len = -1  # nothing to step from
+            raise
         return self.tokens
+
+    def _first_tokens(self):
+        import torch
+
+        vocab = self.engine.cfg.vocab
+        few = ValueError(f"BranchDecoder.start: fewer than {self.n} tokens to begin with")
+        if self.n > vocab:
+            raise few
+        logits = self.engine.logits.reshape(1, -1)
+        if self._allowed is None or self._allowed.numel() == (vocab + 31) // 32:  # one mask for all
+            first, _ = control_logits(logits, pick=False, **self._control_args(1))
+            if int(torch.isfinite(first).sum()) < self.n:
+                raise few
+            return torch.topk(first[0], self.n).indices.to(torch.int32)
+        rows, _ = control_logits(logits.expand(self.n, -1).contiguous(), pick=False, **self._control_args(self.n))
+        tokens = torch.empty(self.n, dtype=torch.int64, device=rows.device)
+        values = torch.empty(self.n, device=rows.device)
+        for i in range(self.n):
+            values[i], tokens[i] = rows[i].max(dim=0)
+            rows.index_fill_(1, tokens[i:i + 1], float("-inf"))
+        if not bool(torch.isfinite(values).all()):
+            raise few
+        return tokens.to(torch.int32)
 
     def _set_control(self, control: TokenControl) -> None:
         import torch

@@ -157,3 +157,31 @@ def test_refusals(gpu):
     with pytest.raises(ValueError):
         b.step()
     assert b.generate(prompt_of(5), 0) == [[], []]
+
+
+def test_a_mask_row_for_each_continuation(gpu):
+    """Every choice, the first among them, is one that the continuation's own row allows."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    n = 5
+    b = BranchDecoder(engine(), n, 6)
+    v = np.arange(VOCAB)
+    may = np.stack([v % n == j for j in range(n)])
+    may[4] = may[3]  # two rows with one set: distinct first tokens
+    words = np.packbits(may, axis=1, bitorder="little").view(np.int32)
+    out = b.generate(prompt_of(20), control=TokenControl(allowed=torch.from_numpy(words)), eos=())
+    assert all(may[j, t] for j in range(n) for t in out[j]) and out[3][0] != out[4][0]
+    other = engine()  # the first tokens are each row's best after the prompt
+    other.prefill(prompt_of(20))
+    want = other.logits.reshape(-1).cpu().numpy()
+    for j in range(4):
+        assert out[j][0] == int(np.argmax(np.where(may[j], want, -np.inf)))
+    assert out[4][0] == int(np.argmax(np.where(may[4] & (v != out[3][0]), want, -np.inf)))
+    only = np.zeros((n, VOCAB // 32), np.int32)
+    only[:, 0] = 0b1111  # four tokens for five continuations
+    with pytest.raises(ValueError, match="fewer than"):
+        b.start(prompt_of(20), TokenControl(allowed=torch.from_numpy(only)))
+    with pytest.raises(RuntimeError):  # and nothing to step from
+        b.step()
