@@ -1430,28 +1430,45 @@ int splits_for(long long fill, long long jobs, long long n, int most) {
     return s > 1 ? static_cast<int>(s) : 1;
 }
 
-// Which form takes `total` rows of each of `heads` KV heads over at most n keys.
-// The few-rows form reads the keys once per 16 rows and streams better, the
-// many-rows form once per 128.  us a call in a graph, few / many rows, 8 KV
-// heads of 128 dims, by total x keys: 12 x 1000 10.2 / 13.5, 96 x 1000 14.2 /
-// 17.1, 24 x 8000 20.5 / 23.0, 33 x 8000 28.5 / 24.2, 66 x 8000 31.7 / 29.2; of
-// 16 sequences 12 x 2000 27.2 / 35.5, 18 x 2000 42.4 / 35.8.  64 dims, where
-// more of its waves fit a compute unit: 192 x 1000 11.8 / 14.9, 129 x 8000 27.4 /
-// 28.6, 192 x 8000 34.8 / 31.4.  So it goes by the few-rows form's steps.
-bool takes_many(long long total, long long heads, long long n, int head_dim) {
+// Which form takes `total` rows of each of `heads` KV heads over about `keys` keys
+// each.  The few-rows form reads the keys once per 16 rows and streams better, the
+// many-rows form once per 128, whole or not, and is some 6 us slower to start: it
+// pays where the steps of the one, 16 rows by 128 keys, exceed those of the other,
+// 128 rows by 128 keys, by more than `margin` when one of these counts as `worth`
+// of those.  Int8 keys are half the bytes, and their conversion, which the many-rows
+// form saves, is cheap beside 64 dims' softmax.  us few / many in a graph, 8 KV
+// heads, rows x keys (s: for each of s sequences, p: of a causal prompt):
+//   128 dims fp16  36 x 5000 21.2 / 20.0, 48 x 2000 15.5 / 15.9, 144 x 16000 102 / 52,
+//                  p 768 x 256 11.7 / 19.5, p 6144 x 2048 232 / 91
+//   128 dims int8  96 x 5000 24.9 / 29.4, 192 x 5000 40.8 / 35.2, 144 x 16000 77 / 64,
+//                  p 1551 x 517 24.2 / 33.0, p 6144 x 2048 158 / 112
+//   64 dims fp16   64 x 16000 23.8 / 29.3, 108 x 16000 37.1 / 32.5, 64 s 32 x 1000
+//                  32.4 / 58.5, p 2068 x 517 16.7 / 24.0, p 16384 x 4096 438 / 197
+//   64 dims int8   256 x 16000 44.6 / 52.1, 8 s 160 x 8000 107 / 145, 64 s 32 x 1000
+//                  25.3 / 75.4, p 8192 x 2048 85 / 110, p 16384 x 4096 293 / 251
+bool takes_many(long long total, long long heads, long long keys, int head_dim, bool q8) {
     if (total <= kRows) return false;
-    const long long tiles = (total + kRows - 1) / kRows;
-    return tiles * heads * ((n + kLeastKeys - 1) / kLeastKeys) > (head_dim == 128 ? 1024 : 6144);
+    const int wide = kManyWaves * kWideRows;
+    const long long pieces = heads * ((keys + kLeastKeys - 1) / kLeastKeys);
+    const long long few = (total + kRows - 1) / kRows * pieces, many = (total + wide - 1) / wide * pieces;
+    const int worth = head_dim == 128 ? (q8 ? 3 : 2) : (q8 ? 5 : 3);
+    const int margin = head_dim == 128 ? (q8 ? 1900 : 300) : (q8 ? 40000 : 3900);
+    return few - worth * many > margin;
 }
 
 // Workgroups a launch is split up to: two a compute unit.  The many-rows form's
-// partials are 16 times as large a job, so it is split to one a compute unit
-// where those of two would come to a quarter of the keys' bytes (2068 rows over
-// 1000 keys, 4 KV heads: 31 us, 41 with two; 16 sequences of 18 rows over 2000
-// keys, 8 KV heads: 48 us, 36 with two).
+// partials are 16 times as large a job, so with 128 dims it is split to one a
+// compute unit where those of two would come to a quarter of the keys' bytes (2068
+// rows over 1000 keys, 4 KV heads: 31 us, 41 with two; 16 sequences of 18 rows over
+// 2000 keys, 8 KV heads: 48 us, 36 with two).  With 64 dims a tile is shorter and
+// more of its waves fit: two pay (4096 rows over 4096 keys, 8 KV heads: 160 us, 110
+// with two) but where they alone would ask for a join of short pieces (16
+// sequences of 256 rows over 500 keys: 31 us, 37 with two).
 constexpr long long kFillFew = 512;
 
-long long fill_many(long long jobs, long long rows, long long heads, long long n) {
+long long fill_many(long long jobs, long long rows, long long heads, long long n, int head_dim) {
+    if (head_dim == 64)
+        return n <= 4 * kLeastKeys && splits_for(kFillFew / 2, jobs, n, kMaxSlots) == 1 ? kFillFew / 2 : kFillFew;
     const long long splits = splits_for(kFillFew, jobs, n, kMaxSlots);
     return rows * splits * 4 <= heads * n ? kFillFew : kFillFew / 2;
 }
@@ -1484,38 +1501,46 @@ Plan finish(Plan p, int head_dim) {
     return p;
 }
 
-Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, int rows, int window, int sinks) {
+Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, bool q8, int rows, int window,
+                 int sinks) {
     Plan p{};
     p.rows = static_cast<size_t>(n_seq) * n_tokens * n_heads;
     long long n = rows;
     if (window > 0 && static_cast<long long>(window) + sinks + n_tokens - 1 < n)
         n = static_cast<long long>(window) + sinks + n_tokens - 1;
     const long long total = static_cast<long long>(n_tokens) * (n_heads / n_kv);
-    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, n, head_dim);
+    // keys of a row tile: half of the call's own tokens' on average, or the window's
+    long long keys = n - (n_tokens < n ? n_tokens : n) / 2;
+    if (window > 0) {
+        const long long near = static_cast<long long>(window) + sinks + kManyWaves * kWideRows / (n_heads / n_kv);
+        keys = near < keys ? near : keys;
+    }
+    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, keys, head_dim, q8);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
     if (!p.many && n * head_dim <= kAlone)
         p.splits = 1;
     else
-        p.splits = splits_for(p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n) : kFillFew,
+        p.splits = splits_for(p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n, head_dim)
+                                     : kFillFew,
                               p.jobs, n, kMaxSlots);
     p.slots = p.splits;
     p.jobs *= p.splits;
     return finish(p, head_dim);
 }
 
-Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, int prefix_len, int own_rows) {
+Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, bool q8, int prefix_len, int own_rows) {
     Plan p{};
     p.rows = static_cast<size_t>(n_seq) * n_heads;
     const int group = n_heads / n_kv;
     const long long total = static_cast<long long>(n_seq) * group;
-    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim);
+    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, q8);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
     const int own_splits = splits_for(kFillFew, p.own_jobs, own_rows, kMaxSlots / 4);
     const long long jobs = (total + p.wg_rows - 1) / p.wg_rows * n_kv;
     if (prefix_len > 0)
-        p.splits = splits_for(p.many ? fill_many(jobs, p.rows, n_kv, prefix_len) : kFillFew, jobs, prefix_len,
+        p.splits = splits_for(p.many ? fill_many(jobs, p.rows, n_kv, prefix_len, head_dim) : kFillFew, jobs, prefix_len,
                               kMaxSlots - own_splits);
     p.jobs = jobs * p.splits;
     p.own_jobs *= own_splits;
@@ -1555,7 +1580,7 @@ asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, c
     ASDSL_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window and sinks must not be negative", what);
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(c.k) && aligned16(c.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
-    const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window, sinks);
+    const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, q8, rows, window, sinks);
     st = work_of(what, p, work, work_bytes, stream);
     if (st != ASDSL_OK) return st;
     AttnArgs g{q, out, nullptr, nullptr, c, c, pos, n_seq, n_tokens, n_heads, n_kv_heads, rows, rows, -1, window,
@@ -1592,7 +1617,7 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(shared.k) && aligned16(shared.v) && aligned16(own.k) &&
                         aligned16(own.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
-    const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows);
+    const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, q8, prefix_len, own_rows);
     st = work_of(what, p, work, work_bytes, stream);
     if (st != ASDSL_OK) return st;
     AttnArgs g{q, out, nullptr, nullptr, shared, own, own_pos, n_seq, 1, n_heads, n_kv_heads, prefix_rows, own_rows,
@@ -1637,7 +1662,12 @@ extern "C" size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int
     if (check_heads("attention_window", n_seq, n_tokens, n_heads, n_kv_heads, head_dim) != ASDSL_OK || rows <= 0 ||
         rows > kMaxRows || window_size < 0 || sinks < 0)
         return 0;
-    return plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks).work;
+    size_t most = 0;  // of the two cache types
+    for (const bool q8 : {false, true}) {
+        const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, q8, rows, window_size, sinks);
+        most = p.work > most ? p.work : most;
+    }
+    return most;
 }
 
 extern "C" asdsl_status asdsl_attention_window_f16kv(const float* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -1663,7 +1693,12 @@ extern "C" size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int 
     if (check_heads("attention_prefix", n_seq, 1, n_heads, n_kv_heads, head_dim) != ASDSL_OK || prefix_len < 0 ||
         prefix_len > kMaxRows || own_rows <= 0 || own_rows > kMaxRows)
         return 0;
-    return plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows).work;
+    size_t most = 0;  // of the two cache types
+    for (const bool q8 : {false, true}) {
+        const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, q8, prefix_len, own_rows);
+        most = p.work > most ? p.work : most;
+    }
+    return most;
 }
 
 extern "C" asdsl_status asdsl_attention_prefix_f16kv(const float* q, const uint16_t* k_prefix,

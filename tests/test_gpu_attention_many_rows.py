@@ -1,7 +1,8 @@
-"""Windowed and shared-prefix attention at sizes that take the kernels' form
-for many query rows (more than 16 rows a KV head over enough keys: tiles of 16
-rows, times KV heads and sequences, times 128-key pieces above 1024 for heads
-of 128 dims, above 6144 for 64), against the definitions in 64 bits."""
+"""Windowed and shared-prefix attention at sizes about the kernels' two forms,
+for few and for many query rows, against the definitions in 64 bits.  The form
+goes by rows a KV head, keys, head dim and cache type; most of the sizes here
+take the one for many rows, which for int8 caches asks for long caches (of
+which little is seen)."""
 
 from __future__ import annotations
 
@@ -31,6 +32,15 @@ WINDOW = [
     (1, 200, 16, 4, 64, "int8", 20000, [300], 0, 0),
     (6, 65, 12, 6, 64, "int8", 4000, [3935, 100, -64, 0, 3999, 77], 3900, 3),
     (40, 65, 12, 3, 64, "fp16", 200, [3 * i for i in range(40)], 170, 2),
+    (1, 64, 24, 8, 128, "int8", 8000, [700], 0, 0),
+    (1, 130, 8, 2, 128, "int8", 8000, [1900], 0, 0),
+    (20, 30, 16, 4, 128, "int8", 700, [-30, -29, -5, 0, 20, 23, 24, 300, 670, 671, 695, 699, 700, 2**31 - 9, -2**31,
+                                       64, 127, 128, 129, 255], 0, 0),
+    (60, 90, 6, 2, 128, "int8", 400, [5 * i for i in range(60)], 60, 31),
+    (1, 128, 8, 1, 64, "int8", 214000, [300], 0, 0),
+    (1, 131, 8, 1, 64, "int8", 256000, [-3], 255000, 3),
+    (130, 65, 12, 3, 64, "fp16", 200, [3 * (i % 46) for i in range(130)], 170, 2),
+    (12, 96, 12, 6, 64, "fp16", 1600, [131 * i for i in range(12)], 0, 0),
 ]
 
 
@@ -94,6 +104,65 @@ def test_unseen_rows_do_not_reach_the_output(gpu, kv, d, n, rows, win, sinks):
         check(got[:, :-1].contiguous(), want[:, :-1], bound[:, :-1], str(x))
         if not np.isfinite(x):
             assert not torch.isfinite(got[:, -1]).any()
+
+
+@pytest.mark.parametrize("d,n,tokens,h,kvh,rows,win", [(128, 1, 90, 6, 2, 16400, 0), (128, 64, 90, 6, 2, 400, 200),
+                                                     (64, 1, 128, 8, 1, 216000, 0)])
+def test_unseen_rows_of_int8_caches(gpu, d, n, tokens, h, kvh, rows, win):
+    """As above, at sizes where int8 caches take the form for many rows."""
+    import torch
+
+    from asdsl.kernels import attention_window
+
+    rng = np.random.default_rng(15)
+    p0 = 200
+    q = rng.standard_normal((n, tokens, h, d)).astype(np.float32)
+    k, ks, kw = make_cache(rng, "int8", n, kvh, rows, d)
+    v, vs, vw = make_cache(rng, "int8", n, kvh, rows, d)
+    want, bound = ref.window(q, kw, vw, [p0] * n, win, 3)
+    seen = np.zeros(rows, bool)
+    for t in range(tokens):
+        seen[ref.seen_rows(p0 + t, rows, win, 3)] = True
+    bad = np.flatnonzero(~seen)
+    for i, x in enumerate((float("nan"), float("inf"), float("-inf"), 1e20)):
+        at = torch.from_numpy(bad[i::4]).cuda()
+        ks[:, :, at], vs[:, :, at] = x, x
+    pos = dev(np.array([p0] * n, np.int32))
+
+    def call():
+        return attention_window(dev(q), k, v, pos, window=win, sinks=3, k_scale=ks, v_scale=vs)
+    check(call(), want, bound)
+    last = p0 + tokens - 1
+    for x in (float("nan"), float("inf"), 1e6, 1e20):
+        vs[:, :, last] = x
+        got = call()
+        check(got[:, :-1].contiguous(), want[:, :-1], bound[:, :-1], str(x))
+        if not np.isfinite(x):
+            assert not torch.isfinite(got[:, -1]).any()
+
+
+def test_prefix_of_a_long_int8_cache_of_narrow_heads(gpu):
+    """Some rows of a call that takes the form for many rows."""
+    from asdsl.kernels import attention_prefix
+
+    rng = np.random.default_rng(16)
+    n, h, d, plen, rows = 128, 8, 64, 214001, 5
+    q = rng.standard_normal((n, h, d)).astype(np.float32)
+    kp, kps, kpw = make_cache(rng, "int8", 1, plen + 9, d)
+    vp, vps, vpw = make_cache(rng, "int8", 1, plen + 9, d)
+    ko, kos, kow = make_cache(rng, "int8", n, 1, rows, d)
+    vo, vos, vow = make_cache(rng, "int8", n, 1, rows, d)
+    for s in (kps, vps):
+        s[:, plen:] = float("nan")
+    own = np.array([i % 6 - 1 for i in range(n)], np.int32)
+    got = attention_prefix(dev(q), kp, vp, ko, vo, dev(own), prefix_len=plen, k_prefix_scale=kps, v_prefix_scale=vps,
+                           k_scale=kos, v_scale=vos)
+    for i in (0, 1, 15, 16, 17, 127):
+        for a in (0, 7):
+            m = int(own[i]) + 1
+            want, bound = ref.attend_row(q[i, a].astype(np.float64), np.concatenate([kpw[0, :plen], kow[i, 0, :m]]),
+                                         np.concatenate([vpw[0, :plen], vow[i, 0, :m]]))
+            assert (np.abs(got[i, a].cpu().numpy() - want) <= bound).all(), (i, a)
 
 
 def test_tokens_outside_the_cache_beside_infinite_rows(gpu):
@@ -168,6 +237,9 @@ PREFIX = [
     (43, 6, 2, 128, "fp16", 9000, 8500, 140, [(i * 17) % 141 - 1 for i in range(42)] + [-2]),
     (130, 16, 16, 64, "fp16", 6000, 5999, 4, [i % 4 for i in range(130)]),
     (64, 8, 2, 64, "int8", 26000, 25601, 3, [i % 4 - 1 for i in range(64)]),
+    (96, 8, 2, 128, "int8", 8300, 8299, 5, [i % 6 - 1 for i in range(96)]),
+    (64, 16, 8, 128, "int8", 6200, 6151, 70, [(i * 13) % 71 - 1 for i in range(64)]),
+    (130, 24, 12, 64, "fp16", 5300, 5300, 4, [i % 4 for i in range(130)]),
 ]
 
 
