@@ -303,3 +303,30 @@ def test_two_graphs_at_once(gpu):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("h,n", [(64, 270_000), (12, 1_400_000)])
+def test_more_than_2_31_query_values(gpu, h, n):
+    """Queries, outputs and qkv rows past 2^31 elements, in both forms."""
+    import torch
+
+    from asdsl.kernels import attention_window, kv_append
+
+    d, rows, p = 128, 2, 1
+    assert n * h * d > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    qkv = torch.empty((n, (h + 2) * d), device="cuda").uniform_(-1, 1, generator=gen)
+    k = torch.randn((n, 1, rows, d), generator=gen, device="cuda").half()
+    v = torch.randn((n, 1, rows, d), generator=gen, device="cuda").half()
+    pos = torch.full((n,), p, dtype=torch.int32, device="cuda")
+    cos, sin = torch.ones((4, d // 2), device="cuda"), torch.zeros((4, d // 2), device="cuda")  # no turn
+    q = kv_append(qkv, k, v, cos, sin, pos, n_heads=h)
+    out = attention_window(q, k, v, pos)
+    for i in (0, 1, n // 2, n - 2, n - 1):
+        x = qkv[i].cpu().numpy().reshape(h + 2, d)
+        assert np.array_equal(q[i].cpu().numpy().reshape(h, d), x[:h])
+        kw, vw = (t[i, 0].cpu().numpy().astype(np.float64) for t in (k, v))
+        assert np.array_equal(kw[p], x[h].astype(np.float16)) and np.array_equal(vw[p], x[h + 1].astype(np.float16))
+        for a in (0, h - 1):
+            want, bound = ref.attend_row(x[a].astype(np.float64), kw, vw)
+            assert (np.abs(out[i].cpu().numpy().reshape(h, d)[a] - want) <= bound).all(), (i, a)

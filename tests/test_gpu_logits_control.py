@@ -135,3 +135,22 @@ def test_captured_and_replayed_with_a_growing_history(gpu):
         assert np.array_equal(out.cpu().numpy(), want) and np.array_equal(tokens.cpu().numpy(), best)
         hist[:, i] = tokens
         length += 1
+
+
+def test_more_than_2_31_logits(gpu):
+    import torch
+
+    from asdsl.kernels import control_logits
+
+    rows, vocab = 11_000, 200_064
+    assert rows * vocab > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((rows, vocab), device="cuda").normal_(generator=gen)
+    words = torch.randint(-2 ** 31, 2 ** 31 - 1, (rows, vocab // 32), generator=gen, device="cuda").int()
+    history = torch.randint(0, vocab, (rows, 50), generator=gen, device="cuda").int()
+    rep = torch.empty(rows, device="cuda").uniform_(1, 2, generator=gen)
+    at = [0, 1, rows // 2, rows - 1]
+    host = [t[at].cpu().numpy() for t in (x, words, history, rep)]
+    out, tokens = control_logits(x, history=history, repetition=rep, frequency=rep, allowed=words, out=x)
+    want, best = ref.control(host[0], history=host[2], repetition=host[3], frequency=host[3], allowed=host[1])
+    assert np.array_equal(out[at].cpu().numpy(), want) and np.array_equal(tokens[at].cpu().numpy(), best)
