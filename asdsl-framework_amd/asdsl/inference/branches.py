@@ -84,7 +84,9 @@ class BranchDecoder:
         """Prefill the prompt; the first tokens are the n best of its controlled
         logits (device int32 [n], also in self.tokens).  With a mask row for
         each continuation, each in turn takes the best that its row allows
-        and no earlier one has taken."""
+        and no earlier one has taken.  If it raises, the next call has to be
+        another start(), unless it refused the prompt's length (nothing was
+        touched then)."""
         import torch
 
         eng, c = self.engine, self.engine.cfg
@@ -93,10 +95,10 @@ class BranchDecoder:
             raise ValueError("BranchDecoder.start: empty prompt")
         if len(prompt) + self.own_rows > c.max_seq:
             raise ValueError("BranchDecoder.start: prompt and continuation out of kv-cache range")
+        self.prefix_len, self._steps, self._graph = -1, 0, None  # nothing to step from until all of this is done
         eng.reset_session()
         eng.prefill(prompt)
-        self.prefix_len, self._steps, self._graph = len(prompt), 0, None
-        nbytes = _hip.LIB.asdsl_decode_branches_work_bytes(ctypes.byref(eng._model), self.n, self.prefix_len,
+        nbytes = _hip.LIB.asdsl_decode_branches_work_bytes(ctypes.byref(eng._model), self.n, len(prompt),
                                                            self.own_rows)
         if nbytes == 0:
             raise ValueError(f"BranchDecoder: {_hip.last_error()}")
@@ -107,10 +109,11 @@ class BranchDecoder:
         self.history[:, :len(prompt)] = torch.tensor(prompt, dtype=torch.int32, device=dev)
         self.history_len = torch.full((self.n,), len(prompt), dtype=torch.int32, device=dev)
         try:
+            self.prefix_len = len(prompt)
             self._set_control(control or TokenControl())
             self._note(self._first_tokens())
-        except Exception:
-            self.prefix_len = -1  # nothing to step from
+        except BaseException:
+            self.prefix_len = -1
             raise
         return self.tokens
 
