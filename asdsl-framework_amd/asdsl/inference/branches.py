@@ -76,7 +76,8 @@ class BranchDecoder:
         self.tokens = torch.zeros(self.n, dtype=torch.int32, device=dev)
         self.own_pos = torch.zeros(self.n, dtype=torch.int32, device=dev)
         self.prefix_len = -1  # nothing started
-        self._steps = 0
+        self._steps = 0  # passes run
+        self._passed = False  # whether self.tokens have been through one
         self._graph = None
 
     # ------------------------------------------------------------ one prompt
@@ -184,6 +185,7 @@ class BranchDecoder:
         self.tokens.copy_(tokens)
         self.history.scatter_(1, self.history_len.long().unsqueeze(1), self.tokens.unsqueeze(1))
         self.history_len.add_(1)
+        self._passed = False
 
     # -------------------------------------------------------------- stepping
     def _forward(self) -> None:
@@ -199,37 +201,53 @@ class BranchDecoder:
         _, tokens = control_logits(self.logits, out=self.logits, **self._control_args(self.n))
         self._note(tokens)
 
-    def _room(self) -> None:
+    def _started(self) -> None:
         if self.prefix_len < 0:
             raise RuntimeError("BranchDecoder: start() has not been called")
+
+    def _room(self) -> None:
+        self._started()
         if self._steps >= self.own_rows:
             raise ValueError(f"BranchDecoder: {self.own_rows} tokens a continuation are stepped")
-        self._steps += 1
 
     def forward(self, tokens=None):
-        """One pass over self.tokens (or the given n tokens, which replace the
-        chosen ones): the n rows of logits (device [n, vocab]), nothing chosen."""
+        """One pass over self.tokens, or over the given n tokens: the n rows of
+        logits (device [n, vocab]), nothing chosen.  Given tokens take the
+        place of chosen ones that no pass has had; behind another forward()
+        they go on from its tokens.  All of them are part of the continuations,
+        as control and masks see them.  A step() behind it chooses from these
+        logits and runs no pass of its own."""
         import torch
 
         self._room()
         if tokens is not None:
             ids = [int(t) for t in tokens]
             if len(ids) != self.n or any(not 0 <= t < self.engine.cfg.vocab for t in ids):
-                self._steps -= 1
                 raise ValueError(f"BranchDecoder.forward: {self.n} tokens of the vocabulary are wanted")
-            self.tokens.copy_(torch.tensor(ids, dtype=torch.int32))
-            self.history.scatter_(1, (self.history_len - 1).long().unsqueeze(1), self.tokens.unsqueeze(1))
+            if not self._passed:
+                self.history_len.sub_(1)
+            self._note(torch.tensor(ids, dtype=torch.int32))
+        elif self._passed:
+            raise RuntimeError("BranchDecoder.forward: no tokens were given or chosen since the last pass")
         self._forward()
+        self._steps, self._passed = self._steps + 1, True
         return self.logits
 
     def step(self) -> None:
-        """One pass over self.tokens and the choice of the next ones (then in
-        self.tokens; self.logits are the controlled ones).  Queued eagerly the
-        first time and replayed from a HIP graph from the second on, as the
-        engine's steps are; token, position and history advance on the device."""
+        """One pass over self.tokens (unless forward() has run it) and the
+        choice of the next ones (then in self.tokens; self.logits are the
+        controlled ones).  Queued eagerly the first time and replayed from a
+        HIP graph from the second on, as the engine's steps are; token,
+        position and history advance on the device."""
         import torch
 
+        self._started()
+        if self._passed:
+            self._ask()
+            self._choose()
+            return
         self._room()
+        self._steps += 1
         if self._mask is not None or not self.engine.graph_calls or torch.cuda.is_current_stream_capturing():
             self._forward()
             self._ask()
@@ -247,8 +265,8 @@ class BranchDecoder:
         self._graph = graph
 
     def continuations(self) -> list[list[int]]:
-        """The tokens chosen so far, per continuation (one device read); -1
-        where nothing was allowed."""
+        """The tokens chosen or given so far, per continuation (one device
+        read); -1 where nothing was allowed."""
         return self.history[:, self.prefix_len:int(self.history_len[0])].tolist()
 
     def generate(self, prompt_ids, max_new_tokens: int | None = None, control: TokenControl | None = None,

@@ -34,3 +34,73 @@ def test_a_start_that_fails_leaves_nothing_to_step(gpu):
             b.start(bad)
     b.step()
     assert [len(r) for r in b.continuations()] == [3, 3]
+
+
+def test_forwarded_tokens_are_the_history(gpu):
+    """Tokens given to forward() are the continuations that control and masks
+    see; a step() behind a forward() chooses from that pass and runs none."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    n, steps = 3, 4
+    own = np.random.default_rng(4).permutation(VOCAB)[:n * steps].reshape(steps, n)
+    asked = []
+
+    def mask(rows):
+        asked.append([list(r) for r in rows])
+    eng, other, ids = engine(), engine(), prompt_of(30)
+    b = BranchDecoder(eng, n, steps + 1)
+    b.start(ids, TokenControl(frequency=1000.0, bias={int(t): 500.0 for t in own.flat}, allowed=mask))
+    for i in range(steps):
+        logits = b.forward(own[i])
+        assert b.continuations() == own[:i + 1].T.tolist()
+    raw = logits.cpu().numpy()
+    with pytest.raises(RuntimeError, match="chosen"):
+        b.forward()
+    b.step()
+    y = raw.copy()
+    y[:, own.reshape(-1)] += np.float32(500)
+    for j in range(n):
+        y[j, own[:, j]] = raw[j, own[:, j]] - np.float32(1000) + np.float32(500)
+    chosen = y.argmax(axis=1)
+    assert asked[-1] == own.T.tolist() and b.own_pos.tolist() == [steps] * n
+    assert b.continuations() == [[*own[:, j].tolist(), int(chosen[j])] for j in range(n)]
+    # that token is passed once, in the next row
+    b.step()
+    assert b.own_pos.tolist() == [steps + 1] * n and [len(r) for r in b.continuations()] == [steps + 2] * n
+    other.prefill(ids)
+    for i, t in enumerate([*own[:, 1].tolist(), int(chosen[1])]):
+        other.forward_token(t, len(ids) + i)
+    at = len(ids)
+    assert torch.equal(b.k[0, 1], other.layers[0]["k_cache"][:, at:at + steps + 1])
+    # full: nothing more is passed or chosen
+    for call in (b.step, lambda: b.forward([1] * n)):
+        with pytest.raises(ValueError, match="stepped"):
+            call()
+
+
+def test_forward_between_steps(gpu):
+    """Steps (queued, then replayed), a pass over the chosen tokens or over
+    others in their place, and the choice behind it: the plain steps' run."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    control = TokenControl(repetition=1.3, frequency=0.5, presence=0.1)
+    plain, mixed = (BranchDecoder(engine("int8"), 4, 12) for _ in range(2))
+    for b in (plain, mixed):
+        b.start(prompt_of(25), control)
+    for _ in range(12):
+        plain.step()
+    for i in range(6):
+        mixed.step()
+        mixed.forward() if i % 2 else mixed.forward(mixed.tokens.tolist())
+        mixed.step()
+    assert mixed.continuations() == plain.continuations() and mixed.own_pos.tolist() == plain.own_pos.tolist()
+    assert torch.equal(mixed.k, plain.k) and torch.equal(mixed.logits, plain.logits)
+    # a token in place of the chosen one
+    mixed.start(prompt_of(25), control)
+    first = mixed.continuations()
+    mixed.forward([7, 8, 9, 10])
+    assert mixed.continuations() == [[7], [8], [9], [10]] != first
