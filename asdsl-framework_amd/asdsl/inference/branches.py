@@ -168,7 +168,11 @@ class BranchDecoder:
     def _ask(self) -> None:
         """A callable mask's words for the next choice."""
         if self._mask is not None:
+            import torch
+
             words = self._mask(self.continuations())
+            if words is not None and not isinstance(words, torch.Tensor):
+                raise ValueError("TokenControl: allowed must give int32 mask words or None")
             self._allowed = None if words is None else words.to(self.tokens.device).contiguous()
 
     def _control_args(self, rows: int) -> dict:
@@ -238,7 +242,8 @@ class BranchDecoder:
         choice of the next ones (then in self.tokens; self.logits are the
         controlled ones).  Queued eagerly the first time and replayed from a
         HIP graph from the second on, as the engine's steps are; token,
-        position and history advance on the device."""
+        position and history advance on the device.  Where a mask raises or
+        gives no mask the pass has run, and another step() asks again."""
         import torch
 
         self._started()
@@ -247,17 +252,16 @@ class BranchDecoder:
             self._choose()
             return
         self._room()
-        self._steps += 1
-        if self._mask is not None or not self.engine.graph_calls or torch.cuda.is_current_stream_capturing():
-            self._forward()
-            self._ask()
-            self._choose()
-            return
-        if self._graph is not None:
+        graphs = self._mask is None and self.engine.graph_calls and not torch.cuda.is_current_stream_capturing()
+        if graphs and self._graph is not None:
             self._graph.replay()
+            self._steps += 1
             return
-        self._forward()
+        self.forward()  # if the choice fails, the next step() has only that left to do
+        self._ask()
         self._choose()
+        if not graphs:
+            return
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._forward()

@@ -104,3 +104,33 @@ def test_forward_between_steps(gpu):
     first = mixed.continuations()
     mixed.forward([7, 8, 9, 10])
     assert mixed.continuations() == [[7], [8], [9], [10]] != first
+
+
+@pytest.mark.parametrize("words", [None, 3, "text"])
+def test_a_mask_that_fails_leaves_the_step_undone(gpu, words):
+    """A mask that raises once, or gives what is no mask: the step can be
+    taken again."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    failed = []
+
+    def mask(rows):
+        if len(rows[0]) == 3 and not failed:
+            failed.append(True)
+            if words is None:
+                raise KeyError("grammar")
+            return torch.zeros(words, dtype=torch.int32) if words == 3 else words
+        return None
+    plain, b = (BranchDecoder(engine(), 3, 6) for _ in range(2))
+    plain.start(prompt_of(20))
+    b.start(prompt_of(20), TokenControl(allowed=mask))
+    for i in range(6):
+        plain.step()
+        if i == 2:
+            with pytest.raises((KeyError, ValueError)):
+                b.step()
+        b.step()
+    assert failed and b.continuations() == plain.continuations()
+    assert b.own_pos.tolist() == plain.own_pos.tolist() and torch.equal(b.k, plain.k)
