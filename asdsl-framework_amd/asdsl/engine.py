@@ -316,6 +316,10 @@ class DecodeEngine:
         # the prompt's last pass, (tokens, start), until verify_next_tokens
         # forms its tokens; () once its K/V rows were cut or overwritten
         self._prompt_pass: tuple | None = None
+        # rows [0, _held_rows) are read by a BranchDecoder between its calls;
+        # _rows_version counts the changes of any of them
+        self._held_rows = 0
+        self._rows_version = 0
         self._prefill_work = None  # work buffer of a prefill chunk of up to _prefill_tokens tokens
         self._prefill_tokens = 0
         # ASDSL_ENGINE_PROFILE / ASDSL_ENGINE_PROFILE_TOKEN, read like the
@@ -542,6 +546,7 @@ class DecodeEngine:
         # memory must not go to that stream's next tensor before they are done.
         self._prefill_work.record_stream(torch.cuda.current_stream())
         ids = torch.tensor(toks, dtype=torch.int32).to(self.token.device)
+        self._rows_change(0)
         stream = _hip.stream_handle()
         for pos in range(0, len(toks), chunk):
             n = min(chunk, len(toks) - pos)
@@ -742,6 +747,7 @@ class DecodeEngine:
                 "logits": torch.empty((self.MAX_VERIFY_TOKENS, c.vocab), dtype=torch.float32, device=dev),
             }
         v = self._verify
+        self._rows_change(start_pos)
         v["tokens"][:n].copy_(torch.tensor(toks, dtype=torch.int32))
         self.pos.fill_(start_pos)
 
@@ -771,10 +777,11 @@ class DecodeEngine:
         if self._prompt_pass == ():
             raise RuntimeError("verify_next_tokens: the prompt's K/V rows were cut or overwritten since its prefill")
         if self._prompt_pass:
-            pos, host_pos, kv_len = self.pos.clone(), self._host_pos, self.kv_seq_len
+            pos = self.pos.clone()
+            host = self._host_pos, self.kv_seq_len, self._held_rows, self._rows_version  # the rows keep their bits
             self.forward_batch_all_logits(*self._prompt_pass)
             self.pos.copy_(pos)
-            self._host_pos, self.kv_seq_len = host_pos, kv_len
+            self._host_pos, self.kv_seq_len, self._held_rows, self._rows_version = host
         if self._verify is None:
             raise RuntimeError("verify_next_tokens: no multi-token pass yet")
         return [int(t) for t in self._verify["next"][: self._verify_n].tolist()]
@@ -782,9 +789,18 @@ class DecodeEngine:
     # ------------------------------------------------------------ KV bookkeeping
     def _rows_change(self, from_pos: int) -> None:
         """K/V rows from from_pos on are about to change."""
+        if from_pos < self._held_rows:
+            self._held_rows, self._rows_version = 0, self._rows_version + 1
         p = self._prompt_pass
         if p and from_pos < p[1] + len(p[0]):
             self._prompt_pass = ()
+
+    def hold_rows(self, n: int) -> int:
+        """The version of K/V rows [0, n), which a caller reads between its
+        own calls: _rows_version differs from it once any row that was held
+        has changed."""
+        self._held_rows = max(self._held_rows, int(n))
+        return self._rows_version
 
     def get_kv_seq_len(self) -> int:
         return self.kv_seq_len

@@ -45,7 +45,9 @@ class BranchDecoder:
     """n continuations of one prompt of at most max_new_tokens tokens each.
 
     store: a weight store or a DecodeEngine, whose caches hold the prompt's
-    rows and must not be changed between start() and the last step()."""
+    rows.  An engine call that changes any of them between start() and the
+    last step(), another decoder's start() among them, ends the run: the next
+    step() or forward() raises RuntimeError."""
 
     CHUNK = 16  # steps between two reads of the device's tokens in generate()
 
@@ -99,6 +101,7 @@ class BranchDecoder:
         self.prefix_len, self._steps, self._graph = -1, 0, None  # nothing to step from until all of this is done
         eng.reset_session()
         eng.prefill(prompt)
+        self._rows = eng.hold_rows(len(prompt))
         nbytes = _hip.LIB.asdsl_decode_branches_work_bytes(ctypes.byref(eng._model), self.n, len(prompt),
                                                            self.own_rows)
         if nbytes == 0:
@@ -208,6 +211,8 @@ class BranchDecoder:
     def _started(self) -> None:
         if self.prefix_len < 0:
             raise RuntimeError("BranchDecoder: start() has not been called")
+        if self._rows != self.engine._rows_version:
+            raise RuntimeError("BranchDecoder: the engine's prompt rows have changed since start()")
 
     def _room(self) -> None:
         self._started()

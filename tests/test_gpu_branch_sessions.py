@@ -134,3 +134,34 @@ def test_a_mask_that_fails_leaves_the_step_undone(gpu, words):
         b.step()
     assert failed and b.continuations() == plain.continuations()
     assert b.own_pos.tolist() == plain.own_pos.tolist() and torch.equal(b.k, plain.k)
+
+
+def test_the_engines_rows_changed_under_the_decoder(gpu):
+    """The prompt's rows are the engine's.  Whatever changes them ends the
+    decoder's run with an error; what leaves them alone does not."""
+    from asdsl.inference.branches import BranchDecoder
+
+    eng, ids = engine(), prompt_of(30)
+    b, second = BranchDecoder(eng, 2, 12), BranchDecoder(eng, 3, 4)
+    want = b.generate(ids, eos=())
+    for change in (eng.reset_session, lambda: eng.prefill(prompt_of(5)), lambda: eng.prefill([1, 2]),
+                   lambda: eng.forward_token(5, 29), lambda: eng.forward_batch_all_logits([1, 2, 3], 28),
+                   lambda: eng.truncate_kv(29), lambda: eng.prefill_kv_random(7),
+                   lambda: (eng.truncate_kv(29), eng.step()), lambda: second.start(prompt_of(6))):
+        b.start(ids)
+        b.step()
+        change()
+        for call in (b.step, b.forward):
+            with pytest.raises(RuntimeError, match="rows"):
+                call()
+    second.step()  # the newer one goes on, also behind a change of rows that only the older one had
+    eng.step()
+    second.step()
+    b.start(ids)
+    for harmless in (lambda: eng.forward_token(5, 30), lambda: eng.truncate_kv(30), eng.step, eng.verify_next_tokens,
+                     lambda: eng.forward_batch_all_logits([1, 2, 3], 40), eng.snapshot_kv, eng.capture, eng.next_token):
+        b.step()
+        harmless()
+    while len(b.continuations()[0]) < 12:
+        b.step()
+    assert b.continuations() == want
