@@ -107,6 +107,7 @@ class BranchDecoder:
         if nbytes == 0:
             raise ValueError(f"BranchDecoder: {_hip.last_error()}")
         dev = self.tokens.device
+        self._stream = _hip.stream_handle()  # which allocates what follows
         self._work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         self.own_pos.zero_()
         self.history = torch.full((self.n, len(prompt) + self.own_rows + 1), -1, dtype=torch.int32, device=dev)
@@ -213,6 +214,15 @@ class BranchDecoder:
             raise RuntimeError("BranchDecoder: start() has not been called")
         if self._rows != self.engine._rows_version:
             raise RuntimeError("BranchDecoder: the engine's prompt rows have changed since start()")
+        if _hip.stream_handle() != self._stream:
+            import torch
+
+            # The next start() replaces these while launches queued here may
+            # still use them: their memory must not go to the next tensor of
+            # the stream that allocated them before those are done.
+            for t in (self._work, self.history, self.history_len, self._bias, self._allowed, *self._control.values()):
+                if t is not None:
+                    t.record_stream(torch.cuda.current_stream())
 
     def _room(self) -> None:
         self._started()

@@ -165,3 +165,45 @@ def test_the_engines_rows_changed_under_the_decoder(gpu):
     while len(b.continuations()[0]) < 12:
         b.step()
     assert b.continuations() == want
+
+
+def test_buffers_outlive_their_launches(gpu, monkeypatch):
+    """A start() replaces buffers that steps queued on another stream may still
+    use: their memory is not handed out again on the stream that allocated
+    them while those steps have not run."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    eng = engine()
+    eng.graph_calls = False  # to drop a graph waits for its replays
+    b = BranchDecoder(eng, 4, 8)
+    control = TokenControl(repetition=1.2)
+    b.start(prompt_of(40), control)
+    torch.cuda.synchronize()
+    sizes = {t.data_ptr(): t.numel() * t.element_size()
+             for t in (b._work, b.history, b.history_len, *b._control.values())}
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    got, kept, full, upload = [], [], torch.full, torch.tensor
+
+    def later(*a, **k):
+        """Called by start() behind each buffer that it has replaced."""
+        with torch.cuda.stream(main):
+            kept.extend(torch.empty(n, dtype=torch.uint8, device="cuda") for n in sizes.values())
+        got.extend(t.data_ptr() for t in kept)
+        return full(*a, **k)
+
+    def aside(*a, **k):  # an upload on the side stream would wait for its work
+        with torch.cuda.stream(main):
+            return upload(*a, **k)
+    with torch.cuda.stream(side):
+        b.step()
+        b.step()
+        torch.cuda._sleep(400_000_000)
+        with monkeypatch.context() as m:
+            m.setattr(eng, "prefill", lambda tokens: None)
+            m.setattr(torch, "full", later)
+            m.setattr(torch, "tensor", aside)
+            b.start(prompt_of(41), control)
+    assert len(got) > 3 * len(sizes) and not set(got) & set(sizes)
+    torch.cuda.synchronize()
