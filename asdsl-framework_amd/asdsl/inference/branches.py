@@ -85,9 +85,10 @@ class BranchDecoder:
     # ------------------------------------------------------------ one prompt
     def start(self, prompt_ids, control: TokenControl | None = None):
         """Prefill the prompt; the first tokens are the n best of its controlled
-        logits (device int32 [n], also in self.tokens).  With a mask row for
-        each continuation, each in turn takes the best that its row allows
-        and no earlier one has taken.  If it raises, the next call has to be
+        logits (device int32 [n], also in self.tokens), all different: each
+        continuation in turn takes the best (as control_logits chooses) that
+        its mask allows and no earlier one has taken, and where none is left
+        ValueError is raised.  If it raises, the next call has to be
         another start(), unless it refused the prompt's length (nothing was
         touched then)."""
         import torch
@@ -123,26 +124,30 @@ class BranchDecoder:
         return self.tokens
 
     def _first_tokens(self):
+        """Each continuation in turn takes the token that control_logits
+        chooses among those that its mask allows and no earlier one has taken."""
         import torch
 
         vocab = self.engine.cfg.vocab
-        few = ValueError(f"BranchDecoder.start: fewer than {self.n} tokens to begin with")
-        if self.n > vocab:
-            raise few
         logits = self.engine.logits.reshape(1, -1)
         if self._allowed is None or self._allowed.numel() == (vocab + 31) // 32:  # one mask for all
-            first, _ = control_logits(logits, pick=False, **self._control_args(1))
-            if int(torch.isfinite(first).sum()) < self.n:
-                raise few
-            return torch.topk(first[0], self.n).indices.to(torch.int32)
-        rows, _ = control_logits(logits.expand(self.n, -1).contiguous(), pick=False, **self._control_args(self.n))
+            rows, _ = control_logits(logits, pick=False, **self._control_args(1))
+            rows = rows.expand(self.n, -1)
+        else:
+            rows, _ = control_logits(logits.expand(self.n, -1).contiguous(), pick=False, **self._control_args(self.n))
+        open_ = torch.ones(vocab, dtype=torch.bool, device=rows.device)
         tokens = torch.empty(self.n, dtype=torch.int64, device=rows.device)
         values = torch.empty(self.n, device=rows.device)
         for i in range(self.n):
-            values[i], tokens[i] = rows[i].max(dim=0)
-            rows.index_fill_(1, tokens[i:i + 1], float("-inf"))
-        if not bool(torch.isfinite(values).all()):
-            raise few
+            left = rows[i].masked_fill(~open_, float("-inf"))
+            _, token = control_logits(left)
+            tokens[i:i + 1] = token.clamp(min=0)
+            values[i:i + 1] = left.index_select(0, tokens[i:i + 1])
+            open_.index_fill_(0, tokens[i:i + 1], False)
+        taken = (values > float("-inf")).tolist()
+        if not all(taken):
+            raise ValueError(f"BranchDecoder.start: fewer than {self.n} tokens to begin with: none is left for "
+                             f"continuation {taken.index(False)}")
         return tokens.to(torch.int32)
 
     def _set_control(self, control: TokenControl) -> None:

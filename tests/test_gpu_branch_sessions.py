@@ -207,3 +207,34 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
             b.start(prompt_of(41), control)
     assert len(got) > 3 * len(sizes) and not set(got) & set(sizes)
     torch.cuda.synchronize()
+
+
+def test_first_tokens_by_the_rule_of_every_choice(gpu):
+    """The largest controlled logits, ties to the lower token, a NaN never, as
+    control_logits takes them one by one; one mask for all, or a row each."""
+    import torch
+
+    from asdsl.inference.branches import BranchDecoder, TokenControl
+
+    tied = [1500, 700, 41, 9, 3, 2047]
+    level = torch.zeros(VOCAB)
+    level[tied] = 1e9  # the logits beside it are less than half a step
+    level[5] = float("nan")
+    for rows in (False, True):
+        words = torch.full((4, VOCAB // 32) if rows else (VOCAB // 32,), -1, dtype=torch.int32)
+        for n, want in ((1, [3]), (4, [3, 9, 41, 700])):
+            b = BranchDecoder(engine(), n, 2)
+            b.start(prompt_of(20), TokenControl(bias=level, allowed=words[:n] if rows else words))
+            assert b.tokens.tolist() == want and b.continuations() == [[t] for t in want]
+    level[8] = float("inf")
+    b = BranchDecoder(engine(), 3, 2)
+    b.start(prompt_of(20), TokenControl(bias=level))
+    assert b.tokens.tolist() == [8, 3, 9]
+    # a row whose only token an earlier one took
+    may = np.zeros((2, VOCAB // 32), np.int32)
+    may[0, 0], may[1, 0] = 0b11, 0b01
+    b = BranchDecoder(engine(), 2, 2)
+    with pytest.raises(ValueError, match="fewer than 2 .*continuation 1"):
+        b.start(prompt_of(20), TokenControl(bias={0: 1e6}, allowed=torch.from_numpy(may)))
+    b.start(prompt_of(20), TokenControl(bias={1: 1e6}, allowed=torch.from_numpy(may)))
+    assert b.tokens.tolist() == [1, 0]
