@@ -163,12 +163,15 @@ def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, p
     return q_out
 
 
-def attention_window(q, k_cache, v_cache, pos, *, window: int = 0, sinks: int = 0, k_scale=None, v_scale=None,
-                     out=None):
+def attention_window(q, k_cache, v_cache, pos, *, n_heads: int | None = None, window: int = 0, sinks: int = 0,
+                     k_scale=None, v_scale=None, out=None):
     """Attention over KV caches with a sliding window and first tokens that stay visible.
 
     q: fp32, the tokens of the caches' sequences, sequence by sequence, each
-    n_heads heads of head_dim; caches as in kv_append.  Token t of sequence s
+    n_heads heads of head_dim: [..., n_heads, head_dim] of three dimensions or
+    more, or [tokens, n_heads * head_dim], or with n_heads given any shape.
+    (Rows of one head_dim over one KV head could be tokens of one head or one
+    token's heads: without n_heads they are refused.)  Caches as in kv_append.  Token t of sequence s
     is at position p = pos[s] + t and sees cache rows j <= p with j < sinks or
     j > p - window (window 0: all j <= p).  Returns softmax(q.K /
     sqrt(head_dim)) V in q's shape (in out if given); a token whose position
@@ -176,8 +179,13 @@ def attention_window(q, k_cache, v_cache, pos, *, window: int = 0, sinks: int = 
     fn = "attention_window"
     n_seq, n_kv, rows, d = _cache_dims(fn, "kv", k_cache, v_cache)
     per_seq = _heads(fn, q, d, n_seq)  # tokens * heads
-    n_heads = q.shape[-2] if q.dim() >= 3 and q.shape[-1] == d else q.shape[-1] // d
-    if n_heads == 0 or per_seq % n_heads or n_heads % n_kv or q.shape[-1] % d:
+    if n_heads is not None:
+        n_heads = int(n_heads)
+    elif q.dim() == 2 and n_kv == 1 and q.shape[-1] == d and per_seq > 1:
+        raise ValueError(f"{fn}: q of shape {tuple(q.shape)} over one KV head is tokens or heads: give n_heads")
+    else:
+        n_heads = q.shape[-2] if q.dim() >= 3 and q.shape[-1] == d else q.shape[-1] // d if q.shape[-1] % d == 0 else 0
+    if n_heads <= 0 or per_seq % n_heads or n_heads % n_kv:
         raise ValueError(f"{fn}: q must be [..., n_heads, {d}] or [tokens, n_heads * {d}], n_heads a multiple of {n_kv}")
     n = q.numel()
     tokens = per_seq // n_heads
