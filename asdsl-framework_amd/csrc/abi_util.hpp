@@ -78,6 +78,10 @@ asdsl_status launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 bloc
     return launch_status(what);
 }
 
+// Whether one launch takes that many workgroups: its grid is counted in work
+// items, in 32 bits.
+constexpr bool fits_launch(long long workgroups, int threads) { return workgroups <= 0xFFFFFFFFLL / threads; }
+
 // Device buffer private to the library, one per device, grown on demand;
 // every buffer it hands out stays allocated until the process ends.  Calls
 // that use it and overlap on one device (different streams, no ordering

@@ -1406,7 +1406,7 @@ asdsl_status append(const char* what, bool q8, const float* qkv, void* k, void* 
                     "%s: qkv, caches and q_out must be 16-byte aligned", what);
     const int chunks = ((n_heads + 2 * n_kv_heads) * (head_dim / 4) + kAppendThreads - 1) / kAppendThreads;
     const long long grid = static_cast<long long>(n_seq) * n_tokens * chunks;
-    ASDSL_CHECK_ARG(grid <= INT_MAX, "%s: n_seq * n_tokens * heads exceeds 2^31", what);
+    ASDSL_CHECK_ARG(fits_launch(grid, kAppendThreads), "%s: n_seq * n_tokens * heads: more than 2^32 work items", what);
     const AppendArgs a{qkv, k, v, ks, vs, rope_cos, rope_sin, pos, q_out, n_tokens, n_heads, n_kv_heads,
                        rotary_dim / 2, rows, pos_offset, rope_rows, chunks};
     const bool vec = rotary_dim % 8 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
@@ -1548,6 +1548,15 @@ Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, bool q8, int pr
     return finish(p, head_dim);
 }
 
+// The grids of the call's launches: the keys' pieces, and the join's.
+asdsl_status check_launches(const char* what, const Plan& p) {
+    static_assert(kFewWaves == kManyWaves, "one workgroup size");
+    const long long join = p.slots > 1 ? static_cast<long long>((p.rows + kJoinRows - 1) / kJoinRows) : 0;
+    ASDSL_CHECK_ARG(fits_launch(p.jobs + p.own_jobs, kFewWaves * 64) && fits_launch(join, kJoinRows * 64),
+                    "%s: too many query rows: more than 2^32 work items", what);
+    return ASDSL_OK;
+}
+
 void place_work(AttnArgs& g, const Plan& p, void* work, int head_dim) {
     if (p.work == 0) return;
     g.part = static_cast<float*>(work);
@@ -1581,12 +1590,13 @@ asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, c
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(c.k) && aligned16(c.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
     const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, q8, rows, window, sinks);
+    st = check_launches(what, p);
+    if (st != ASDSL_OK) return st;
     st = work_of(what, p, work, work_bytes, stream);
     if (st != ASDSL_OK) return st;
     AttnArgs g{q, out, nullptr, nullptr, c, c, pos, n_seq, n_tokens, n_heads, n_kv_heads, rows, rows, -1, window,
                sinks, p.splits, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    ASDSL_CHECK_ARG(p.jobs <= INT_MAX, "%s: too many query rows", what);
     const dim3 grid(static_cast<unsigned>(p.jobs));
     auto with = [&](auto dim, auto codes) {
         constexpr int kD = decltype(dim)::value;
@@ -1618,12 +1628,13 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
                         aligned16(own.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
     const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, q8, prefix_len, own_rows);
+    st = check_launches(what, p);
+    if (st != ASDSL_OK) return st;
     st = work_of(what, p, work, work_bytes, stream);
     if (st != ASDSL_OK) return st;
     AttnArgs g{q, out, nullptr, nullptr, shared, own, own_pos, n_seq, 1, n_heads, n_kv_heads, prefix_rows, own_rows,
                prefix_len, 0, 0, 0, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    ASDSL_CHECK_ARG(p.jobs + p.own_jobs <= INT_MAX, "%s: too many query rows", what);
     st = with_form(head_dim, q8, [&](auto dim, auto codes) {
         constexpr int kD = decltype(dim)::value;
         constexpr bool kQ8 = decltype(codes)::value;

@@ -6,8 +6,6 @@
 //   y = seen ? (x > 0 ? x / repetition : x * repetition) : x
 //   y = y - frequency * n;  y = n > 0 ? y - presence : y;  y = y + bias
 //   out = allowed ? y : -inf;  token = the first largest allowed y (-1: none)
-#include <climits>
-
 #include "abi_util.hpp"
 #include "device_common.hpp"
 
@@ -211,7 +209,8 @@ extern "C" asdsl_status asdsl_logits_control(const float* logits, float* out, in
                     "%s: bias_stride must be 0 or at least vocab", what);
     ASDSL_CHECK_ARG(!allowed || allowed_stride == 0 || allowed_stride >= (vocab + 31LL) / 32,
                     "%s: allowed_stride must be 0 or at least (vocab + 31) / 32", what);
-    ASDSL_CHECK_ARG(n_rows * slices_of(n_rows, vocab) <= INT_MAX, "%s: too many rows", what);
+    ASDSL_CHECK_ARG(fits_launch(n_rows * slices_of(n_rows, vocab), kThreads),
+                    "%s: too many rows: more than 2^32 work items", what);
     void* ws = nullptr;
     if (tokens) {
         ASDSL_CHECK_ARG(work, "%s: tokens need a work buffer", what);
