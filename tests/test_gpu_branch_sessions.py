@@ -183,7 +183,11 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
     torch.cuda.synchronize()
     sizes = {t.data_ptr(): t.numel() * t.element_size()
              for t in (b._work, b.history, b.history_len, *b._control.values())}
-    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), side := torch.cuda.Stream()):
+        with torch.cuda.stream(stream):  # room in the allocator: to ask the driver for more waits
+            room = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in (1 << 20, *sizes.values()) for _ in range(40)]
+            del room
+    main = torch.cuda.current_stream()
     got, kept, full, upload = [], [], torch.full, torch.tensor
 
     def later(*a, **k):
@@ -199,7 +203,7 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
     with torch.cuda.stream(side):
         b.step()
         b.step()
-        torch.cuda._sleep(400_000_000)
+        torch.cuda._sleep(1_500_000_000)
         with monkeypatch.context() as m:
             m.setattr(eng, "prefill", lambda tokens: None)
             m.setattr(torch, "full", later)
