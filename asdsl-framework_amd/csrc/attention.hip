@@ -161,7 +161,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kRows = 16;      // query rows of a wave's tile
 constexpr int kKeys = 32;      // keys of a wave's step
 constexpr float kShift = 8.0f;
-constexpr float kMost = 14.0f;  // and 2 more for an int8 cache's scales: below fp16's 2^16
+constexpr float kMost = 14.0f;
 constexpr int kFewWaves = 4;
 
 // The keys of one KV head that a workgroup's rows see between them: rows [0, na)
@@ -376,45 +376,33 @@ struct VRaw<D, true> {
 // Running state of one query row, held by the lanes of equal lane % kStep: the
 // base m of its weights exp2(score - m) and their sum over the lane's share of
 // the keys.  A base is set kShift below the row's largest score so far and
-// stays while the scores keep kMost above it at most: nearly always after a
+// stays while the scores keep kTop above it at most: nearly always after a
 // row's first keys, so that a step then needs no exchange between lanes and no
-// scaling of what was accumulated.  An int8 cache's value scales go into the
-// weights before they are cut; ev is the power of two that keeps those in
-// fp16's range (the row's accumulators are 2^-ev times O'), at least kEvLow,
-// below which scales leave no trace in a sum (2^-ev and 2^kMost have room
-// in fp32 together).
-constexpr int kEvLow = -100;
+// scaling of what was accumulated.  Over int8 caches bases are whole numbers
+// (Scaled).
 template <bool Q8, int kStep>
 struct Softmax {
+    static constexpr float kTop = Q8 ? 12.9f : kMost;
     float m = -INFINITY, l = 0.0f;
-    int ev = kEvLow;
 
-    // Whether a step's products (score = s * c) or its value scales (vs_max, the
-    // largest, seen or not) may ask for a new base, in any lane of the wave;
-    // then the base and the factor of what the row has accumulated (vs_max: the
-    // largest of use that the row sees).
+    // Whether a step's products (score = s * c) ask for a new base in this lane;
+    // top: the largest score.
     template <int N>
-    __device__ __forceinline__ bool rises(const float (&s)[N], float c, float vs_max, float& top) const {
+    __device__ __forceinline__ bool rises(const float (&s)[N], float c, float& top) const {
         top = s[0];
 #pragma unroll
         for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
         top *= c;
-        bool up = top - m > kMost;
-        if constexpr (Q8) up |= exponent(vs_max) > ev;
-        return __builtin_amdgcn_ballot_w64(up) != 0ull;
+        return top - m > kTop;
     }
-    __device__ __forceinline__ float rebase(float top, float vs_max) {
+    // The new base where any lane of the wave asks for one: how far it rose.
+    __device__ __forceinline__ float rebase(float top) {
         top = lanes_max<kStep>(top);
-        const float m1 = top - m > kMost ? top - kShift : m;
-        float alpha = m == m1 ? 1.0f : exp2_fast(m - m1);
+        const float m1 = top - m > kTop ? (Q8 ? ceilf(top) : top) - kShift : m;
+        const float up = m == m1 ? 0.0f : m1 - m;
         m = m1;
-        l *= alpha;
-        if constexpr (Q8) {
-            const int e1 = max(ev, exponent(lanes_max<kStep>(vs_max)));
-            alpha *= pow2(max(ev - e1, -126));
-            ev = e1;
-        }
-        return alpha;
+        l *= exp2_fast(-up);
+        return up;
     }
     // The weights of N keys from their products, in place.
     template <int N>
@@ -428,49 +416,91 @@ struct Softmax {
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    __device__ __forceinline__ float out_scale() const {
-        return Q8 ? pow2(ev) : 1.0f;
+};
+
+// An int8 cache's value scales go into a row's weights before those are cut into
+// fp16 parts: products of weight and scale, times a power of two 2^-ev of the
+// row's own, which puts the largest product so far at 2^8 or more, so that each is
+// held to 2^-22 of itself or 2^-33 of the largest one, however far the scales are
+// from each other and whatever weight the loud values have.  (By the largest
+// scale, a loud value of small weight takes the bits of all others.)  The
+// accumulators are 2^-ev times O'.  The base of the weights is a whole number:
+// where it rises the accumulators stay and ev falls.  A step whose weights, 2^12.9
+// at most, times scales stay below 2^15.9 by the scales' exponents alone needs no
+// look at its products: nearly every one whose scales are within 4 of the others'.
+// 4096 tokens over as many rows take 249 us, 245 by the largest scale (24 heads of
+// 128, 8 KV heads); of 64 dims 235 and 246.
+struct Scaled {
+    static constexpr int kNone = 127;  // no keys yet: no scale asks for more
+    static constexpr int kLow = -100;  // products below 2^-92 keep fewer bits
+    static constexpr int kLook = -1000;
+    int ev = kNone;
+
+    // Whether a value scale, seen or not, asks for a look at the products.
+    static __device__ __forceinline__ bool asks(float scale, int ev) { return exponent(fabsf(scale)) > ev + 2; }
+    // The row's base has risen, from no keys (first) or by `rose`.
+    __device__ __forceinline__ void rebase(bool first, float rose, bool keys) {
+        ev = !first ? ev - static_cast<int>(fminf(rose, 1000.0f)) : keys ? kLow : kNone;
+    }
+    // The power for a step whose largest product in this lane is `most`: the factor
+    // of the accumulators.
+    template <int kStep>
+    __device__ __forceinline__ float raise(float most) {
+        const int held = ev;
+        ev = max(max(held, exponent(lanes_max<kStep>(most)) - 8), kLow);
+        return pow2(max(held - ev, -126));
     }
 };
 
-// The largest value scale of the N keys that the row sees (those that are no
-// number of any use, infinite ones among them, make their weights infinite).
-template <int N, int D>
-__device__ __forceinline__ float top_scale(const float (&vs)[N][D / 64], uint32_t seen) {
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int b = 0; b < D / 64; ++b) {
-            const float a = fabsf(vs[i][b]);
-            top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
-        }
-    return top;
+// A product of a weight and a scale where the scale is of any use (others make
+// their weights infinite); zero for a key that the row does not see.
+__device__ __forceinline__ float use(float weight, float scale) {
+    const float a = fabsf(scale);
+    return a < 1e30f ? weight * a : 0.0f;
 }
 
 // O' of 16 rows: element i of acc[j] at dim *_dim(4 * (lane / 16) + i, j).
 template <int D, bool Q8>
 struct State : Softmax<Q8, 16> {
     f32x4 acc[D / 16];
+    std::conditional_t<Q8, Scaled, char> sc;
 
     __device__ __forceinline__ State() {
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ void step(float (&s)[8], float c, const float (&vs)[8][D / 64], uint32_t seen) {
-        float top, any = 0.0f;
+    __device__ __forceinline__ void step(float (&s)[8], float c, const float (&vs)[8][D / 64]) {
+        float top;
+        bool look = __builtin_amdgcn_ballot_w64(this->rises(s, c, top)) != 0ull;
+        if (look) {
+            const bool first = this->m == -INFINITY;
+            const float rose = this->rebase(top);
+            if constexpr (Q8) {
+                sc.rebase(first, rose, this->m != -INFINITY);
+            } else {
+                const float alpha = exp2_fast(-rose);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
+            }
+        }
+        this->weigh(s, c);
         if constexpr (Q8) {
+            float any = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int b = 0; b < D / 64; ++b) any = fmaxf(any, fabsf(vs[i][b]));
-        }
-        if (this->rises(s, c, any, top)) {
-            const float alpha = this->rebase(top, Q8 ? top_scale<8, D>(vs, seen) : 0.0f);
+            if (look || __builtin_amdgcn_ballot_w64(Scaled::asks(any, sc.ev)) != 0ull) {
+                float most = 0.0f;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int b = 0; b < D / 64; ++b) most = fmaxf(most, use(s[i], vs[i][b]));
+                const float f = sc.template raise<16>(most);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j) acc[j] *= f;
+            }
         }
-        this->weigh(s, c);
     }
 };
 
@@ -508,7 +538,7 @@ struct Weights {
     uint32_t h[kBlocks][4], l[kBlocks][4];
 
     // vs: the keys' value scales; one of a key that the row does not see may be
-    // anything (all: the row sees them all).  ev: the row's Softmax::ev.
+    // anything (all: the row sees them all).  ev: the row's Scaled::ev.
     __device__ __forceinline__ void cut(const float* s, const float (*vs)[D / 64], bool all, uint32_t seen, int ev) {
         if constexpr (Q8) {
             const float f = pow2(-ev);
@@ -712,9 +742,11 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, c
         const bool all = all_seen(K, t * kKeys, kKeys);  // the same in every lane
         uint32_t seen = 0xFFu;
         if (!all) seen = mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
-        st.step(s, q.c, x.vs, seen);
+        st.step(s, q.c, x.vs);
         Weights<D, Q8> w;
-        w.cut(s, x.vs, all, seen, st.ev);
+        int ev = 0;
+        if constexpr (Q8) ev = st.sc.ev;
+        w.cut(s, x.vs, all, seen, ev);
         bool odd = false;
         if constexpr (!Q8) odd = !all && __builtin_amdgcn_ballot_w64(x.v.odd()) != 0ull;
         if (__builtin_expect(!odd, 1)) {
@@ -743,15 +775,18 @@ __device__ __forceinline__ float share(float2 ml, float m) {
     return ml.y == 0.0f ? 0.0f : ml.y == ml.y ? exp2_fast(ml.x - m) : ml.y;
 }
 
-// O' times f to a row of D floats; kBlocks: operand j's dims are code_dim's.
-template <int D, bool kBlocks>
-__device__ __forceinline__ void store_row(float* dst, const f32x4 (&acc)[D / 16], int gq, float f) {
+// A state's O' to a row of D floats; over int8 caches operand j's dims are code_dim's.
+template <int D, bool Q8>
+__device__ __forceinline__ void store_row(float* dst, const State<D, Q8>& st, int gq) {
+    const auto& acc = st.acc;
+    float f = 1.0f;
+    if constexpr (Q8) f = pow2(st.sc.ev);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = 4 * gq + i;
 #pragma unroll
         for (int j = 0; j < D / 16; j += 4) {
-            const int d = kBlocks ? code_dim(r, j) : fp16_dim<D>(r, j);
+            const int d = Q8 ? code_dim(r, j) : fp16_dim<D>(r, j);
             *reinterpret_cast<float4*>(dst + d) =
                 make_float4(acc[j][i] * f, acc[j + 1][i] * f, acc[j + 2][i] * f, acc[j + 3][i] * f);
         }
@@ -792,7 +827,7 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
     const int per = ((steps + splits - 1) / splits + kFewWaves - 1) / kFewWaves * kFewWaves;
     few_rows<D, Q8>(K, q, see, split * per + wave, min(steps, (split + 1) * per), kFewWaves, lane, st);
     st.l = lanes_sum<16>(st.l);
-    store_row<D, Q8>(area.acc[wave][lane & 15], st.acc, gq, st.out_scale());
+    store_row<D, Q8>(area.acc[wave][lane & 15], st, gq);
     if (gq == 0) area.ml[wave][lane & 15] = make_float2(st.m, st.l);
     __syncthreads();
     constexpr int kPer = kRows * D / (kFewWaves * 64);  // values a thread: 8 (D 128) or 4
@@ -1044,11 +1079,10 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     Query<D, 16> q;
     q.load(n < map.total ? g.q + map.at(n) * D : nullptr, h, g.scale);
     const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
-    Softmax<false, 32> st;
+    Softmax<Q8, 32> st;
     f32x16 acc[D / 32];
-    // int8: the power of two that keeps the row's weights times the value scales it
-    // sees in fp16's range (acc is 2^-ev times O'), and the least of the wave's
-    int ev = kEvLow, ev_low = kEvLow;
+    Scaled sc;  // int8; and the least power of the wave's rows that have keys
+    int ev_low = Scaled::kNone;
 #pragma unroll
     for (int u = 0; u < D / 32; ++u)
 #pragma unroll
@@ -1110,36 +1144,37 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
         uint32_t seen = 0xFFFFu;
         if (!all) seen = mask_keys<16>(K, see, p, [&](int i) { return t * kKeys + wide_key(i, h); });
         float high;
-        if (st.rises(p, q.c, 0.0f, high)) {
-            const float alpha = st.rebase(high, 0.0f);
+        if (__builtin_amdgcn_ballot_w64(st.rises(p, q.c, high)) != 0ull) {
+            const bool first = st.m == -INFINITY;
+            const float rose = st.rebase(high);
+            if constexpr (Q8) {
+                sc.rebase(first, rose, st.m != -INFINITY);
+                ev_low = Scaled::kLook;
+            } else {
+                const float alpha = exp2_fast(-rose);
 #pragma unroll
-            for (int u = 0; u < D / 32; ++u) acc[u] *= alpha;
+                for (int u = 0; u < D / 32; ++u) acc[u] *= alpha;
+            }
         }
+        st.weigh(p, q.c);
         if constexpr (Q8) {
-            // A value scale a lane; then each row by the keys that it sees, whose scales
-            // may be anything else.  One of no use makes its weights infinite.
-            const float any = fabsf(s.vs[lane % (D / 64)][lane / (D / 64) % kKeys]);
-            if (__builtin_amdgcn_ballot_w64(exponent(any) > ev_low) != 0ull) {
-                float top = 0.0f;
+            // A value scale a lane; then each row by its products.
+            const float any = s.vs[lane % (D / 64)][lane / (D / 64) % kKeys];
+            if (__builtin_amdgcn_ballot_w64(Scaled::asks(any, ev_low)) != 0ull) {
+                float most = 0.0f;
 #pragma unroll 1
                 for (int b = 0; b < D / 64; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float a = fabsf(s.vs[b][wide_key(i, h)]);
-                        top = (seen >> i) & 1u && a < 1e30f ? fmaxf(top, a) : top;
-                    }
-                top = fmaxf(top, __shfl_xor(top, 32, kWave));
-                const int e1 = max(ev, exponent(top));
-                const float f = pow2(max(ev - e1, -126));
+                    for (int i = 0; i < 16; ++i) most = fmaxf(most, use(p[i], s.vs[b][wide_key(i, h)]));
+                const float f = sc.template raise<32>(most);
 #pragma unroll
                 for (int u = 0; u < D / 32; ++u) acc[u] *= f;
-                ev = ev_low = e1;
+                ev_low = sc.ev;
 #pragma unroll
                 for (int x = 16; x >= 1; x >>= 1) ev_low = min(ev_low, __shfl_xor(ev_low, x, kWave));
                 ev_low = uniform(ev_low);
             }
         }
-        st.weigh(p, q.c);
         Weights<D, Q8> w;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -1160,7 +1195,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                         vs[i + 3][b] = sc.w;
                     }
             }
-            w.cut(p + 8 * e, vs, all, seen >> (8 * e), ev);
+            w.cut(p + 8 * e, vs, all, seen >> (8 * e), sc.ev);
             const half8* v = &o[kBoth ? e * (D / 32) : 0];
 #pragma unroll
             for (int u = 0; u < D / 32; ++u) acc[u] = mfma(v[u], w.first(u >> 1), acc[u]);
@@ -1190,7 +1225,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     }
     if (n >= map.total) return;
     const long long at = map.at(n);
-    float f = Q8 ? pow2(ev) : 1.0f;
+    float f = Q8 ? pow2(sc.ev) : 1.0f;
     float* dst;
     if (g.slots == 1) {
         const bool any = see.any && l != 0.0f;
@@ -1217,9 +1252,9 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
         for (int i = 0; i < 8; ++i) {
             float4 o = make_float4(acc[u][i] * f, acc[u][i + 8] * f, acc[u + 1][i] * f, acc[u + 1][i + 8] * f);
             if constexpr (!Q8) {
-                const uint32_t x = (h ? bad[2 * u + 2 * (i >> 2) + 1] : bad[2 * u + 2 * (i >> 2)]) >> (8 * (i & 3));
+                const uint32_t no = (h ? bad[2 * u + 2 * (i >> 2) + 1] : bad[2 * u + 2 * (i >> 2)]) >> (8 * (i & 3));
                 const float nan = __builtin_nanf("");
-                o = make_float4(x & 1u ? nan : o.x, x & 2u ? nan : o.y, x & 4u ? nan : o.z, x & 8u ? nan : o.w);
+                o = make_float4(no & 1u ? nan : o.x, no & 2u ? nan : o.y, no & 4u ? nan : o.z, no & 8u ? nan : o.w);
             }
             *reinterpret_cast<float4*>(dst + 32 * u + 4 * wide_key(i, h)) = o;
         }

@@ -640,9 +640,10 @@ asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, const int* to
  * [n_seq * n_tokens][n_heads][head_dim], token t of sequence s in row
  * s * n_tokens + t.  head_dim is 64 or 128, n_heads any multiple of n_kv_heads.
  * qkv, q, out, q_out and the caches are 16-byte aligned.  An int8 cache's value
- * scales that a query row sees are finite and below 1e30; values whose scale is
- * 2^-s of the largest that the row sees are held to 2^-min(22, 33 - s).  Work buffers are the
- * caller's (256-byte aligned, the size from the *_work_bytes query, contents
+ * scales that a query row sees are finite and below 1e30.  A softmax weight, of
+ * an int8 cache its product with the value's scale, is held to 2^-22 of itself
+ * or 2^-33 of the row's largest one.  Work buffers are the caller's (256-byte
+ * aligned, the size from the *_work_bytes query, contents
  * afterwards unspecified; null where the query gives 0): calls that may
  * overlap, two captured graphs among them, take one each.  Nothing is
  * allocated, and a captured call replays with the positions that the device
