@@ -188,7 +188,7 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
             room = [torch.empty(n, dtype=torch.uint8, device="cuda") for n in (1 << 20, *sizes.values()) for _ in range(40)]
             del room
     main = torch.cuda.current_stream()
-    got, kept, full, upload = [], [], torch.full, torch.tensor
+    got, kept, full = [], [], torch.full
 
     def later(*a, **k):
         """Called by start() behind each buffer that it has replaced."""
@@ -197,9 +197,7 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
         got.extend(t.data_ptr() for t in kept)
         return full(*a, **k)
 
-    def aside(*a, **k):  # an upload on the side stream would wait for its work
-        with torch.cuda.stream(main):
-            return upload(*a, **k)
+    ids = torch.tensor(prompt_of(41), dtype=torch.int32, device="cuda")  # an upload would wait for the work queued
     with torch.cuda.stream(side):
         b.step()
         b.step()
@@ -207,7 +205,7 @@ def test_buffers_outlive_their_launches(gpu, monkeypatch):
         with monkeypatch.context() as m:
             m.setattr(eng, "prefill", lambda tokens: None)
             m.setattr(torch, "full", later)
-            m.setattr(torch, "tensor", aside)
+            m.setattr(torch, "tensor", lambda *a, **k: ids)
             b.start(prompt_of(41), control)
     assert len(got) > 3 * len(sizes) and not set(got) & set(sizes)
     torch.cuda.synchronize()
