@@ -239,6 +239,11 @@ __device__ __forceinline__ int exponent(float x) {
     return static_cast<int>((__builtin_bit_cast(uint32_t, x) >> 23) & 0xFFu) - 127;
 }
 
+constexpr float kLeast = 0x1p-126f;
+// The factor 2^x of what was accumulated where a larger base comes, x <= 0: never
+// zero, so that an infinite value of next to no weight stays one.
+__device__ __forceinline__ float factor(float x) { return fmaxf(exp2_fast(x), kLeast); }
+
 // x = hi + lo with fp16 parts, two at a time.
 __device__ __forceinline__ void two_parts(float x0, float x1, uint32_t& hi, uint32_t& lo) {
     const half2v h = __builtin_convertvector((f32x2{x0, x1}), half2v);
@@ -268,12 +273,6 @@ __device__ __forceinline__ half8 codes_half8(uint2 c) {
     w[2] = codes_half2(__builtin_amdgcn_perm(0u, c.y, 0x0C010C00u));
     w[3] = codes_half2(__builtin_amdgcn_perm(0u, c.y, 0x0C030C02u));
     return as_half8(w);
-}
-
-// All ones in each half of w that is an infinity or NaN (an exponent of all ones).
-__device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
-    const uint32_t t = (w & 0x7C007C00u) + 0x04000400u;
-    return (t & 0x8000u ? 0xFFFFu : 0u) | (t & 0x80000000u ? 0xFFFF0000u : 0u);
 }
 
 // A query row's operands: dims kDims * s + 8 * part .. + 8 in step s, part =
@@ -343,15 +342,6 @@ struct VRaw<D, false> {
         for (int p = 0; p < 4; ++p)
             o[p] = __builtin_amdgcn_perm(w[2 * p + 1][j >> 1], w[2 * p][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
         return as_half8(o);
-    }
-    // whether any value is an infinity or NaN (an exponent of all ones)
-    __device__ __forceinline__ bool odd() const {
-        uint32_t any = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) any |= (w[i][d] & 0x7C007C00u) + 0x04000400u;
-        return (any & 0x80008000u) != 0u;
     }
 };
 template <int D>
@@ -478,7 +468,7 @@ struct State : Softmax<Q8, 16> {
             if constexpr (Q8) {
                 sc.rebase(first, rose, this->m != -INFINITY);
             } else {
-                const float alpha = exp2_fast(-rose);
+                const float alpha = factor(-rose);
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) acc[j] *= alpha;
             }
@@ -571,25 +561,6 @@ struct Weights {
     __device__ __forceinline__ T add(half8 o, int b, T acc) const {
         b = Q8 ? b : 0;
         return mfma(o, as_half8(l[b]), mfma(o, as_half8(h[b]), acc));
-    }
-    // The same where V may hold infinities or NaN at keys that not every row
-    // sees: a weight of zero would make them NaN in every row.  They are taken
-    // out, and NaN goes to the outputs of the rows that see them.
-    __device__ __forceinline__ f32x4 add_odd(half8 o, uint32_t seen, f32x4 acc) const {
-        const uint4 v = __builtin_bit_cast(uint4, o);
-        uint32_t w[4], clean[4] = {v.x, v.y, v.z, v.w}, bad[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t mask = odd_mask(clean[i]);
-            bad[i] = mask & 0x3C003C00u;
-            clean[i] &= ~mask;
-            w[i] = ((seen >> (2 * i)) & 1u ? 0x3C00u : 0u) | ((seen >> (2 * i + 1)) & 1u ? 0x3C000000u : 0u);
-        }
-        const f32x4 hit = mfma(as_half8(bad), as_half8(w), f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-        acc = add(as_half8(clean), 0, acc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = hit[i] == 0.0f ? acc[i] : __builtin_nanf("");
-        return acc;
     }
 };
 
@@ -747,17 +718,84 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, c
         int ev = 0;
         if constexpr (Q8) ev = st.sc.ev;
         w.cut(s, x.vs, all, seen, ev);
-        bool odd = false;
-        if constexpr (!Q8) odd = !all && __builtin_amdgcn_ballot_w64(x.v.odd()) != 0ull;
-        if (__builtin_expect(!odd, 1)) {
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add_odd(x.v.operand(j), seen, st.acc[j]);
-        }
+        for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
         if (next < t1) x.load_v(K, next, lane);
     }
+}
+
+// Infinities and NaN at keys that a row sees.  The loops take the products as they
+// come: an infinite key times a second part of the query that is zero or of the
+// other sign is NaN there, and so is an infinite value times a second part of a
+// weight, or times the zero of a row that does not see it.  All of it leaves a sum
+// or an accumulator that is not finite, and finite fp16 rows never do; such a row is
+// taken again here, in fp32 and with the definition's own products: a score of
+// +inf or NaN makes the row NaN, a key of score -inf has no weight, and an infinite
+// value is its dim's at any weight above none.  A row at a time: the keys of steps
+// t0, t0 + stride, ... below t1 over the lanes, then the dims: 5.9 ms for a prompt of
+// 2048 whose every value is NaN (99 us without), 0.77 for 32 tokens over 4000 rows
+// (0.099).  O' (or, without ml, the output of a row that the call has whole) to dst,
+// base and sum to ml.
+template <int D>
+__device__ __forceinline__ void strict_row(const Keys& K, const float* row, float scale, const RowSight& see, int t0, int t1,
+                                           int stride, int lane, float* dst, float2* ml) {
+    constexpr int kDims = D / kWave;  // of a lane
+    float m = -INFINITY, l = 0.0f, acc[kDims] = {};
+#pragma unroll 1
+    for (int t = t0; t < t1; t += 2 * stride) {
+        const int step = t + (lane >> 5) * stride, key = step * kKeys + (lane & 31);
+        const int r = cache_row(K, min(key, K.n - 1));
+        const bool ok = step < t1 && key < K.n && r <= see.p && (r >= see.lo || r < K.sinks);
+        float s = 0.0f;
+        if (ok) {
+            const char* src = static_cast<const char*>(K.k) + static_cast<size_t>(r) * (2 * D);
+#pragma unroll 1
+            for (int d0 = 0; d0 < D; d0 += 64) {
+                half8 k[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const half8*>(src + 2 * d0 + 16 * j);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s = fmaf(static_cast<float>(k[j][i]), row[d0 + 8 * j + i], s);
+            }
+        }
+        s = ok ? s * scale : -INFINITY;
+        float top = s;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+        const float m1 = fmaxf(m, top), alpha = m == m1 ? 1.0f : factor(m - m1);
+        m = m1;
+        float p = exp2_fast(s - (m == -INFINITY ? 0.0f : m));
+        p = s == -INFINITY ? 0.0f : p < kLeast ? kLeast : p;
+        l = l * alpha + p;
+#pragma unroll
+        for (int e = 0; e < kDims; ++e) acc[e] *= alpha;
+        const uint64_t seen = __builtin_amdgcn_ballot_w64(ok);
+#pragma unroll 1
+        for (int i0 = 0; i0 < kWave; i0 += 16) {
+            float v[16][kDims];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const _Float16* src = static_cast<const _Float16*>(K.v) +
+                                      static_cast<size_t>(__builtin_amdgcn_readlane(r, i0 + i)) * D + kDims * lane;
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) v[i][e] = static_cast<float>(src[e]);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (((seen >> (i0 + i)) & 1ull) == 0ull) continue;
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), i0 + i));
+#pragma unroll
+                for (int e = 0; e < kDims; ++e) acc[e] = fmaf(w, v[i][e], acc[e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) l += __shfl_xor(l, o, kWave);
+    if (ml && lane == 0) *ml = make_float2(m, l);
+#pragma unroll
+    for (int e = 0; e < kDims; ++e) dst[kDims * lane + e] = ml ? acc[e] : l != 0.0f ? acc[e] / l : 0.0f;
 }
 
 // The workgroup's waves joined: their (maximum, sum) and O' through LDS, then
@@ -769,10 +807,10 @@ struct JoinArea {
     float2 ml[W][kRows];
 };
 
-// The factor of a part (base, sum) under the common base m: none without keys,
-// NaN for a sum that is NaN.
+// The factor of a part (base, sum) under the common base m: 0 without keys, NaN
+// for a sum that is NaN.
 __device__ __forceinline__ float share(float2 ml, float m) {
-    return ml.y == 0.0f ? 0.0f : ml.y == ml.y ? exp2_fast(ml.x - m) : ml.y;
+    return ml.y == 0.0f ? 0.0f : ml.y == ml.y ? factor(ml.x - m) : ml.y;
 }
 
 // A state's O' to a row of D floats; over int8 caches operand j's dims are code_dim's.
@@ -830,9 +868,12 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
     store_row<D, Q8>(area.acc[wave][lane & 15], st, gq);
     if (gq == 0) area.ml[wave][lane & 15] = make_float2(st.m, st.l);
     __syncthreads();
-    constexpr int kPer = kRows * D / (kFewWaves * 64);  // values a thread: 8 (D 128) or 4
+    constexpr int kPer = kRows * D / (kFewWaves * 64);  // values a thread, 16 threads a row: 8 (D 128) or 4
     const int r = tid * kPer / D, d = tid * kPer % D;
-    if (row0 + r >= map.total) return;
+    if (row0 + 4 * wave >= map.total) return;
+    const bool mine = row0 + r < map.total;
+    const bool any = mine && sight(K, p0 + (row0 + r) / map.g, rows, g.window).any;
+    const long long at = mine ? map.at(row0 + r) : 0;
     float m = -INFINITY, l = 0.0f, w[kFewWaves];
 #pragma unroll
     for (int i = 0; i < kFewWaves; ++i) m = fmaxf(m, area.ml[i][r].x);
@@ -850,12 +891,30 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
 #pragma unroll
             for (int e = 0; e < kPer; ++e) o[e] = fmaf(area.acc[i][r][d + e], w[i], o[e]);
         }
-    const long long at = map.at(row0 + r);
+    if constexpr (!Q8) {
+        float none = l * 0.0f;  // 0, or NaN
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) none = fmaf(o[e], 0.0f, none);
+        uint64_t odd = __builtin_amdgcn_ballot_w64(none != 0.0f && any);
+        if (__builtin_expect(odd != 0ull, 0)) {
+            const bool again = ((odd >> (lane & 48)) & 0xFFFFull) != 0ull;
+            for (int i = 0; i < 4; ++i) {
+                if (((odd >> (16 * i)) & 0xFFFFull) == 0ull) continue;
+                const int n1 = row0 + 4 * wave + i;
+                const long long at1 = map.at(n1);
+                strict_row<D>(K, g.q + at1 * D, g.scale, sight(K, p0 + n1 / map.g, rows, g.window), split * per,
+                              min(steps, (split + 1) * per), 1, lane,
+                              g.slots == 1 ? g.out + at1 * D : g.part + (at1 * g.slots + slot) * D,
+                              g.slots == 1 ? nullptr : g.ml + at1 * g.slots + slot);
+            }
+            if (again) return;
+        }
+    }
+    if (!mine) return;
     float* dst;
     if (g.slots == 1) {
-        const bool any = sight(K, p0 + (row0 + r) / map.g, rows, g.window).any && l != 0.0f;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) o[e] = any ? o[e] / l : 0.0f;
+        for (int e = 0; e < kPer; ++e) o[e] = any && l != 0.0f ? o[e] / l : 0.0f;
         dst = g.out + at * D + d;
     } else {
         if (d == 0) g.ml[at * g.slots + slot] = make_float2(m, l);
@@ -934,8 +993,6 @@ struct Stage {
     half8 k[D / 8][kKeys + 1];     // [8 dims][key]: the odd stride spreads a key's dims over the banks
     half8 v[D / 32][2][2][32];     // [dim tile][step][h][m]
     float ks[Q8 ? D / 64 : 1][Q8 ? kKeys : 4], vs[Q8 ? D / 64 : 1][Q8 ? kKeys : 4];
-    uint32_t odd[2];                             // fp16: the wave brought infinities or NaN, as bits j
-    uint8_t bad[Q8 ? 1 : kKeys][Q8 ? 4 : D / 4];  // of byte r of a key: dims 4 r + j, zero in v
 };
 
 // A wave's share of a tile on its way, 8 or 16 dwords.
@@ -1015,23 +1072,6 @@ struct Bring {
         if (wave < 2) {
             if (wave < D / 64) {
                 const int q = lane >> 4;
-                if constexpr (!Q8) {
-                    uint32_t any = 0u;  // an exponent of all ones
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) any |= (w[i] & 0x7C007C00u) + 0x04000400u;
-                    const bool odd = __builtin_amdgcn_ballot_w64((any & 0x80008000u) != 0u) != 0ull;
-                    if (lane == 0) s.odd[wave] = odd ? 1u : 0u;
-                    if (odd) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t m0 = odd_mask(w[2 * i]), m1 = odd_mask(w[2 * i + 1]);
-                            s.bad[v_key(i, q)][16 * wave + (lane & 15)] =
-                                static_cast<uint8_t>((m0 & 1u) | (m0 >> 16 & 2u) | (m1 & 4u) | (m1 >> 16 & 8u));
-                            w[2 * i] &= ~m0;
-                            w[2 * i + 1] &= ~m1;
-                        }
-                    }
-                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     uint32_t o[4];
@@ -1087,10 +1127,6 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     for (int u = 0; u < D / 32; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
-    // Values that are infinite or NaN are zero in the products (times the zero
-    // weight of a row that does not see them they would be NaN); the dims
-    // where the row sees one are kept here and become NaN at the end.
-    uint32_t bad[Q8 ? 1 : D / 16] = {};
     Bring<D, Q8> next;
     if (t0 < t1) {
         next.load(K, t0, wave, lane);
@@ -1151,7 +1187,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                 sc.rebase(first, rose, st.m != -INFINITY);
                 ev_low = Scaled::kLook;
             } else {
-                const float alpha = exp2_fast(-rose);
+                const float alpha = factor(-rose);
 #pragma unroll
                 for (int u = 0; u < D / 32; ++u) acc[u] *= alpha;
             }
@@ -1202,26 +1238,30 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
 #pragma unroll
             for (int u = 0; u < D / 32; ++u) acc[u] = mfma(v[u], w.rest(u >> 1), acc[u]);
         }
-        if constexpr (!Q8) {
-            if (uniform(static_cast<int>(s.odd[0] | s.odd[D / 64 - 1])) != 0) {
-#pragma unroll
-                for (int b = 0; b < D / 64; ++b)
-                    if (s.odd[b] != 0u) {
-#pragma unroll 1
-                        for (int i = 0; i < 16; ++i)
-#pragma unroll
-                            for (int e = 4 * b; e < 4 * b + 4; ++e)
-                                bad[e] |= (seen >> i) & 1u
-                                              ? *reinterpret_cast<const uint32_t*>(&s.bad[wide_key(i, h)][4 * e]) : 0u;
-                    }
-            }
-        }
         if (t + 2 < t1) next.store(stage[(at + 2) % kStages], wave, lane);
     }
     const float l = lanes_sum<32>(st.l);
     if constexpr (!Q8) {
+        float none[4] = {l * 0.0f, 0.0f, 0.0f, 0.0f};  // 0, or NaN
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) bad[e] |= __shfl_xor(bad[e], 32, kWave);
+        for (int u = 0; u < D / 32; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) none[i & 3] = fmaf(acc[u][i], 0.0f, none[i & 3]);
+        const bool odd = (none[0] + none[1]) + (none[2] + none[3]) != 0.0f;
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(odd && n < map.total && see.any);
+        uint32_t again = static_cast<uint32_t>(lanes) | static_cast<uint32_t>(lanes >> 32);
+        if (__builtin_expect(again != 0u, 0)) {
+            const bool mine = ((again >> (lane & 31)) & 1u) == 0u;
+            for (; again != 0u; again &= again - 1u) {
+                const int m = row0 + wave * kWideRows + __builtin_ctz(again);
+                const long long at = map.at(m);
+                const bool whole = g.slots == 1;
+                strict_row<D>(K, g.q + at * D, g.scale, sight(K, p0 + m / map.g, rows, g.window), t0, t1, 1, lane,
+                              whole ? g.out + at * D : g.part + (at * g.slots + slot) * D,
+                              whole ? nullptr : g.ml + at * g.slots + slot);
+            }
+            if (!mine) return;
+        }
     }
     if (n >= map.total) return;
     const long long at = map.at(n);
@@ -1235,10 +1275,6 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
             for (int u = 0; u < D / 32; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
-            if constexpr (!Q8) {  // a row that sees nothing meets the tile's keys where all others see them
-#pragma unroll
-                for (int e = 0; e < D / 16; ++e) bad[e] = 0u;
-            }
         }
         dst = g.out + at * D;
     } else {
@@ -1250,12 +1286,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     for (int u = 0; u < D / 32; u += 2)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float4 o = make_float4(acc[u][i] * f, acc[u][i + 8] * f, acc[u + 1][i] * f, acc[u + 1][i + 8] * f);
-            if constexpr (!Q8) {
-                const uint32_t no = (h ? bad[2 * u + 2 * (i >> 2) + 1] : bad[2 * u + 2 * (i >> 2)]) >> (8 * (i & 3));
-                const float nan = __builtin_nanf("");
-                o = make_float4(no & 1u ? nan : o.x, no & 2u ? nan : o.y, no & 4u ? nan : o.z, no & 8u ? nan : o.w);
-            }
+            const float4 o = make_float4(acc[u][i] * f, acc[u][i + 8] * f, acc[u + 1][i] * f, acc[u + 1][i + 8] * f);
             *reinterpret_cast<float4*>(dst + 32 * u + 4 * wide_key(i, h)) = o;
         }
 }

@@ -673,7 +673,11 @@ asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, int8_t* v_cac
  * out = softmax(q.K / sqrt(head_dim)) V over them.  A token whose position is
  * outside [0, rows) sees nothing: its out is zero (a padded sequence has pos
  * -n_tokens or less).  Rows that no token sees are not looked at, whatever
- * they hold; a row that is not finite reaches only the tokens that see it. */
+ * they hold.  An fp16 row with infinities or NaN reaches only the tokens that see
+ * it, as the definition has it: a score of +inf or NaN makes their outputs NaN, a
+ * key of score -inf has no weight (out is zero where all have none), and an
+ * infinite value is its dim's output at any weight (NaN at none).  Such tokens are
+ * taken again one by one, at up to sixty times the cost. */
 size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
                                          int window, int sinks);
 asdsl_status asdsl_attention_window_f16kv(const float* q, const uint16_t* k_cache, const uint16_t* v_cache,
