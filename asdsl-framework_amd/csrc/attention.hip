@@ -37,10 +37,12 @@ struct Cache {
 // amax * (1/127) (1e-12 when amax <= 1e-12) and code = round-half-even(x * (1 /
 // scale)) clamped to [-127, 127].
 //
-// Bound by HBM: 2045 tokens of 24 + 2 * 8 heads of 128 dims move 76 MB in 14.3 us
-// (5.3 TB/s; a copy of 1 GiB gets 5.15), a head per workgroup of scalar lanes took
-// 47.  16 tokens take 2.9 us, of which the launch and one chain of loads
-// (position, then tables) are nearly all.
+// Bound by memory: 2045 tokens of 24 + 2 * 8 heads of 128 dims move 76 MB in 18.1 us
+// where nothing of a call is in the caches (24 calls' buffers in turn; 4.2 TB/s, a
+// copy of 1 GiB gets 5.15) and in 14.8 where the last call's are; into int8 caches
+// 18.8 and 15.1.  A head per workgroup of scalar lanes took 47.  16 tokens take 3.0
+// us (int8 3.1), of which the launch and one chain of loads (position, then
+// tables) are nearly all.
 struct AppendArgs {
     const float* qkv;
     void* k;
@@ -147,7 +149,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
 //              read for the same 8 keys: every lane loads its D / 16 dims of those
 //              keys and turns the block in registers; no transposition in memory.
 // This form for few rows streams: 32 sequences of one token (24 heads of 128, 8 KV
-// heads, int8 caches, about 3300 rows each seen, 232 MB) take 52.4 us and 4.7 of
+// heads, int8 caches, about 3300 rows each seen, 232 MB) take 52.6 us and 4.8 of
 // join, 4.4 TB/s, bound by HBM and by the bytes its waves keep on the way.  For
 // small calls a workgroup's chain of position, first keys and join in LDS counts:
 // 6.3 us at 128 keys, where a compute unit then draws 32 bytes a ns.  Keys of many
@@ -969,13 +971,13 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
 // apart and one barrier does for two tiles.
 //
 // 4096 tokens with a window of 2048 over up to 6000 rows (24 heads of 128, 8 KV
-// heads, fp16): 225 us, 455 TFLOP/s of the definition's products and twice that
-// in the matrix cores, which are busy 43 % of the time; two products in fp16
-// parts at the rate of a large library product would take 189.  Neither the
-// loads nor the softmax alone bounds it: left out, each takes some 25 us off.  A
-// tile of 32 keys takes 1.24 us with one workgroup on a compute unit and 2.0 with
-// two.  Two buffers and a barrier a tile took 260 us, the form for few rows 462.
-// Over int8 caches 4096 tokens take 254 us with all of 4096 rows to see.
+// heads, fp16): 215 us, 480 TFLOP/s of the definition's products and twice that
+// in the matrix cores, which are busy 48 % of the time; two products in fp16
+// parts at the rate of a large library product would take 189.  Of 227 us in one
+// run, without the tiles' loads 198 were left, without their stores to LDS 211,
+// without the softmax 213, without all three 174: none alone bounds it.  Two
+// buffers and a barrier a tile took 260 us, the form for few rows 816.  Over int8
+// caches 4096 tokens take 253 us with all of 4096 rows to see.
 //
 // A lane holds one row n = lane % 32 and, with h = lane / 32, the keys
 // wide_key(i, h) of a tile's score registers i = 0..15; operand step s of the
@@ -1504,14 +1506,16 @@ int splits_for(long long fill, long long jobs, long long n, int most) {
 // of those.  Int8 keys are half the bytes, and their conversion, which the many-rows
 // form saves, is cheap beside 64 dims' softmax.  us few / many in a graph, 8 KV
 // heads, rows x keys (s: for each of s sequences, p: of a causal prompt):
-//   128 dims fp16  36 x 5000 21.2 / 20.0, 48 x 2000 15.5 / 15.9, 144 x 16000 102 / 52,
-//                  p 768 x 256 11.7 / 19.5, p 6144 x 2048 232 / 91
-//   128 dims int8  96 x 5000 24.9 / 29.4, 192 x 5000 40.8 / 35.2, 144 x 16000 77 / 64,
-//                  p 1551 x 517 24.2 / 33.0, p 6144 x 2048 158 / 112
-//   64 dims fp16   64 x 16000 23.8 / 29.3, 108 x 16000 37.1 / 32.5, 64 s 32 x 1000
-//                  32.4 / 58.5, p 2068 x 517 16.7 / 24.0, p 16384 x 4096 438 / 197
-//   64 dims int8   256 x 16000 44.6 / 52.1, 8 s 160 x 8000 107 / 145, 64 s 32 x 1000
-//                  25.3 / 75.4, p 8192 x 2048 85 / 110, p 16384 x 4096 293 / 251
+//   128 dims fp16  36 x 5000 19.9 / 19.1, 48 x 2000 15.0 / 14.9, 144 x 16000 102 / 49,
+//                  p 768 x 256 11.6 / 18.7, p 6144 x 2048 232 / 86
+//   128 dims int8  96 x 5000 23.7 / 29.5, 192 x 5000 41.6 / 35.3, 144 x 16000 76 / 63,
+//                  p 1551 x 517 23.9 / 31.7, p 6144 x 2048 158 / 114
+//   64 dims fp16   64 x 16000 22.4 / 27.7, 108 x 16000 36.6 / 30.6, 64 s 32 x 1000
+//                  32.1 / 54.6, p 2068 x 517 16.1 / 22.8, p 16384 x 4096 436 / 184
+//   64 dims int8   256 x 16000 43.8 / 46.5, 8 s 160 x 8000 104 / 138, 64 s 32 x 1000
+//                  25.6 / 72.9, p 8192 x 2048 82 / 107, p 16384 x 4096 269 / 235
+// One rule by steps does not fit all: 4 s 4096 rows of 64 dims over int8 caches with
+// a window of 256 take 74 in the form for few, 54 in the other.
 bool takes_many(long long total, long long heads, long long keys, int head_dim, bool q8) {
     if (total <= kRows) return false;
     const int wide = kManyWaves * kWideRows;
@@ -1525,11 +1529,11 @@ bool takes_many(long long total, long long heads, long long keys, int head_dim, 
 // Workgroups a launch is split up to: two a compute unit.  The many-rows form's
 // partials are 16 times as large a job, so with 128 dims it is split to one a
 // compute unit where those of two would come to a quarter of the keys' bytes (2068
-// rows over 1000 keys, 4 KV heads: 31 us, 41 with two; 16 sequences of 18 rows over
-// 2000 keys, 8 KV heads: 48 us, 36 with two).  With 64 dims a tile is shorter and
-// more of its waves fit: two pay (4096 rows over 4096 keys, 8 KV heads: 160 us, 110
+// rows over 1000 keys, 4 KV heads: 29 us, 38 with two; 16 sequences of 36 rows over
+// 2000 keys, 8 KV heads: 46 us, 41 with two).  With 64 dims a tile is shorter and
+// more of its waves fit: two pay (4096 rows over 4096 keys, 8 KV heads: 141 us, 101
 // with two) but where they alone would ask for a join of short pieces (16
-// sequences of 256 rows over 500 keys: 31 us, 37 with two).
+// sequences of 256 rows over 500 keys: 27 us, 35 with two).
 constexpr long long kFillFew = 512;
 
 long long fill_many(long long jobs, long long rows, long long heads, long long n, int head_dim) {
@@ -1542,9 +1546,9 @@ long long fill_many(long long jobs, long long rows, long long heads, long long n
 // Values of a KV head's keys that few rows take in one piece: a second launch
 // for the join costs more than the pieces save.  us a call in a graph (queued
 // one by one), whole / in pieces of 128 keys, 8 KV heads of 128 dims: 200 keys
-// 8.1 (9.5) / 9.0 (13.4), 256 8.3 (9.6) / 9.0 (13.6), 400 11.7 (11.7) / 9.1
-// (13.4); a compute unit alone draws some 32 bytes a ns.  64 dims: 512 keys 7.1
-// (9.4) / 7.0 (13.4), 1024 10.2 / 7.3.
+// 7.9 (9.5) / 9.2 (13.6), 256 8.5 (9.5) / 9.3 (13.1), 400 11.6 (11.6) / 9.3
+// (13.1); a compute unit alone draws some 32 bytes a ns.  64 dims: 512 keys 7.1
+// (9.5) / 7.1 (13.1), 1024 10.2 / 7.3.
 constexpr long long kAlone = 256 * 128;
 
 // How a call is laid out; the same for the work buffer's size and the launch.

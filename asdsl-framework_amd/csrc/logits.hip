@@ -36,12 +36,14 @@ struct ControlArgs {
 // whole history (integer atomics: any order gives the same).  kVec: the rows of
 // logits, out and bias lie in whole 16-byte units.
 //
-// Bound by HBM for many rows: 64 of 200064 (history 500, masks) read and write 104
-// MB in 22.2 us and 3.5 more for the tokens in a graph, 4.7 TB/s (a copy of 1 GiB
-// gets 5.15); one pass per step of the definition took 59.  Cold and alone the
-// kernel takes 27-29.  Stores past the caches save 1.3 us here and cost as much in
-// the kernel that reads the result.  One row: 4.4 us and 2.0, launches and
-// the chain of history length, ids and counts.
+// 64 rows of 200064 read and write 104 MB (20.2 us at a copy's 5.15 TB/s).  With
+// histories of 4000, masks and one bias they take 37.8 us where nothing of a call is
+// in the caches (16 calls' buffers in turn) and 33.1 where the last call's are, some
+// 4 of them the tokens' launch; with histories of 500 33.5 and 28.5: beside memory
+// each of a row's 49 workgroups counts the row's ids.  One pass per step of the
+// definition took 59.  Stores past the caches save 1.3 us here and cost as much in
+// the kernel that reads the result.  One row: 4.6 us and 2.2, launches and the chain
+// of history length, ids and counts.
 template <int kPer, bool kVec>
 __global__ __launch_bounds__(kThreads) void logits_control_kernel(const ControlArgs a) {
 #pragma clang fp contract(off)  // each step of the definition rounds by itself
