@@ -133,3 +133,32 @@ def test_an_infinite_value_of_next_to_no_weight(gpu, tokens, rows):
         got = attention_window(dev(q), dev(k), dev(v), dev(np.array([p0], np.int32))).cpu().numpy()
         assert (got[..., 5] == INF).all() and (got[..., 6] == -INF).all()
         assert np.isfinite(np.delete(got, (5, 6), axis=-1)).all()
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8"])
+@pytest.mark.parametrize("tokens,h,kvh,d,rows", [(1, 12, 4, 128, 300), (5, 12, 4, 64, 2000), (90, 12, 4, 128, 16400)])
+def test_queries_that_are_not_finite(gpu, kv, tokens, h, kvh, d, rows):
+    """Their own rows alone are NaN, whatever shares a tile with them."""
+    import torch
+
+    from asdsl.kernels import attention_window
+    from test_gpu_attention_ops import make_cache
+
+    rng = np.random.default_rng(tokens)
+    p0 = 200
+    q = rng.standard_normal((1, tokens, h, d)).astype(np.float32)
+    k, ks, kw = make_cache(rng, kv, 1, kvh, rows, d)
+    v, vs, vw = make_cache(rng, kv, 1, kvh, rows, d)
+    spoilt = [(tokens - 1, 2, NAN), (0, 7, INF), (tokens // 2, 11, -INF)]
+    for t, a, x in spoilt:
+        q[0, t, a, 5] = x
+    got = attention_window(dev(q), k, v, dev(np.array([p0], np.int32)), k_scale=ks, v_scale=vs).cpu().numpy()
+    for t in sorted({0, 1, tokens // 2, tokens - 1} & set(range(tokens))):
+        for a in range(h):
+            if any((t, a) == x[:2] for x in spoilt):
+                assert np.isnan(got[0, t, a]).all(), (t, a)
+                continue
+            m = p0 + t + 1
+            want, bound = ref.attend_row(q[0, t, a].astype(np.float64), kw[0, a // 3, :m], vw[0, a // 3, :m])
+            assert (np.abs(got[0, t, a] - want) <= bound).all(), (t, a)
+    assert int(torch.from_numpy(np.isnan(got).any(axis=-1)).sum()) == len(spoilt)
