@@ -105,12 +105,17 @@ SIGNATURES: dict[str, list] = {
     "asdsl_decode_prefill": [_P, _P, _I, _I, _P, _P, _P, _P, _P],
     "asdsl_kv_append_f16": [_P] * 7 + [_I] * 9 + [_P],
     "asdsl_kv_append_q8": [_P] * 9 + [_I] * 9 + [_P],
+    "asdsl_kv_append_q4": [_P] * 9 + [_I] * 9 + [_P],
+    "asdsl_kv_read_q8": [_P] * 7 + [_I] * 6 + [_P],
+    "asdsl_kv_read_q4": [_P] * 7 + [_I] * 6 + [_P],
     "asdsl_attention_window_work_bytes": [_I] * 8,
     "asdsl_attention_window_f16kv": [_P] * 5 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_window_q8kv": [_P] * 7 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_window_q4kv": [_P] * 7 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_prefix_work_bytes": [_I] * 6,
     "asdsl_attention_prefix_f16kv": [_P] * 7 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_prefix_q8kv": [_P] * 11 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_prefix_q4kv": [_P] * 11 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
     "asdsl_logits_control_work_bytes": [_I, _I],
     "asdsl_logits_control": [_P] * 6 + [_I] + [_P] * 4 + [ctypes.c_longlong, _P, ctypes.c_longlong, _I, _I, _P,
                                                          ctypes.c_size_t, _P],

@@ -7,12 +7,12 @@ reference's names and arguments, and the pybind-module stand-ins
 function names.  Every call runs on the GPU through libasdsl_hip.so.  The
 2- and 3-bit kernels and the CPU table-lookup (LUT) kernels of the reference
 are not part of this package.  Beside them, with no counterpart there, are the
-operators of many sequences and long contexts: ``kv_append``,
+operators of many sequences and long contexts: ``kv_append``, ``kv_read``,
 ``attention_window``, ``attention_prefix`` and ``control_logits``.
 """
 
 from asdsl.kernels import _native_gemv  # noqa: F401
-from asdsl.kernels.attention import attention_prefix, attention_window, kv_append
+from asdsl.kernels.attention import attention_prefix, attention_window, kv_append, kv_read
 from asdsl.kernels.gemv_q4 import gemv_q4, gemv_q4_packed, gemv_q4_unpacked, gemv_q4km_q8, has_native_kernel
 from asdsl.kernels.gemv_q8 import gemv_q8_unpacked
 from asdsl.kernels.gemv_q8 import has_native_kernel as has_native_q8_kernel
@@ -42,5 +42,6 @@ __all__ = [
     "attention_prefix",
     "attention_window",
     "kv_append",
+    "kv_read",
     "control_logits",
 ]

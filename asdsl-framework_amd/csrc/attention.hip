@@ -4,8 +4,8 @@
 // stay visible, and attention of sequences that share a prefix.
 //
 // Caches are [sequence][kv head][row][head_dim], fp16, or int8 codes with one
-// fp32 scale per 64 dims (the decode step's two forms); queries and outputs
-// are fp32.
+// fp32 scale per 64 dims (the decode step's two forms), or 4-bit codes with a
+// 16-bit word per 32 dims (kv_int4.hpp); queries and outputs are fp32.
 #include <hip/hip_fp16.h>
 
 #include <climits>
@@ -13,6 +13,7 @@
 
 #include "abi_util.hpp"
 #include "device_common.hpp"
+#include "kv_int4.hpp"
 
 namespace asdsl {
 namespace {
@@ -21,12 +22,17 @@ constexpr int kBlockDims = 64;  // dims per scale of an int8 cache
 constexpr float kInv127 = 1.0f / 127.0f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// One cache: K and V rows, and the scales of the int8 form.
+// What a cache holds.
+enum Kv : int { kF16, kI8, kI4 };
+constexpr int row_bytes(int form, int dims) { return form == kF16 ? 2 * dims : form == kI8 ? dims : dims / 2; }
+
+// One cache: K and V rows, and the fp32 scales of the int8 form or the scale
+// words of the 4-bit one.
 struct Cache {
     const void* k;
     const void* v;
-    const float* ks;
-    const float* vs;
+    const void* ks;
+    const void* vs;
 };
 
 // ------------------------------------------------------------------ append
@@ -47,8 +53,8 @@ struct AppendArgs {
     const float* qkv;
     void* k;
     void* v;
-    float* ks;
-    float* vs;
+    void* ks;
+    void* vs;
     const float* cos;
     const float* sin;
     const int* pos;
@@ -60,8 +66,14 @@ constexpr int kAppendThreads = 256;
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
+// A rotated value in 64 bits: the products are exact and their sum rounds once.
+__device__ __forceinline__ double turned(float own, float other, float c, float s, bool first) {
+    const double a = static_cast<double>(own) * c, b = static_cast<double>(other) * s;
+    return first ? a - b : a + b;
+}
+
 // kVec: rotary pairs and table rows lie in whole 16-byte units.
-template <int D, bool Q8, bool kVec>
+template <int D, int F, bool kVec>
 __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendArgs a) {
     constexpr int kUnits = D / 4;  // per head
     const int heads = a.n_heads + 2 * a.n_kv;
@@ -77,6 +89,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
     const bool inside = r >= 0 && r < a.rows && p >= 0 && p < a.rope_rows;
     if (!inside && head >= a.n_heads) return;
     float x[4] = {own.x, own.y, own.z, own.w};
+    double wide[4] = {own.x, own.y, own.z, own.w};  // 4-bit caches: what is quantized
     const int half = a.rot_half;
     if (!inside) {
         x[0] = x[1] = x[2] = x[3] = 0.0f;
@@ -89,8 +102,10 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
             const float4 o = load4(src + (first ? d + half : j)), c4 = load4(cs + j), s4 = load4(sn + j);
             const float y[4] = {o.x, o.y, o.z, o.w}, c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (F == kI4) wide[i] = turned(x[i], y[i], c[i], s[i], first);
                 x[i] = first ? fmaf(x[i], c[i], -(y[i] * s[i])) : fmaf(y[i], s[i], x[i] * c[i]);
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -98,6 +113,7 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
                 const bool first = d + i < half;
                 const int j = first ? d + i : d + i - half;
                 const float lo = src[j], hi = src[j + half];
+                if constexpr (F == kI4) wide[i] = turned(first ? lo : hi, first ? hi : lo, cs[j], sn[j], first);
                 x[i] = first ? fmaf(lo, cs[j], -(hi * sn[j])) : fmaf(lo, sn[j], hi * cs[j]);
             }
         }
@@ -111,7 +127,13 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
     const int kvh = head - a.n_heads - (key ? 0 : a.n_kv);
     const size_t crow = (static_cast<size_t>(seq) * a.n_kv + kvh) * a.rows + static_cast<size_t>(r);
     void* base = key ? a.k : a.v;
-    if constexpr (Q8) {
+    if constexpr (F == kI4) {
+        uint32_t word;
+        const uint32_t codes = quantize4(wide, word);
+        static_cast<uint16_t*>(base)[(crow * D + d) / 4] = static_cast<uint16_t>(codes);
+        if (d % kGroup4 == 0)
+            static_cast<uint16_t*>(key ? a.ks : a.vs)[crow * (D / kGroup4) + d / kGroup4] = static_cast<uint16_t>(word);
+    } else if constexpr (F == kI8) {
         const float m = group_max<16>(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
         const float scale = m > 1e-12f ? m * kInv127 : 1e-12f;
         const float inv = 1.0f / scale;
@@ -120,7 +142,8 @@ __global__ __launch_bounds__(kAppendThreads) void kv_append_kernel(const AppendA
         for (int i = 0; i < 4; ++i)
             q[i] = static_cast<int>(fminf(fmaxf(__builtin_rintf(x[i] * inv), -127.0f), 127.0f));
         *reinterpret_cast<uint32_t*>(static_cast<int8_t*>(base) + crow * D + d) = pack4_i8(q[0], q[1], q[2], q[3]);
-        if (d % kBlockDims == 0) (key ? a.ks : a.vs)[crow * (D / kBlockDims) + d / kBlockDims] = scale;
+        if (d % kBlockDims == 0)
+            static_cast<float*>(key ? a.ks : a.vs)[crow * (D / kBlockDims) + d / kBlockDims] = scale;
     } else {
         uint32_t w[2];
 #pragma unroll
@@ -173,8 +196,8 @@ constexpr int kFewWaves = 4;
 struct Keys {
     const void* k;
     const void* v;
-    const float* ks;
-    const float* vs;
+    const void* ks;
+    const void* vs;
     int na, db, n;
     bool masked;
     int p_first;  // smallest position of the workgroup's tokens that is in the cache
@@ -277,9 +300,19 @@ __device__ __forceinline__ half8 codes_half8(uint2 c) {
     return as_half8(w);
 }
 
+// Eight 4-bit codes of one row as fp16 numbers, dims i and i + 4 in a pair.
+__device__ __forceinline__ half8 codes4_half8(uint32_t c, const Step4& step) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = step.values(c, i);
+    return as_half8(w);
+}
+
 // A query row's operands: dims kDims * s + 8 * part .. + 8 in step s, part =
-// lane / (512 / kDims): kDims 32 for 16x16 tiles, 16 for 32x32 tiles.
-template <int D, int kDims>
+// lane / (512 / kDims): kDims 32 for 16x16 tiles, 16 for 32x32 tiles.  Over 4-bit
+// caches (kFour) dims i and i + 4 of 8 are neighbours, as the codes come out of a
+// word, and with 16x16 tiles a lane's dims lie together, D / 4 * part + 8 * s.
+template <int D, int kDims, bool kFour>
 struct Query {
     half8 hi[D / kDims], lo[D / kDims];
     float c;  // score = product * c, in powers of two
@@ -290,10 +323,15 @@ struct Query {
 #pragma unroll
         for (int s = 0; s < D / kDims; ++s) {
             if (row) {
-                const float4 a = *reinterpret_cast<const float4*>(row + kDims * s + 8 * part);
-                const float4 b = *reinterpret_cast<const float4*>(row + kDims * s + 8 * part + 4);
-                x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
-                x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+                const float* src = row + (kFour && kDims == 32 ? D / 4 * part + 8 * s : kDims * s + 8 * part);
+                const float4 a = load4(src), b = load4(src + 4);
+                if constexpr (kFour) {
+                    x[s][0] = a.x; x[s][2] = a.y; x[s][4] = a.z; x[s][6] = a.w;
+                    x[s][1] = b.x; x[s][3] = b.y; x[s][5] = b.z; x[s][7] = b.w;
+                } else {
+                    x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w;
+                    x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[s][i] = 0.0f;
@@ -323,10 +361,10 @@ template <int D>
 __device__ __forceinline__ int fp16_dim(int r, int j) { return D / 16 * r + j; }
 __device__ __forceinline__ int code_dim(int r, int j) { return 64 * (j >> 2) + 4 * r + (j & 3); }
 
-template <int D, bool Q8>
+template <int D, int F>
 struct VRaw;
 template <int D>
-struct VRaw<D, false> {
+struct VRaw<D, kF16> {
     uint32_t w[8][D / 32];
     __device__ __forceinline__ void load(const char* row, int key, int r) {
         const char* src = row + D / 8 * r;
@@ -346,8 +384,29 @@ struct VRaw<D, false> {
         return as_half8(o);
     }
 };
+// 4-bit: dims D / 16 * r .. of a key, 32 or 16 bits, and the word of their scale.
+// The codes of two keys in one register come out as operands.
 template <int D>
-struct VRaw<D, true> {
+struct VRaw<D, kI4> {
+    uint32_t w[8], words[8];
+    __device__ __forceinline__ void load(const char* row, int key, int r) {
+        if constexpr (D == 128)
+            w[key] = *reinterpret_cast<const uint32_t*>(row + 4 * r);
+        else
+            w[key] = *reinterpret_cast<const uint16_t*>(row + 2 * r);
+    }
+    __device__ __forceinline__ half8 operand(int j) const {
+        uint32_t o[4];
+        const uint32_t sel = (j & 4) ? 0x07060302u : 0x05040100u;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+            o[p] = Step4(__builtin_amdgcn_perm(words[2 * p + 1], words[2 * p], 0x05040100u))
+                       .values(__builtin_amdgcn_perm(w[2 * p + 1], w[2 * p], sel), j & 3);
+        return as_half8(o);
+    }
+};
+template <int D>
+struct VRaw<D, kI8> {
     uint32_t w[8][D / 64];
     __device__ __forceinline__ void load(const char* row, int key, int r) {
         const char* src = row + 4 * r;
@@ -586,20 +645,38 @@ __device__ __forceinline__ uint32_t mask_keys(const Keys& K, const RowSight& see
 // Steps t0, t0 + stride, ... below t1 of 32 keys each, K and V straight from
 // the cache into the operands' registers: 16 lanes read a V row's 256 bytes, 4
 // lanes 64 bytes of a K row.  A step's loads are issued one phase ahead.
-template <int D, bool Q8>
+template <int D, int F>
 struct Step {
+    static constexpr bool Q8 = F == kI8;
     uint4 k16[2][D / 32];
     uint2 k8[2][D / 32];
-    VRaw<D, Q8> v;
+    uint32_t k4[2][D / 32], kw[2];
+    VRaw<D, F> v;
     float ks[8][D / 64], vs[8][D / 64];
 
     // Key i's row is at(i) rows past `first`; kFollow: at(i) = i, so that the
     // addresses are one scalar and constants, and a lane's scales lie together.
-    template <bool kFollow, typename F>
-    __device__ __forceinline__ void k_rows(const Keys& K, size_t first, F at, int lane) {
+    template <bool kFollow, typename At>
+    __device__ __forceinline__ void k_rows(const Keys& K, size_t first, At at, int lane) {
         constexpr int kBytes = Q8 ? 1 : 2;
         const int r = lane & 15, gq = lane >> 4;
-        const char* src = static_cast<const char*>(K.k) + first * (D * kBytes);
+        const char* src = static_cast<const char*>(K.k) + first * row_bytes(F, D);
+        if constexpr (F == kI4) {
+            const uint16_t* words = static_cast<const uint16_t*>(K.ks) + first * (D / kGroup4);
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+                const char* x = src + (at(16 * kt + r) * (D / 2) + D / 8 * gq);
+                if constexpr (D == 128) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(x);
+                    k4[kt][0] = c.x; k4[kt][1] = c.y; k4[kt][2] = c.z; k4[kt][3] = c.w;
+                } else {
+                    const uint2 c = *reinterpret_cast<const uint2*>(x);
+                    k4[kt][0] = c.x; k4[kt][1] = c.y;
+                }
+                kw[kt] = words[at(16 * kt + r) * (D / kGroup4) + D / 4 * gq / kGroup4];
+            }
+            return;
+        }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             const char* x = src + (at(16 * kt + r) * (D * kBytes) + 8 * gq * kBytes);
@@ -611,20 +688,24 @@ struct Step {
                     k16[kt][s] = *reinterpret_cast<const uint4*>(x + 64 * s);
             }
         }
-        if constexpr (Q8) scale_rows<kFollow>(K.ks, first, at, gq, ks);
+        if constexpr (Q8) scale_rows<kFollow>(static_cast<const float*>(K.ks), first, at, gq, ks);
     }
-    template <bool kFollow, typename F>
-    __device__ __forceinline__ void v_rows(const Keys& K, size_t first, F at, int lane) {
-        constexpr int kBytes = Q8 ? 1 : 2;
+    template <bool kFollow, typename At>
+    __device__ __forceinline__ void v_rows(const Keys& K, size_t first, At at, int lane) {
         const int r = lane & 15, gq = lane >> 4;
-        const char* src = static_cast<const char*>(K.v) + first * (D * kBytes);
+        const char* src = static_cast<const char*>(K.v) + first * row_bytes(F, D);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.load(src + at((i & 4) * 4 + 4 * gq + (i & 3)) * (D * kBytes), i, r);
-        if constexpr (Q8) scale_rows<kFollow>(K.vs, first, at, gq, vs);
+        for (int i = 0; i < 8; ++i) v.load(src + at((i & 4) * 4 + 4 * gq + (i & 3)) * row_bytes(F, D), i, r);
+        if constexpr (Q8) scale_rows<kFollow>(static_cast<const float*>(K.vs), first, at, gq, vs);
+        if constexpr (F == kI4) {
+            const uint16_t* words = static_cast<const uint16_t*>(K.vs) + first * (D / kGroup4) + D / 16 * r / kGroup4;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v.words[i] = words[at((i & 4) * 4 + 4 * gq + (i & 3)) * (D / kGroup4)];
+        }
     }
     // The scales of the lane's 8 keys.
-    template <bool kFollow, typename F>
-    __device__ __forceinline__ void scale_rows(const float* src, size_t first, F at, int gq, float (&dst)[8][D / 64]) {
+    template <bool kFollow, typename At>
+    __device__ __forceinline__ void scale_rows(const float* src, size_t first, At at, int gq, float (&dst)[8][D / 64]) {
         typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));  // a row's scales start anywhere
         src += first * (D / 64);
         if constexpr (kFollow) {
@@ -660,12 +741,14 @@ struct Step {
             v_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
     }
     __device__ __forceinline__ half8 k_operand(int kt, int s) const {
-        if constexpr (Q8)
+        if constexpr (F == kI4)
+            return codes4_half8(k4[kt][s], Step4(both4(kw[kt])));
+        else if constexpr (Q8)
             return codes_half8(k8[kt][s]);
         else
             return __builtin_bit_cast(half8, k16[kt][s]);
     }
-    __device__ __forceinline__ void scores(const Query<D, 32>& q, float (&s)[8]) const {
+    __device__ __forceinline__ void scores(const Query<D, 32, F == kI4>& q, float (&s)[8]) const {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             if constexpr (Q8) {
@@ -699,12 +782,13 @@ struct Step {
     }
 };
 
-template <int D, bool Q8>
-__device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, const RowSight& see, int t0, int t1,
-                                         int stride, int lane, State<D, Q8>& st) {
+template <int D, int F>
+__device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, F == kI4>& q, const RowSight& see, int t0,
+                                         int t1, int stride, int lane, State<D, F == kI8>& st) {
+    constexpr bool Q8 = F == kI8;
     if (t0 >= t1) return;
     const int gq = lane >> 4;
-    Step<D, Q8> x;
+    Step<D, F> x;
     x.load_k(K, t0, lane);
     x.load_v(K, t0, lane);
     for (int t = t0; t < t1; t += stride) {
@@ -738,7 +822,7 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32>& q, c
 // 2048 whose every value is NaN (99 us without), 0.77 for 32 tokens over 4000 rows
 // (0.099).  O' (or, without ml, the output of a row that the call has whole) to dst,
 // base and sum to ml.
-template <int D>
+template <int D, int F>
 __device__ __forceinline__ void strict_row(const Keys& K, const float* row, float scale, const RowSight& see, int t0, int t1,
                                            int stride, int lane, float* dst, float2* ml) {
     constexpr int kDims = D / kWave;  // of a lane
@@ -750,16 +834,28 @@ __device__ __forceinline__ void strict_row(const Keys& K, const float* row, floa
         const bool ok = step < t1 && key < K.n && r <= see.p && (r >= see.lo || r < K.sinks);
         float s = 0.0f;
         if (ok) {
-            const char* src = static_cast<const char*>(K.k) + static_cast<size_t>(r) * (2 * D);
+            const char* src = static_cast<const char*>(K.k) + static_cast<size_t>(r) * row_bytes(F, D);
+            if constexpr (F == kI4) {
+                const uint16_t* words = static_cast<const uint16_t*>(K.ks) + static_cast<size_t>(r) * (D / kGroup4);
 #pragma unroll 1
-            for (int d0 = 0; d0 < D; d0 += 64) {
-                half8 k[8];
+                for (int d0 = 0; d0 < D; d0 += kGroup4) {
+                    const uint4 c = *reinterpret_cast<const uint4*>(src + d0 / 2);
+                    const uint32_t w[4] = {c.x, c.y, c.z, c.w}, word = words[d0 / kGroup4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const half8*>(src + 2 * d0 + 16 * j);
+                    for (int i = 0; i < kGroup4; ++i)
+                        s = fmaf(value4((w[i / 8] >> (4 * (i % 8))) & 15u, word), row[d0 + i], s);
+                }
+            } else {
+#pragma unroll 1
+                for (int d0 = 0; d0 < D; d0 += 64) {
+                    half8 k[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 8; ++j) k[j] = *reinterpret_cast<const half8*>(src + 2 * d0 + 16 * j);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) s = fmaf(static_cast<float>(k[j][i]), row[d0 + 8 * j + i], s);
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) s = fmaf(static_cast<float>(k[j][i]), row[d0 + 8 * j + i], s);
+                }
             }
         }
         s = ok ? s * scale : -INFINITY;
@@ -779,10 +875,17 @@ __device__ __forceinline__ void strict_row(const Keys& K, const float* row, floa
             float v[16][kDims];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const _Float16* src = static_cast<const _Float16*>(K.v) +
-                                      static_cast<size_t>(__builtin_amdgcn_readlane(r, i0 + i)) * D + kDims * lane;
+                const size_t at = static_cast<size_t>(__builtin_amdgcn_readlane(r, i0 + i)) * D + kDims * lane;
+                if constexpr (F == kI4) {
+                    const uint32_t c = static_cast<const uint8_t*>(K.v)[at / 2];
+                    const uint32_t word = static_cast<const uint16_t*>(K.vs)[at / kGroup4];
 #pragma unroll
-                for (int e = 0; e < kDims; ++e) v[i][e] = static_cast<float>(src[e]);
+                    for (int e = 0; e < kDims; ++e) v[i][e] = value4((c >> (4 * ((at + e) & 1))) & 15u, word);
+                } else {
+                    const _Float16* src = static_cast<const _Float16*>(K.v) + at;
+#pragma unroll
+                    for (int e = 0; e < kDims; ++e) v[i][e] = static_cast<float>(src[e]);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -852,20 +955,21 @@ __device__ __forceinline__ RowSight sight(const Keys& K, long long p, int rows, 
     return s;
 }
 
-template <int D, bool Q8>
+template <int D, int F>
 __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const RowMap& map, int row0, long long p0,
                                         int rows, int split, int splits, int slot, JoinArea<D, kFewWaves>& area) {
+    constexpr bool Q8 = F == kI8;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
     const int n = row0 + (lane & 15), gq = lane >> 4;
     const bool real = n < map.total;
-    Query<D, 32> q;
+    Query<D, 32, F == kI4> q;
     q.load(real ? g.q + map.at(n) * D : nullptr, gq, g.scale);
     const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
     State<D, Q8> st;
     const int steps = (K.n + kKeys - 1) / kKeys;
     // a split's steps, a multiple of the waves'
     const int per = ((steps + splits - 1) / splits + kFewWaves - 1) / kFewWaves * kFewWaves;
-    few_rows<D, Q8>(K, q, see, split * per + wave, min(steps, (split + 1) * per), kFewWaves, lane, st);
+    few_rows<D, F>(K, q, see, split * per + wave, min(steps, (split + 1) * per), kFewWaves, lane, st);
     st.l = lanes_sum<16>(st.l);
     store_row<D, Q8>(area.acc[wave][lane & 15], st, gq);
     if (gq == 0) area.ml[wave][lane & 15] = make_float2(st.m, st.l);
@@ -904,7 +1008,7 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
                 if (((odd >> (16 * i)) & 0xFFFFull) == 0ull) continue;
                 const int n1 = row0 + 4 * wave + i;
                 const long long at1 = map.at(n1);
-                strict_row<D>(K, g.q + at1 * D, g.scale, sight(K, p0 + n1 / map.g, rows, g.window), split * per,
+                strict_row<D, F>(K, g.q + at1 * D, g.scale, sight(K, p0 + n1 / map.g, rows, g.window), split * per,
                               min(steps, (split + 1) * per), 1, lane,
                               g.slots == 1 ? g.out + at1 * D : g.part + (at1 * g.slots + slot) * D,
                               g.slots == 1 ? nullptr : g.ml + at1 * g.slots + slot);
@@ -927,24 +1031,25 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
     for (int e = 0; e < kPer; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
 }
 
-template <int D, bool Q8>
+template <int D, int F>
 __device__ __forceinline__ Keys head_keys(const Cache& c, long long head, int rows) {
     Keys K{};
     const size_t row = static_cast<size_t>(head) * rows;
-    const size_t bytes = row * D * (Q8 ? 1 : 2);
+    const size_t bytes = row * row_bytes(F, D);
     K.k = static_cast<const char*>(c.k) + bytes;
     K.v = static_cast<const char*>(c.v) + bytes;
-    if constexpr (Q8) {
-        K.ks = c.ks + row * (D / 64);
-        K.vs = c.vs + row * (D / 64);
+    if constexpr (F != kF16) {
+        const size_t scales = row * (F == kI8 ? D / kBlockDims * sizeof(float) : D / kGroup4 * sizeof(uint16_t));
+        K.ks = static_cast<const char*>(c.ks) + scales;
+        K.vs = static_cast<const char*>(c.vs) + scales;
     }
     return K;
 }
 
 // The keys that tokens [t0, t1) of a sequence see with a window.
-template <int D, bool Q8>
+template <int D, int F>
 __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh, int t0, int t1) {
-    Keys K = head_keys<D, Q8>(g.b, static_cast<long long>(seq) * g.n_kv + kvh, g.rows_b);
+    Keys K = head_keys<D, F>(g.b, static_cast<long long>(seq) * g.n_kv + kvh, g.rows_b);
     const long long p0 = g.pos[seq];
     const long long first = p0 + t0 > 0 ? p0 + t0 : 0;
     const long long last = p0 + t1 - 1 < g.rows_b ? p0 + t1 - 1 : g.rows_b - 1;
@@ -998,9 +1103,10 @@ struct Stage {
 };
 
 // A wave's share of a tile on its way, 8 or 16 dwords.
-template <int D, bool Q8>
+template <int D, int F>
 struct Bring {
-    static constexpr int kV = Q8 ? 1 : 2;   // dwords of 4 dims of V
+    static constexpr bool Q8 = F == kI8;
+    static constexpr int kV = Q8 ? 1 : 2;   // dwords of 4 dims of V (4-bit: codes and word)
     static constexpr int kK = Q8 ? 2 : 4;   // dwords of 8 dims of K
     static constexpr int kLoads = D / 32;   // 16 keys of K
     uint32_t w[8 * kV];
@@ -1013,9 +1119,66 @@ struct Bring {
     static __device__ __forceinline__ int k_key(int i, int wave, int lane) {
         return 16 * (wave - 2) + (16 / kLoads) * i + lane / (D / 8);
     }
+    // 4-bit codes: the key of which a lane brings dims D / 4 * (lane % 4) ..
+    static __device__ __forceinline__ int k4_key(int wave, int lane) { return 16 * (wave - 2) + (lane >> 2); }
+    template <typename At>
+    __device__ __forceinline__ void load4_rows(const Keys& K, size_t first, At at, int wave, int lane) {
+        if (wave < 2) {
+            if (wave < D / 64) {
+                const int d = 64 * wave + 4 * (lane & 15);
+                const char* src = static_cast<const char*>(K.v) + first * (D / 2) + d / 2;
+                const uint16_t* words = static_cast<const uint16_t*>(K.vs) + first * (D / kGroup4) + d / kGroup4;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const auto key = at(v_key(i, lane >> 4));
+                    w[i] = *reinterpret_cast<const uint16_t*>(src + key * (D / 2));
+                    w[8 + i] = words[key * (D / kGroup4)];
+                }
+            }
+        } else {
+            const auto key = at(k4_key(wave, lane));
+            const char* x = static_cast<const char*>(K.k) + first * (D / 2) + (key * (D / 2) + D / 8 * (lane & 3));
+            if constexpr (D == 128) {
+                const uint4 c = *reinterpret_cast<const uint4*>(x);
+                w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w;
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2*>(x);
+                w[0] = c.x; w[1] = c.y;
+            }
+            w[8] = static_cast<const uint16_t*>(K.ks)[first * (D / kGroup4) + key * (D / kGroup4) +
+                                                      D / 4 * (lane & 3) / kGroup4];
+        }
+    }
+    __device__ __forceinline__ void store4(Stage<D, false>& s, int wave, int lane) {
+        if (wave < 2) {
+            if (wave < D / 64) {
+                const int q = lane >> 4;
+                uint32_t o[4][4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const Step4 step(w[8 + 2 * p] | (w[9 + 2 * p] << 16));
+                    const uint32_t c = w[2 * p] | (w[2 * p + 1] << 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[j][p] = step.values(c, j);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    s.v[2 * wave + (j >> 1)][q >> 1][q & 1][16 * (j & 1) + (lane & 15)] = as_half8(o[j]);
+            }
+        } else {
+            const Step4 step(both4(w[8]));
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x)
+                s.k[D / 32 * (lane & 3) + x][k4_key(wave, lane)] = codes4_half8(w[x], step);
+        }
+    }
     // Key i's row is at(i) rows past `first`.
-    template <typename F>
-    __device__ __forceinline__ void load_rows(const Keys& K, size_t first, F at, int wave, int lane) {
+    template <typename At>
+    __device__ __forceinline__ void load_rows(const Keys& K, size_t first, At at, int wave, int lane) {
+        if constexpr (F == kI4) {
+            load4_rows(K, first, at, wave, lane);
+            return;
+        }
         constexpr int kBytes = Q8 ? 1 : 2;
         if (wave < 2) {
             if (wave < D / 64) {
@@ -1056,7 +1219,7 @@ struct Bring {
             const int e = wave * 64 + lane;
             if (e < 2 * kKeys * (D / 64)) {
                 const int i = e % (kKeys * (D / 64));
-                const float* src = (e < kKeys * (D / 64) ? K.ks : K.vs) + first * (D / 64);
+                const float* src = static_cast<const float*>(e < kKeys * (D / 64) ? K.ks : K.vs) + first * (D / 64);
                 scale = src[at(i / (D / 64)) * (D / 64) + i % (D / 64)];
             }
         }
@@ -1071,6 +1234,10 @@ struct Bring {
             load_rows(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, wave, lane);
     }
     __device__ __forceinline__ void store(Stage<D, Q8>& s, int wave, int lane) {
+        if constexpr (F == kI4) {
+            store4(s, wave, lane);
+            return;
+        }
         if (wave < 2) {
             if (wave < D / 64) {
                 const int q = lane >> 4;
@@ -1110,15 +1277,17 @@ struct Bring {
     }
 };
 
-template <int D, bool Q8>
+template <int D, int F>
 __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const RowMap& map, int row0, long long p0,
-                                         int rows, int split, int splits, int slot, Stage<D, Q8> (&stage)[kStages]) {
+                                         int rows, int split, int splits, int slot,
+                                         Stage<D, F == kI8> (&stage)[kStages]) {
+    constexpr bool Q8 = F == kI8;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = uniform(tid >> 6);
     const int n = row0 + wave * kWideRows + (lane & 31), h = lane >> 5;
     const int tiles = (K.n + kKeys - 1) / kKeys;
     const int per = (tiles + splits - 1) / splits;
     const int t0 = split * per, t1 = min(tiles, t0 + per);
-    Query<D, 16> q;
+    Query<D, 16, F == kI4> q;
     q.load(n < map.total ? g.q + map.at(n) * D : nullptr, h, g.scale);
     const RowSight see = sight(K, p0 + n / map.g, rows, g.window);
     Softmax<Q8, 32> st;
@@ -1129,7 +1298,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
     for (int u = 0; u < D / 32; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[u][i] = 0.0f;
-    Bring<D, Q8> next;
+    Bring<D, F> next;
     if (t0 < t1) {
         next.load(K, t0, wave, lane);
         next.store(stage[0], wave, lane);
@@ -1258,7 +1427,7 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
                 const int m = row0 + wave * kWideRows + __builtin_ctz(again);
                 const long long at = map.at(m);
                 const bool whole = g.slots == 1;
-                strict_row<D>(K, g.q + at * D, g.scale, sight(K, p0 + m / map.g, rows, g.window), t0, t1, 1, lane,
+                strict_row<D, F>(K, g.q + at * D, g.scale, sight(K, p0 + m / map.g, rows, g.window), t0, t1, 1, lane,
                               whole ? g.out + at * D : g.part + (at * g.slots + slot) * D,
                               whole ? nullptr : g.ml + at * g.slots + slot);
             }
@@ -1294,9 +1463,9 @@ __device__ __forceinline__ void many_job(const AttnArgs& g, const Keys& K, const
 }
 
 // Row tiles from the last one down: with no window its tokens see the most.
-template <int D, bool Q8>
+template <int D, int F>
 __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const AttnArgs g) {
-    __shared__ Stage<D, Q8> stage[kStages];
+    __shared__ Stage<D, F == kI8> stage[kStages];
     constexpr int kWgRows = kManyWaves * kWideRows;
     const int group = g.n_heads / g.n_kv;
     const int total = g.n_tokens * group;
@@ -1310,14 +1479,14 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const A
     const int seq = b / tiles;
     const RowMap map{static_cast<long long>(seq) * g.n_tokens * g.n_heads + static_cast<long long>(kvh) * group, group,
                      g.n_heads, total};
-    const Keys K = window_keys<D, Q8>(g, seq, kvh, row0 / group, (min(row0 + kWgRows, total) - 1) / group + 1);
-    many_job<D, Q8>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, stage);
+    const Keys K = window_keys<D, F>(g, seq, kvh, row0 / group, (min(row0 + kWgRows, total) - 1) / group + 1);
+    many_job<D, F>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, stage);
 }
 
 // ------------------------------------------------------- few rows: kernels
 // blockIdx.x = ((sequence * row tiles + tile) * splits + split) * n_kv + kv head:
 // with 8 KV heads one head's workgroups share an XCD's L2.
-template <int D, bool Q8>
+template <int D, int F>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void window_few_kernel(const AttnArgs g) {
     __shared__ JoinArea<D, kFewWaves> area;
     const int group = g.n_heads / g.n_kv;
@@ -1332,20 +1501,20 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void window_few_kernel(const Att
     const int seq = b / tiles;
     const RowMap map{static_cast<long long>(seq) * g.n_tokens * g.n_heads + static_cast<long long>(kvh) * group, group,
                      g.n_heads, total};
-    const Keys K = window_keys<D, Q8>(g, seq, kvh, row0 / group, (min(row0 + kRows, total) - 1) / group + 1);
-    few_job<D, Q8>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, area);
+    const Keys K = window_keys<D, F>(g, seq, kvh, row0 / group, (min(row0 + kRows, total) - 1) / group + 1);
+    few_job<D, F>(g, K, map, row0, g.pos[seq], g.rows_b, split, g.splits, split, area);
 }
 
 // Shared prefix: the first `jobs` workgroups take rows of a KV head, 16 or 128
 // of all sequences' (sequence, head) rows, and a split of the prefix, the others
 // a sequence's own keys.
-template <int D, bool Q8, bool kMany>
+template <int D, int F, bool kMany>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArgs g, int prefix_splits, int jobs) {
     static_assert(kFewWaves == kManyWaves, "one workgroup size");
     constexpr int kWgRows = kMany ? kManyWaves * kWideRows : kRows;
     __shared__ union Lds {
         JoinArea<D, kFewWaves> area;
-        Stage<D, Q8> stage[kMany ? kStages : 1];
+        Stage<D, F == kI8> stage[kMany ? kStages : 1];
         __device__ Lds() {}
     } lds;
     const int group = g.n_heads / g.n_kv;
@@ -1358,12 +1527,12 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArg
         const int row0 = b % tiles * kWgRows;
         const int split = b / tiles;
         const RowMap map{static_cast<long long>(kvh) * group, group, g.n_heads, total};
-        Keys K = head_keys<D, Q8>(g.a, kvh, g.rows_a);
+        Keys K = head_keys<D, F>(g.a, kvh, g.rows_a);
         K.n = g.prefix;
         if constexpr (kMany)
-            many_job<D, Q8>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.stage);
+            many_job<D, F>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.stage);
         else
-            few_job<D, Q8>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.area);
+            few_job<D, F>(g, K, map, row0, 0, 0, split, prefix_splits, split, lds.area);
         return;
     }
     b -= jobs;
@@ -1377,10 +1546,10 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void prefix_kernel(const AttnArg
     const int seq = b / tiles;
     const RowMap map{static_cast<long long>(seq) * g.n_heads + static_cast<long long>(kvh) * group, group, g.n_heads,
                      group};
-    Keys K = head_keys<D, Q8>(g.b, static_cast<long long>(seq) * g.n_kv + kvh, g.rows_b);
+    Keys K = head_keys<D, F>(g.b, static_cast<long long>(seq) * g.n_kv + kvh, g.rows_b);
     const int p = g.pos[seq];
     K.n = p >= 0 && p < g.rows_b ? p + 1 : 0;
-    few_job<D, Q8>(g, K, map, row0, 0, 0, split, own_splits, prefix_splits + split, lds.area);
+    few_job<D, F>(g, K, map, row0, 0, 0, split, own_splits, prefix_splits + split, lds.area);
 }
 
 // One wave per query row: its partials in slot order, so that the result does not
@@ -1433,18 +1602,30 @@ __global__ __launch_bounds__(kJoinRows * 64) void attention_join_kernel(const At
 }
 
 // ------------------------------------------------------------- host checks
-// f(head_dim, int8) as compile-time constants.
-template <typename F>
-asdsl_status with_form(int head_dim, bool q8, F f) {
+// f(head_dim, form) as compile-time constants.
+template <typename T>
+asdsl_status with_form(int head_dim, Kv form, T f) {
     using std::integral_constant;
-    if (head_dim == 128)
-        return q8 ? f(integral_constant<int, 128>{}, std::true_type{}) : f(integral_constant<int, 128>{}, std::false_type{});
-    return q8 ? f(integral_constant<int, 64>{}, std::true_type{}) : f(integral_constant<int, 64>{}, std::false_type{});
+    auto with = [&](auto dim) {
+        return form == kF16  ? f(dim, integral_constant<int, kF16>{})
+               : form == kI8 ? f(dim, integral_constant<int, kI8>{})
+                             : f(dim, integral_constant<int, kI4>{});
+    };
+    return head_dim == 128 ? with(integral_constant<int, 128>{}) : with(integral_constant<int, 64>{});
 }
 
 constexpr int kMaxRows = 1 << 30;  // rows seen, so that a tile past the last of them is an int
 
 inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline bool aligned4(const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
+
+// The scales that a cache's form asks for (rows of them start at any row).
+asdsl_status check_scales(const char* what, Kv form, const void* ks, const void* vs) {
+    if (form == kF16) return ASDSL_OK;
+    ASDSL_CHECK_ARG(ks && vs, "%s: null scale array", what);
+    ASDSL_CHECK_ARG(aligned4(ks) && aligned4(vs), "%s: scales must be 4-byte aligned", what);
+    return ASDSL_OK;
+}
 
 asdsl_status check_heads(const char* what, int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim) {
     ASDSL_CHECK_ARG(n_seq > 0 && n_tokens > 0, "%s: n_seq and n_tokens must be positive", what);
@@ -1458,13 +1639,14 @@ asdsl_status check_heads(const char* what, int n_seq, int n_tokens, int n_heads,
     return ASDSL_OK;
 }
 
-asdsl_status append(const char* what, bool q8, const float* qkv, void* k, void* v, float* ks, float* vs,
+asdsl_status append(const char* what, Kv form, const float* qkv, void* k, void* v, void* ks, void* vs,
                     const float* rope_cos, const float* rope_sin, const int* pos, float* q_out, int n_seq,
                     int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int rows, int pos_offset,
                     int rope_rows, asdsl_stream_t stream) {
     ASDSL_CHECK_ARG(qkv && k && v && rope_cos && rope_sin && pos && q_out, "%s: null pointer", what);
-    ASDSL_CHECK_ARG(!q8 || (ks && vs), "%s: null scale array", what);
-    const asdsl_status st = check_heads(what, n_seq, n_tokens, n_heads, n_kv_heads, head_dim);
+    asdsl_status st = check_scales(what, form, ks, vs);
+    if (st != ASDSL_OK) return st;
+    st = check_heads(what, n_seq, n_tokens, n_heads, n_kv_heads, head_dim);
     if (st != ASDSL_OK) return st;
     ASDSL_CHECK_ARG(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
                     "%s: rotary_dim must be even and <= head_dim", what);
@@ -1478,10 +1660,9 @@ asdsl_status append(const char* what, bool q8, const float* qkv, void* k, void* 
     const AppendArgs a{qkv, k, v, ks, vs, rope_cos, rope_sin, pos, q_out, n_tokens, n_heads, n_kv_heads,
                        rotary_dim / 2, rows, pos_offset, rope_rows, chunks};
     const bool vec = rotary_dim % 8 == 0 && aligned16(rope_cos) && aligned16(rope_sin);
-    return with_form(head_dim, q8, [&](auto dim, auto codes) {
-        constexpr int kD = decltype(dim)::value;
-        constexpr bool kQ8 = decltype(codes)::value;
-        return launch("kv_append_kernel", vec ? kv_append_kernel<kD, kQ8, true> : kv_append_kernel<kD, kQ8, false>,
+    return with_form(head_dim, form, [&](auto dim, auto codes) {
+        constexpr int kD = decltype(dim)::value, kF = decltype(codes)::value;
+        return launch("kv_append_kernel", vec ? kv_append_kernel<kD, kF, true> : kv_append_kernel<kD, kF, false>,
                       dim3(static_cast<unsigned>(grid)), dim3(kAppendThreads), 0, as_hip(stream), a);
     });
 }
@@ -1516,7 +1697,8 @@ int splits_for(long long fill, long long jobs, long long n, int most) {
 //                  25.6 / 72.9, p 8192 x 2048 82 / 107, p 16384 x 4096 269 / 235
 // One rule by steps does not fit all: 4 s 4096 rows of 64 dims over int8 caches with
 // a window of 256 take 74 in the form for few, 54 in the other.
-bool takes_many(long long total, long long heads, long long keys, int head_dim, bool q8) {
+bool takes_many(long long total, long long heads, long long keys, int head_dim, Kv form) {
+    const bool q8 = form == kI8;
     if (total <= kRows) return false;
     const int wide = kManyWaves * kWideRows;
     const long long pieces = heads * ((keys + kLeastKeys - 1) / kLeastKeys);
@@ -1571,7 +1753,7 @@ Plan finish(Plan p, int head_dim) {
     return p;
 }
 
-Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, bool q8, int rows, int window,
+Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, Kv form, int rows, int window,
                  int sinks) {
     Plan p{};
     p.rows = static_cast<size_t>(n_seq) * n_tokens * n_heads;
@@ -1585,7 +1767,7 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, b
         const long long near = static_cast<long long>(window) + sinks + kManyWaves * kWideRows / (n_heads / n_kv);
         keys = near < keys ? near : keys;
     }
-    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, keys, head_dim, q8);
+    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, keys, head_dim, form);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
     if (!p.many && n * head_dim <= kAlone)
@@ -1599,12 +1781,12 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, b
     return finish(p, head_dim);
 }
 
-Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, bool q8, int prefix_len, int own_rows) {
+Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, Kv form, int prefix_len, int own_rows) {
     Plan p{};
     p.rows = static_cast<size_t>(n_seq) * n_heads;
     const int group = n_heads / n_kv;
     const long long total = static_cast<long long>(n_seq) * group;
-    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, q8);
+    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, form);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
     const int own_splits = splits_for(kFillFew, p.own_jobs, own_rows, kMaxSlots / 4);
@@ -1648,18 +1830,19 @@ asdsl_status work_of(const char* what, const Plan& p, void* work, size_t work_by
     return work_buffer(as_hip(stream), work, work_bytes, p.work, &out, what);
 }
 
-asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, const int* pos, float* out, int n_seq,
+asdsl_status window(const char* what, Kv form, const float* q, const Cache& c, const int* pos, float* out, int n_seq,
                     int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows, int window, int sinks,
                     void* work, size_t work_bytes, asdsl_stream_t stream) {
     ASDSL_CHECK_ARG(q && c.k && c.v && pos && out, "%s: null pointer", what);
-    ASDSL_CHECK_ARG(!q8 || (c.ks && c.vs), "%s: null scale array", what);
-    asdsl_status st = check_heads(what, n_seq, n_tokens, n_heads, n_kv_heads, head_dim);
+    asdsl_status st = check_scales(what, form, c.ks, c.vs);
+    if (st != ASDSL_OK) return st;
+    st = check_heads(what, n_seq, n_tokens, n_heads, n_kv_heads, head_dim);
     if (st != ASDSL_OK) return st;
     ASDSL_CHECK_ARG(rows > 0 && rows <= kMaxRows, "%s: rows must be positive and at most 2^30", what);
     ASDSL_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window and sinks must not be negative", what);
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(c.k) && aligned16(c.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
-    const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, q8, rows, window, sinks);
+    const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, form, rows, window, sinks);
     st = check_launches(what, p);
     if (st != ASDSL_OK) return st;
     st = work_of(what, p, work, work_bytes, stream);
@@ -1669,19 +1852,18 @@ asdsl_status window(const char* what, bool q8, const float* q, const Cache& c, c
     place_work(g, p, work, head_dim);
     const dim3 grid(static_cast<unsigned>(p.jobs));
     auto with = [&](auto dim, auto codes) {
-        constexpr int kD = decltype(dim)::value;
-        constexpr bool kQ8 = decltype(codes)::value;
+        constexpr int kD = decltype(dim)::value, kF = decltype(codes)::value;
         if (!p.many)
-            return launch("window_few_kernel", window_few_kernel<kD, kQ8>, grid, dim3(kFewWaves * 64), 0,
+            return launch("window_few_kernel", window_few_kernel<kD, kF>, grid, dim3(kFewWaves * 64), 0,
                           as_hip(stream), g);
-        return launch("window_many_kernel", window_many_kernel<kD, kQ8>, grid, dim3(kManyWaves * 64), 0,
+        return launch("window_many_kernel", window_many_kernel<kD, kF>, grid, dim3(kManyWaves * 64), 0,
                       as_hip(stream), g);
     };
-    st = with_form(head_dim, q8, with);
+    st = with_form(head_dim, form, with);
     return st != ASDSL_OK ? st : join(g, p, head_dim, stream);
 }
 
-asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shared, const Cache& own,
+asdsl_status prefix(const char* what, Kv form, const float* q, const Cache& shared, const Cache& own,
                     const int* own_pos, float* out, int n_seq, int n_heads, int n_kv_heads, int head_dim,
                     int prefix_len, int prefix_rows, int own_rows, void* work, size_t work_bytes,
                     asdsl_stream_t stream) {
@@ -1689,15 +1871,16 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
     ASDSL_CHECK_ARG(prefix_len >= 0 && prefix_len <= prefix_rows && prefix_len <= kMaxRows,
                     "%s: prefix_len must be in [0, prefix_rows] and at most 2^30", what);
     ASDSL_CHECK_ARG(prefix_len == 0 || (shared.k && shared.v), "%s: null pointer", what);
-    ASDSL_CHECK_ARG(!q8 || (own.ks && own.vs && (prefix_len == 0 || (shared.ks && shared.vs))),
-                    "%s: null scale array", what);
-    asdsl_status st = check_heads(what, n_seq, 1, n_heads, n_kv_heads, head_dim);
+    asdsl_status st = check_scales(what, form, own.ks, own.vs);
+    if (st == ASDSL_OK && prefix_len > 0) st = check_scales(what, form, shared.ks, shared.vs);
+    if (st != ASDSL_OK) return st;
+    st = check_heads(what, n_seq, 1, n_heads, n_kv_heads, head_dim);
     if (st != ASDSL_OK) return st;
     ASDSL_CHECK_ARG(own_rows > 0 && own_rows <= kMaxRows, "%s: own_rows must be positive and at most 2^30", what);
     ASDSL_CHECK_ARG(aligned16(q) && aligned16(shared.k) && aligned16(shared.v) && aligned16(own.k) &&
                         aligned16(own.v) && aligned16(out),
                     "%s: q, caches and out must be 16-byte aligned", what);
-    const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, q8, prefix_len, own_rows);
+    const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, form, prefix_len, own_rows);
     st = check_launches(what, p);
     if (st != ASDSL_OK) return st;
     st = work_of(what, p, work, work_bytes, stream);
@@ -1705,10 +1888,9 @@ asdsl_status prefix(const char* what, bool q8, const float* q, const Cache& shar
     AttnArgs g{q, out, nullptr, nullptr, shared, own, own_pos, n_seq, 1, n_heads, n_kv_heads, prefix_rows, own_rows,
                prefix_len, 0, 0, 0, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    st = with_form(head_dim, q8, [&](auto dim, auto codes) {
-        constexpr int kD = decltype(dim)::value;
-        constexpr bool kQ8 = decltype(codes)::value;
-        return launch("prefix_kernel", p.many ? prefix_kernel<kD, kQ8, true> : prefix_kernel<kD, kQ8, false>,
+    st = with_form(head_dim, form, [&](auto dim, auto codes) {
+        constexpr int kD = decltype(dim)::value, kF = decltype(codes)::value;
+        return launch("prefix_kernel", p.many ? prefix_kernel<kD, kF, true> : prefix_kernel<kD, kF, false>,
                       dim3(static_cast<unsigned>(p.jobs + p.own_jobs)), dim3(kFewWaves * 64), 0, as_hip(stream), g,
                       p.splits, static_cast<int>(p.jobs));
     });
@@ -1725,7 +1907,7 @@ extern "C" asdsl_status asdsl_kv_append_f16(const float* qkv, uint16_t* k_cache,
                                             float* q_out, int n_seq, int n_tokens, int n_heads, int n_kv_heads,
                                             int head_dim, int rotary_dim, int rows, int pos_offset, int rope_rows,
                                             asdsl_stream_t stream) {
-    return append("kv_append_f16", false, qkv, k_cache, v_cache, nullptr, nullptr, rope_cos, rope_sin, pos, q_out,
+    return append("kv_append_f16", kF16, qkv, k_cache, v_cache, nullptr, nullptr, rope_cos, rope_sin, pos, q_out,
                   n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, rows, pos_offset, rope_rows, stream);
 }
 
@@ -1734,8 +1916,17 @@ extern "C" asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, in
                                            const int* pos, float* q_out, int n_seq, int n_tokens, int n_heads,
                                            int n_kv_heads, int head_dim, int rotary_dim, int rows, int pos_offset,
                                            int rope_rows, asdsl_stream_t stream) {
-    return append("kv_append_q8", true, qkv, k_cache, v_cache, k_scale, v_scale, rope_cos, rope_sin, pos, q_out,
+    return append("kv_append_q8", kI8, qkv, k_cache, v_cache, k_scale, v_scale, rope_cos, rope_sin, pos, q_out,
                   n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, rows, pos_offset, rope_rows, stream);
+}
+
+extern "C" asdsl_status asdsl_kv_append_q4(const float* qkv, uint8_t* k_cache, uint8_t* v_cache, uint16_t* k_scale,
+                                           uint16_t* v_scale, const float* rope_cos, const float* rope_sin,
+                                           const int* pos, float* q_out, int n_seq, int n_tokens, int n_heads,
+                                           int n_kv_heads, int head_dim, int rotary_dim, int rows, int pos_offset,
+                                           int rope_rows, asdsl_stream_t stream) {
+    return append("kv_append_q4", kI4, qkv, k_cache, v_cache, k_scale, v_scale, rope_cos, rope_sin, pos, q_out, n_seq,
+                  n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, rows, pos_offset, rope_rows, stream);
 }
 
 extern "C" size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
@@ -1743,9 +1934,9 @@ extern "C" size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int
     if (check_heads("attention_window", n_seq, n_tokens, n_heads, n_kv_heads, head_dim) != ASDSL_OK || rows <= 0 ||
         rows > kMaxRows || window_size < 0 || sinks < 0)
         return 0;
-    size_t most = 0;  // of the two cache types
-    for (const bool q8 : {false, true}) {
-        const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, q8, rows, window_size, sinks);
+    size_t most = 0;  // of the cache types
+    for (const Kv form : {kF16, kI8, kI4}) {
+        const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, form, rows, window_size, sinks);
         most = p.work > most ? p.work : most;
     }
     return most;
@@ -1756,7 +1947,7 @@ extern "C" asdsl_status asdsl_attention_window_f16kv(const float* q, const uint1
                                                      int n_kv_heads, int head_dim, int rows, int window_size,
                                                      int sinks, void* work, size_t work_bytes,
                                                      asdsl_stream_t stream) {
-    return window("attention_window_f16kv", false, q, Cache{k_cache, v_cache, nullptr, nullptr}, pos, out, n_seq,
+    return window("attention_window_f16kv", kF16, q, Cache{k_cache, v_cache, nullptr, nullptr}, pos, out, n_seq,
                   n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks, work, work_bytes, stream);
 }
 
@@ -1765,7 +1956,16 @@ extern "C" asdsl_status asdsl_attention_window_q8kv(const float* q, const int8_t
                                                     float* out, int n_seq, int n_tokens, int n_heads, int n_kv_heads,
                                                     int head_dim, int rows, int window_size, int sinks, void* work,
                                                     size_t work_bytes, asdsl_stream_t stream) {
-    return window("attention_window_q8kv", true, q, Cache{k_cache, v_cache, k_scale, v_scale}, pos, out, n_seq,
+    return window("attention_window_q8kv", kI8, q, Cache{k_cache, v_cache, k_scale, v_scale}, pos, out, n_seq,
+                  n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks, work, work_bytes, stream);
+}
+
+extern "C" asdsl_status asdsl_attention_window_q4kv(const float* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                                    const uint16_t* k_scale, const uint16_t* v_scale, const int* pos,
+                                                    float* out, int n_seq, int n_tokens, int n_heads, int n_kv_heads,
+                                                    int head_dim, int rows, int window_size, int sinks, void* work,
+                                                    size_t work_bytes, asdsl_stream_t stream) {
+    return window("attention_window_q4kv", kI4, q, Cache{k_cache, v_cache, k_scale, v_scale}, pos, out, n_seq,
                   n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks, work, work_bytes, stream);
 }
 
@@ -1774,9 +1974,9 @@ extern "C" size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int 
     if (check_heads("attention_prefix", n_seq, 1, n_heads, n_kv_heads, head_dim) != ASDSL_OK || prefix_len < 0 ||
         prefix_len > kMaxRows || own_rows <= 0 || own_rows > kMaxRows)
         return 0;
-    size_t most = 0;  // of the two cache types
-    for (const bool q8 : {false, true}) {
-        const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, q8, prefix_len, own_rows);
+    size_t most = 0;  // of the cache types
+    for (const Kv form : {kF16, kI8, kI4}) {
+        const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, form, prefix_len, own_rows);
         most = p.work > most ? p.work : most;
     }
     return most;
@@ -1788,7 +1988,7 @@ extern "C" asdsl_status asdsl_attention_prefix_f16kv(const float* q, const uint1
                                                      int n_heads, int n_kv_heads, int head_dim, int prefix_len,
                                                      int prefix_rows, int own_rows, void* work, size_t work_bytes,
                                                      asdsl_stream_t stream) {
-    return prefix("attention_prefix_f16kv", false, q, Cache{k_prefix, v_prefix, nullptr, nullptr},
+    return prefix("attention_prefix_f16kv", kF16, q, Cache{k_prefix, v_prefix, nullptr, nullptr},
                   Cache{k_own, v_own, nullptr, nullptr}, own_pos, out, n_seq, n_heads, n_kv_heads, head_dim,
                   prefix_len, prefix_rows, own_rows, work, work_bytes, stream);
 }
@@ -1800,7 +2000,20 @@ extern "C" asdsl_status asdsl_attention_prefix_q8kv(const float* q, const int8_t
                                                     int n_seq, int n_heads, int n_kv_heads, int head_dim,
                                                     int prefix_len, int prefix_rows, int own_rows, void* work,
                                                     size_t work_bytes, asdsl_stream_t stream) {
-    return prefix("attention_prefix_q8kv", true, q, Cache{k_prefix, v_prefix, k_prefix_scale, v_prefix_scale},
+    return prefix("attention_prefix_q8kv", kI8, q, Cache{k_prefix, v_prefix, k_prefix_scale, v_prefix_scale},
+                  Cache{k_own, v_own, k_own_scale, v_own_scale}, own_pos, out, n_seq, n_heads, n_kv_heads, head_dim,
+                  prefix_len, prefix_rows, own_rows, work, work_bytes, stream);
+}
+
+extern "C" asdsl_status asdsl_attention_prefix_q4kv(const float* q, const uint8_t* k_prefix, const uint8_t* v_prefix,
+                                                    const uint16_t* k_prefix_scale, const uint16_t* v_prefix_scale,
+                                                    const uint8_t* k_own, const uint8_t* v_own,
+                                                    const uint16_t* k_own_scale, const uint16_t* v_own_scale,
+                                                    const int* own_pos, float* out, int n_seq, int n_heads,
+                                                    int n_kv_heads, int head_dim, int prefix_len, int prefix_rows,
+                                                    int own_rows, void* work, size_t work_bytes,
+                                                    asdsl_stream_t stream) {
+    return prefix("attention_prefix_q4kv", kI4, q, Cache{k_prefix, v_prefix, k_prefix_scale, v_prefix_scale},
                   Cache{k_own, v_own, k_own_scale, v_own_scale}, own_pos, out, n_seq, n_heads, n_kv_heads, head_dim,
                   prefix_len, prefix_rows, own_rows, work, work_bytes, stream);
 }

@@ -636,7 +636,12 @@ asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, const int* to
  * Operators beside the single-sequence decode step.  Caches are
  * [n_seq][n_kv_heads][rows][head_dim], fp16, or int8 codes with fp32 scales
  * [n_seq][n_kv_heads][rows][head_dim / 64] (the decode step's two forms; its
- * caches are such caches with n_seq = 1); queries and outputs are fp32
+ * caches are such caches with n_seq = 1), or 4-bit codes, two a byte with the
+ * low nibble the even dim's, [n_seq][n_kv_heads][rows][head_dim / 2], with words
+ * [n_seq][n_kv_heads][rows][head_dim / 32].  A word holds an fp16 scale of 7
+ * significant bits and, in the 4 low bits that such a scale leaves, a zero point
+ * z: value = (code - z) * scale, exactly an fp16 number (infinite past its
+ * range).  Queries and outputs are fp32
  * [n_seq * n_tokens][n_heads][head_dim], token t of sequence s in row
  * s * n_tokens + t.  head_dim is 64 or 128, n_heads any multiple of n_kv_heads.
  * qkv, q, out, q_out and the caches are 16-byte aligned.  An int8 cache's value
@@ -655,7 +660,12 @@ asdsl_status asdsl_decode_prefill(const asdsl_decode_model* model, const int* to
  * (rope_cos/rope_sin [rope_rows][rotary_dim / 2], half split, as in
  * asdsl_attention_f16kv): q_out = the rotated queries, the cache row = the
  * rotated key and the value, rounded to fp16 or quantized as
- * asdsl_attention_q8kv does, with the same bits.  A token whose row is outside
+ * asdsl_attention_q8kv does, with the same bits, or to 4 bits, in 64-bit
+ * arithmetic, keys as their rotated values in 64 bits: per 32 dims, held to
+ * +-2^15, lo = min(0, x), hi = max(0, x), scale = (hi - lo) / 15 rounded up to 7
+ * significant bits (below 2^-14 to a multiple of 2^-20, at least 2^-20), z =
+ * rne(-lo / scale), code = clamp(rne(x / scale) + z, 0, 15); with a value that is
+ * not finite the scale is NaN, and all 32 read as NaN.  A token whose row is outside
  * [0, rows), or whose position is outside the tables, writes no cache row, and
  * its q_out is zero.  q_out must not overlap qkv. */
 asdsl_status asdsl_kv_append_f16(const float* qkv, uint16_t* k_cache, uint16_t* v_cache, const float* rope_cos,
@@ -666,6 +676,22 @@ asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, int8_t* v_cac
                                 const float* rope_cos, const float* rope_sin, const int* pos, float* q_out, int n_seq,
                                 int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int rows,
                                 int pos_offset, int rope_rows, asdsl_stream_t stream);
+asdsl_status asdsl_kv_append_q4(const float* qkv, uint8_t* k_cache, uint8_t* v_cache, uint16_t* k_scale,
+                                uint16_t* v_scale, const float* rope_cos, const float* rope_sin, const int* pos,
+                                float* q_out, int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                int rotary_dim, int rows, int pos_offset, int rope_rows, asdsl_stream_t stream);
+
+/* Cache rows as the values they stand for: rows pos[s] .. pos[s] + n_rows - 1 of
+ * every KV head of sequence s (pos null: from row 0) to k_out and v_out
+ * [n_seq][n_kv_heads][n_rows][head_dim], fp32 or (out_fp32 0) fp16: int8 codes
+ * times their scale in fp32, rounded once more to fp16; 4-bit values exactly.
+ * Rows outside [0, rows) read as zero.  Caches and outputs 16-byte aligned. */
+asdsl_status asdsl_kv_read_q8(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale, const float* v_scale,
+                              const int* pos, void* k_out, void* v_out, int out_fp32, int n_seq, int n_kv_heads,
+                              int head_dim, int rows, int n_rows, asdsl_stream_t stream);
+asdsl_status asdsl_kv_read_q4(const uint8_t* k_cache, const uint8_t* v_cache, const uint16_t* k_scale,
+                              const uint16_t* v_scale, const int* pos, void* k_out, void* v_out, int out_fp32,
+                              int n_seq, int n_kv_heads, int head_dim, int rows, int n_rows, asdsl_stream_t stream);
 
 /* Attention with a sliding window and first tokens that stay visible: token t
  * of sequence s, at position p = pos[s] + t, sees cache rows j <= p with
@@ -673,7 +699,7 @@ asdsl_status asdsl_kv_append_q8(const float* qkv, int8_t* k_cache, int8_t* v_cac
  * out = softmax(q.K / sqrt(head_dim)) V over them.  A token whose position is
  * outside [0, rows) sees nothing: its out is zero (a padded sequence has pos
  * -n_tokens or less).  Rows that no token sees are not looked at, whatever
- * they hold.  An fp16 row with infinities or NaN reaches only the tokens that see
+ * they hold.  An fp16 or 4-bit row with infinities or NaN reaches only the tokens that see
  * it, as the definition has it: a score of +inf or NaN makes their outputs NaN, a
  * key of score -inf has no weight (out is zero where all have none), and an
  * infinite value is its dim's output at any weight (NaN at none).  Such tokens are
@@ -686,6 +712,10 @@ asdsl_status asdsl_attention_window_f16kv(const float* q, const uint16_t* k_cach
                                           size_t work_bytes, asdsl_stream_t stream);
 asdsl_status asdsl_attention_window_q8kv(const float* q, const int8_t* k_cache, const int8_t* v_cache,
                                          const float* k_scale, const float* v_scale, const int* pos, float* out,
+                                         int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
+                                         int window, int sinks, void* work, size_t work_bytes, asdsl_stream_t stream);
+asdsl_status asdsl_attention_window_q4kv(const float* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                                         const uint16_t* k_scale, const uint16_t* v_scale, const int* pos, float* out,
                                          int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
                                          int window, int sinks, void* work, size_t work_bytes, asdsl_stream_t stream);
 
@@ -709,6 +739,12 @@ asdsl_status asdsl_attention_prefix_q8kv(const float* q, const int8_t* k_prefix,
                                          const int* own_pos, float* out, int n_seq, int n_heads, int n_kv_heads,
                                          int head_dim, int prefix_len, int prefix_rows, int own_rows, void* work,
                                          size_t work_bytes, asdsl_stream_t stream);
+asdsl_status asdsl_attention_prefix_q4kv(const float* q, const uint8_t* k_prefix, const uint8_t* v_prefix,
+                                         const uint16_t* k_prefix_scale, const uint16_t* v_prefix_scale,
+                                         const uint8_t* k_own, const uint8_t* v_own, const uint16_t* k_own_scale,
+                                         const uint16_t* v_own_scale, const int* own_pos, float* out, int n_seq,
+                                         int n_heads, int n_kv_heads, int head_dim, int prefix_len, int prefix_rows,
+                                         int own_rows, void* work, size_t work_bytes, asdsl_stream_t stream);
 
 /* Control of the next token: logits [n_rows][vocab] -> out (may be logits
  * itself) and tokens[n_rows] (may be null), per row, each step rounded to fp32:
