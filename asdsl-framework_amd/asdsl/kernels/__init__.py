@@ -8,7 +8,8 @@ function names.  Every call runs on the GPU through libasdsl_hip.so.  The
 2- and 3-bit kernels and the CPU table-lookup (LUT) kernels of the reference
 are not part of this package.  Beside them, with no counterpart there, are the
 operators of many sequences and long contexts: ``kv_append``, ``kv_read``,
-``attention_window``, ``attention_prefix`` and ``control_logits``.
+``attention_window``, ``attention_prefix``, ``control_logits`` and
+``sample_logits``.
 """
 
 from asdsl.kernels import _native_gemv  # noqa: F401
@@ -22,7 +23,7 @@ from asdsl.kernels.gemv_sparse import (
     gemv_sparse_with_indices,
     has_native_sparse_kernel,
 )
-from asdsl.kernels.logits import control_logits
+from asdsl.kernels.logits import control_logits, sample_logits
 
 KERNEL_TIER = "HIP_GFX950"
 
@@ -44,4 +45,5 @@ __all__ = [
     "kv_append",
     "kv_read",
     "control_logits",
+    "sample_logits",
 ]

@@ -1,6 +1,7 @@
-"""Control of the next token on the HIP library: penalties for tokens that
-occurred, biases, a grammar's mask, and the greedy token of what is left.  No
-counterpart in the reference, whose decoding is plain greedy
+"""The choice of the next token on the HIP library: penalties for tokens that
+occurred, biases, a grammar's mask, and the greedy token of what is left; or a
+token drawn with temperature, top-k, top-p and min-p.  No counterpart in the
+reference, whose decoding is plain greedy
 (asdsl/kernels/native/unified_engine.cpp:207-233)."""
 
 from __future__ import annotations
@@ -98,3 +99,52 @@ def control_logits(logits, *, history=None, prompt_len=None, history_len=None, r
               a_prompt, a_len, cap, a_rep, a_freq, a_pres, a_bias, strides[0], a_allowed, strides[1], rows, vocab,
               None if work is None else work.data_ptr(), nbytes, _stream(dev))
     return out, tokens
+
+
+@functools.lru_cache(maxsize=4096)
+def _sample_bytes(rows: int, vocab: int) -> int:
+    return _hip.LIB.asdsl_sample_logits_work_bytes(rows, vocab)
+
+
+def sample_logits(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
+    """A token of each row drawn by its weights, and the share it had: (tokens, probs).
+
+    logits: fp32 [rows, vocab] (or one row's [vocab]), vocab at most 2^20, as
+    control_logits leaves them (pick=False).  uniform: fp32 [rows], the random
+    numbers, in [0, 1).  temperature, top_p, min_p: fp32 [rows]; top_k: int32
+    [rows]; each may be left out.  Per row, with the tokens ranked by logit and
+    equal ones by index:
+
+        w(v) = exp((x(v) - max x) / temperature)   (temperature left out: 1)
+        kept are the first top_k                   (0 or less: all)
+        of those the shortest part of the ranking that comes to
+            top_p of their total                   (1 or more: all; 0 or less: the first)
+        of those the ones with w >= min_p          (and always the first)
+        token = in index order the first whose running sum of kept weights
+            exceeds uniform * their sum
+
+    Weights are whole multiples of 2^-43, so sums are exact and a call gives the
+    same each time.  -inf and NaN are never taken; where the largest is +inf,
+    those share evenly.  A temperature that is not above 0 takes the first of the
+    ranking.  Returns int32 tokens [rows], -1 where no token has a weight, and
+    fp32 probs [rows], the token's share of the kept weights (0 for -1)."""
+    fn = "sample_logits"
+    if not isinstance(logits, _Tensor) or logits.dim() not in (1, 2) or logits.numel() == 0:
+        raise ValueError(f"{fn}: logits must be a device tensor [rows, vocab] or [vocab]")
+    vocab = logits.shape[-1]
+    n = logits.numel()
+    rows = n // vocab
+    if vocab > 1 << 20:
+        raise ValueError(f"{fn}: a vocabulary of at most 2^20 tokens")
+    dev = _device(logits)
+    at = (_addr(fn, dev, "logits", logits, _f32, n), _addr(fn, dev, "uniform", uniform, _f32, rows),
+          None if temperature is None else _addr(fn, dev, "temperature", temperature, _f32, rows),
+          None if top_k is None else _addr(fn, dev, "top_k", top_k, _i32, rows),
+          None if top_p is None else _addr(fn, dev, "top_p", top_p, _f32, rows),
+          None if min_p is None else _addr(fn, dev, "min_p", min_p, _f32, rows))
+    tokens, probs = logits.new_empty(rows, dtype=_i32), logits.new_empty(rows)
+    nbytes = _sample_bytes(rows, vocab)
+    work = _work(nbytes, logits)
+    _hip.call("asdsl_sample_logits", *at, tokens.data_ptr(), probs.data_ptr(), rows, vocab,
+              None if work is None else work.data_ptr(), nbytes, _stream(dev))
+    return tokens, probs

@@ -769,6 +769,23 @@ asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, 
                                   long long allowed_stride, int n_rows, int vocab, void* work, size_t work_bytes,
                                   asdsl_stream_t stream);
 
+/* The next token of each row drawn from logits [n_rows][vocab] (vocab at most
+ * 2^20) with a given random number uniform[row] in [0, 1).  w(v) = exp((x(v) -
+ * max x) / temperature), in whole units of 2^-43 (smaller ones are none: NaN and
+ * -inf have no weight, and where the largest is +inf only those have).  Tokens
+ * are ranked by logit, equal ones by index.  Kept are the first top_k (0 or less:
+ * all); of those the shortest part of the ranking whose weights come to at least
+ * top_p of their total (1 or more: all; 0 or less: the first); of those the ones
+ * with w >= min_p, and always the first.  tokens[row] = in index order the first
+ * whose running sum of kept weights exceeds uniform * their sum, probs[row] = its
+ * share of that sum; -1 and 0 where no token has a weight.  A temperature that is
+ * not above 0 takes the first of the ranking.  temperature, top_k, top_p and min_p
+ * [n_rows] may each be null: 1, all, all, all. */
+size_t asdsl_sample_logits_work_bytes(int n_rows, int vocab);
+asdsl_status asdsl_sample_logits(const float* logits, const float* uniform, const float* temperature,
+                                 const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs,
+                                 int n_rows, int vocab, void* work, size_t work_bytes, asdsl_stream_t stream);
+
 /* One layer's caches of the branches' own rows (device pointers):
  * [n_branches][n_kv_heads][own_rows][128], fp16 or int8 as the model's
  * kv_format, int8 with scales [n_branches][n_kv_heads][own_rows][2]. */

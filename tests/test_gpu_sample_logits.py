@@ -1,0 +1,249 @@
+"""Sampling on the GPU against its definition in 64 bits."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("temperature", "top_k", "top_p", "min_p")
+
+
+def dev(a):
+    import torch
+
+    return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def row_kept(x, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(indices in rising order, weights) of the kept tokens of one row."""
+    x = np.asarray(x, np.float64)
+    can = np.flatnonzero(x > -np.inf)
+    if len(can) == 0:
+        return can, np.zeros(0)
+    order = can[np.argsort(-x[can], kind="stable")]
+    with np.errstate(all="ignore"):
+        d = np.where(x[order] == x[order[0]], 0.0, x[order] - x[order[0]])
+        w = np.where(d == -np.inf, 0.0, np.exp(d / np.float64(temperature))) if temperature > 0 else np.zeros(len(d))
+    w[0] = 1.0
+    w[w < 2.0 ** -44] = 0.0
+    most = len(w) if temperature > 0 else 1
+    if top_k > 0:
+        most = min(most, top_k)
+    if top_p < 1:
+        run = np.cumsum(w[:most])
+        most = min(most, int(np.searchsorted(run, np.float64(top_p) * run[-1], side="left")) + 1)
+    keep = np.arange(len(w)) < most
+    keep &= (w >= min_p) & (w > 0)
+    keep[0] = True
+    ids, w = order[keep], w[keep]
+    by = np.argsort(ids)
+    return ids[by], w[by]
+
+
+def reference(x, u, **kw):
+    """(tokens, probs, room): room is how far u * total lies from the nearest border of the running sum, in totals."""
+    tokens, probs, room = [], [], []
+    for i in range(len(x)):
+        ids, w = row_kept(x[i], **{name: a[i] for name, a in kw.items()})
+        if len(ids) == 0:
+            tokens.append(-1), probs.append(0.0), room.append(1.0)
+            continue
+        run = np.cumsum(w)
+        at = np.clip(np.float64(u[i]) if u[i] > 0 else 0.0, 0, 1 - 2.0 ** -53) * run[-1]
+        j = min(int(np.searchsorted(run, at, side="right")), len(ids) - 1)
+        tokens.append(int(ids[j])), probs.append(w[j] / run[-1])
+        room.append(np.abs(np.concatenate([[0.0 if at > 0 else 1.0], run[:-1]]) - at).min() / run[-1] if at > 0 else 1)
+    return np.array(tokens, np.int32), np.array(probs), np.array(room)
+
+
+def run(x, u, **kw):
+    from asdsl.kernels import sample_logits
+
+    tokens, probs = sample_logits(dev(x), dev(np.asarray(u, np.float32)), **{n: dev(a) for n, a in kw.items()})
+    return tokens.cpu().numpy(), probs.cpu().numpy()
+
+
+def check(x, u, **kw):
+    got, probs = run(x, u, **kw)
+    want, share, room = reference(x, u, **kw)
+    # a weight is off by half a unit of 2^-43 and by 2^-43 of fp64 rounding at most, a sum of n of them by n of those:
+    # beside a border by less than that either token is the definition's
+    near = room < x.shape[1] * 2.0 ** -42
+    assert near.sum() <= 1 + len(near) // 50  # draws beside a border are rare
+    assert np.array_equal(got[~near], want[~near]), (got, want)
+    # rounded to fp32 once; the sums' own error is far below
+    same = got == want
+    assert (np.abs(probs - share)[same] <= share[same] * (2.0 ** -24 + x.shape[1] * 2.0 ** -42)).all()
+
+
+def settings(rng, rows, form):
+    kw = {}
+    if form != "plain":
+        kw["temperature"] = rng.uniform(0.3, 2.0, rows).astype(np.float32)
+    if form in ("k", "all"):
+        kw["top_k"] = rng.choice([0, 1, 2, 7, 40, 1000, 10 ** 6, -3], rows).astype(np.int32)
+    if form in ("p", "all"):
+        kw["top_p"] = rng.choice([0.0, 0.1, 0.5, 0.9, 0.99, 1.0, 1.5, -1.0], rows).astype(np.float32)
+    if form in ("min", "all"):
+        kw["min_p"] = rng.choice([0.0, 0.01, 0.2, 1.0, 1.5, -1.0], rows).astype(np.float32)
+    return kw
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (2, 255), (5, 256), (4, 1023), (3, 1025), (7, 4099), (30, 5003),
+                                        (2, 32003), (3, 131072), (2, 200064), (600, 300), (1, 1 << 20)])
+@pytest.mark.parametrize("form", ["plain", "temperature", "k", "p", "min", "all"])
+def test_sample(gpu, rows, vocab, form):
+    rng = np.random.default_rng(rows * vocab + len(form))
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    check(x, rng.random(rows, dtype=np.float32), **settings(rng, rows, form))
+
+
+@pytest.mark.parametrize("vocab", [9, 9001, 70000])
+def test_flat_and_tied_logits(gpu, vocab):
+    """All or many logits equal: cuts fall among ties, by index; the lists overflow."""
+    rng = np.random.default_rng(vocab)
+    rows = 24
+    for x in (np.zeros((rows, vocab), np.float32), np.round(rng.standard_normal((rows, vocab))).astype(np.float32),
+              (rng.integers(0, 2, (rows, vocab)) * -0.0).astype(np.float32)):
+        kw = {"top_k": rng.integers(1, vocab + 1, rows).astype(np.int32),
+              "top_p": rng.uniform(0.05, 1, rows).astype(np.float32)}
+        u = rng.random(rows, dtype=np.float32)
+        for use in (("top_k",), ("top_p",), ("top_k", "top_p")):
+            check(x, u, **{n: kw[n] for n in use})
+        # a tie's border is a whole number of equal weights, which the sums hold exactly
+        half = {"top_k": np.full(rows, 4, np.int32), "top_p": np.full(rows, 0.5, np.float32)}
+        if not x.any():
+            got = run(x, np.full(rows, 0.5, np.float32), **half)
+            assert (got[0] == 1).all() and (got[1] == 0.5).all()
+
+
+def test_every_kept_token_by_its_share(gpu):
+    """u over a grid draws each kept token as often as its share, in index order, and no other."""
+    rng = np.random.default_rng(1)
+    vocab, rows = 700, 4096
+    x = np.repeat((rng.standard_normal((1, vocab)) * 2).astype(np.float32), rows, axis=0)
+    u = (np.arange(rows) / rows).astype(np.float32)
+    kw = {"temperature": 0.8, "top_k": 60, "top_p": 0.9, "min_p": 0.02}
+    ids, w = row_kept(x[0], **{n: np.float32(v) if n != "top_k" else v for n, v in kw.items()})
+    got, probs = run(x, u, **{n: np.full(rows, v, np.int32 if n == "top_k" else np.float32) for n, v in kw.items()})
+    assert (np.diff(got) >= 0).all() and set(got) <= set(ids.tolist())
+    share = w / w.sum()
+    times = np.array([(got == i).sum() for i in ids])
+    assert (np.abs(times - share * rows) <= 1).all()
+    assert np.allclose(probs, share[np.searchsorted(ids, got)], rtol=2.0 ** -23)
+
+
+def test_odd_values(gpu):
+    """Infinities, NaN, rows with nothing to draw, zeros of both signs, settings and numbers past their ranges."""
+    x = np.zeros((12, 70), np.float32)
+    x[0] = -np.inf
+    x[1] = np.nan
+    x[2, 5], x[2, 60], x[2, 61] = np.inf, np.inf, np.nan
+    x[3], x[3, 33] = -np.inf, -3e38
+    x[4, ::2] = -0.0
+    x[5, 7:9] = 3e38, -3e38
+    x[6, 0], x[6, 69] = np.nan, 1.0
+    u = np.array([.5, .5, .75, .9, .51, .3, .999999, 1.0, -2.0, np.nan, 5.0, 0.0], np.float32)
+    got, probs = run(x, u)
+    assert got[:4].tolist() == [-1, -1, 60, 33] and got[5] == 7 and probs[:4].tolist() == [0, 0, .5, 1]
+    assert got[4] == 35 and got[6] == 69 and got[7] == 69 and got[8] == 0 and got[9] == 0 and got[10] == 69
+    assert got[11] == 0
+    check(x[2:7], u[2:7])
+    nan = np.full(12, np.nan, np.float32)
+    assert np.array_equal(run(x, u, top_p=nan, min_p=nan)[0], got)
+    for t in (0.0, -1.0, np.nan):  # the first of the ranking
+        first = run(x, u, temperature=np.full(12, t, np.float32))
+        assert first[0].tolist() == [-1, -1, 5, 33, 0, 7, 69, 0, 0, 0, 0, 0]
+        assert first[1].tolist() == [0, 0] + [1] * 10
+    hot = run(x, u, temperature=np.full(12, np.inf, np.float32))[0]  # all that are finite share evenly
+    assert hot[0] == -1 and hot[2] == 60 and hot[3] == 33 and hot[5] == 21 and hot[4] == 35
+    cold = run(x[4:6], u[4:6], temperature=np.full(2, 1e-45, np.float32))[0]
+    assert cold.tolist() == [35, 7]
+
+
+def test_one_row_another_stream_and_graphs(gpu):
+    """One row's [vocab]; two captured graphs replayed in turn with new numbers and logits, eager calls between."""
+    import torch
+
+    from asdsl.kernels import control_logits, sample_logits
+
+    rng = np.random.default_rng(9)
+    rows, vocab = 3, 50257
+    x = dev((rng.standard_normal((rows, vocab)) * 3).astype(np.float32))
+    u = dev(rng.random(rows, dtype=np.float32))
+    kw = {"temperature": dev(np.array([.7, 1.0, 1.3], np.float32)), "top_k": dev(np.array([50, 0, 3000], np.int32)),
+          "top_p": dev(np.array([.9, .95, .8], np.float32)), "min_p": dev(np.array([.02, 0, .01], np.float32))}
+    words = dev(rng.integers(-2 ** 31, 2 ** 31, (rows, (vocab + 31) // 32)).astype(np.int32))
+    one = sample_logits(x[0], u[:1], top_p=kw["top_p"][:1])
+    assert one[0].tolist() == sample_logits(x[:1], u[:1], top_p=kw["top_p"][:1])[0].tolist()
+
+    def step():
+        y, _ = control_logits(x, allowed=words, pick=False)
+        return sample_logits(y, u, **kw)
+
+    side = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = step()
+        graphs.append((g, out))
+    for i in range(8):
+        x.copy_(dev((rng.standard_normal((rows, vocab)) * 3).astype(np.float32)))
+        u.copy_(dev(rng.random(rows, dtype=np.float32)))
+        want = step()
+        torch.cuda.synchronize()
+        g, out = graphs[i % 2]
+        with torch.cuda.stream(side):
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        allowed = (words.cpu().numpy().astype(np.uint32)[np.arange(rows), want[0].cpu() // 32] >>
+                   (want[0].cpu().numpy() % 32).astype(np.uint32)) & 1
+        assert allowed.all()
+
+
+def test_two_streams_at_once_and_the_same_each_time(gpu):
+    import torch
+
+    from asdsl.kernels import sample_logits
+
+    rng = np.random.default_rng(10)
+    x = [dev((rng.standard_normal((16, 60000)) * 3).astype(np.float32)) for _ in range(2)]
+    u = dev(rng.random(16, dtype=np.float32))
+    p = dev(rng.uniform(0.5, 1, 16).astype(np.float32))
+    want = [sample_logits(a, u, top_p=p) for a in x]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for a, st in zip(x, streams):
+            with torch.cuda.stream(st):
+                got.append(sample_logits(a, u, top_p=p))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
+def test_more_than_2_31_logits(gpu):
+    import torch
+
+    from asdsl.kernels import sample_logits
+
+    rows, vocab = 11_000, 200_064
+    assert rows * vocab > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((rows, vocab), device="cuda").normal_(generator=gen).mul_(3)
+    u = torch.rand(rows, generator=gen, device="cuda")
+    p = torch.full((rows,), 0.9, device="cuda")
+    at = [0, 1, rows // 2, rows - 1]
+    tokens, probs = sample_logits(x, u, top_p=p)
+    want, share, room = reference(x[at].cpu().numpy(), u[at].cpu().numpy(), top_p=p[at].cpu().numpy())
+    assert (room > vocab * 2.0 ** -42).all() and np.array_equal(tokens[at].cpu().numpy(), want)
+    assert np.allclose(probs[at].cpu().numpy(), share, rtol=2.0 ** -23)
