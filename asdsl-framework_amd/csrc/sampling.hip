@@ -13,6 +13,8 @@
 // last bits of the weights decide a whole number, so exponents are formed in fp64
 // (full rate here): 2^-43 a weight, against some 2^-24 in fp32, which over a flat
 // vocabulary of 200000 would move the token in some of every thousand draws.
+#include <type_traits>
+
 #include "abi_util.hpp"
 #include "device_common.hpp"
 
@@ -20,11 +22,12 @@ namespace asdsl {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 256;             // tokens of a wave's step, whose kept weight is noted
-constexpr int kStep = kThreads * 4;    // tokens of a workgroup's step
-constexpr int kBins = 256;             // of log2 weights in (-kDepth, 0]
-constexpr double kDepth = 44.0;
-constexpr int kListMost = 8192;        // tokens of the bins that a cut runs through
+constexpr int kTile = 1024;            // tokens of a wave's step, whose kept weight is noted
+constexpr int kStep = kThreads / kWave * kTile;  // tokens of a workgroup's step
+constexpr int kBins = 256;             // of log2 weights, between the row's largest and smallest
+constexpr double kDepth = 44.0;        // or 2^-kDepth, from which on there is no weight
+constexpr int kListMost = 4096;        // tokens of the bins that a cut runs through, of a row
+constexpr int kSliceMost = 1024;       // and of a slice
 constexpr int kMaxSlices = 64;
 constexpr int kMaxVocab = 1 << 20;     // 2^20 weights of 2^43 stay below 2^64
 constexpr double kLog2eWide = 1.4426950408889634074;
@@ -34,7 +37,7 @@ struct RowState {
     unsigned long long total;   // weight of all
     unsigned long long base_p;  // weight of the bins before the first that the cut of top-p may run through
     unsigned long long base_k;  // weight and tokens of those before the one that the cut of top-k runs through
-    int count_k;
+    uint32_t count_k;
     int bin_k;                  // that bin, kBins without a cut
     int p_lo, p_hi;             // and those of top-p, p_lo kBins without a cut
 };
@@ -49,13 +52,14 @@ struct SampleArgs {
     int* tokens;
     float* probs;
     unsigned long long* best;  // [rows][slices] largest logit and its first token
+    uint32_t* low;             // [rows][slices] smallest logit above -inf
     unsigned long long* mass;  // [rows][slices][kBins]
     uint32_t* count;           // [rows][slices][kBins]
     unsigned long long* tile;  // [rows][tiles]
     RowState* state;           // [rows]
-    uint32_t* listed;          // [rows]
-    uint2* list;               // [rows][list_cap] (logit, token)
-    int vocab, slices, slice, tiles, list_cap;
+    uint32_t* listed;          // [rows][slices], more than kSliceMost where the list does not hold them
+    uint2* list;               // [rows][slices][kSliceMost] (logit, token)
+    int vocab, slices, slice, tiles;
 };
 
 // Larger for a larger logit, equal for both zeros; 0 for none.
@@ -64,48 +68,67 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return (b >> 31) ? ~b : b | 0x80000000u;
 }
 
-// A row's weights.
-struct Scale {
-    float m;
-    double c;  // log2(e) / temperature
-    bool greedy;  // only the first is kept
+__device__ __forceinline__ float logit_of(uint32_t order) {
+    return __builtin_bit_cast(float, (order >> 31) ? order & 0x7FFFFFFFu : ~order);
+}
 
-    __device__ __forceinline__ Scale(const SampleArgs& a, int row, float top) : m(top) {
-        const float t = a.temperature ? a.temperature[row] : 1.0f;
+// What a row's slices found.
+struct Ends {
+    unsigned long long best;  // order_of the largest logit, and below it ~ its first token; 0: nothing to draw from
+    uint32_t low;             // order_of the smallest logit above -inf
+};
+
+// A row's weights.  Every kernel forms them with the same roundings (none is
+// contracted), so that what one counts is what the next one finds.
+struct Scale {
+    double m, c;      // largest logit, log2(e) / temperature
+    double per_bin;   // bins a unit of log2
+    bool infinite;    // the largest is +inf
+    bool greedy;      // only the first is kept
+
+    __device__ __forceinline__ Scale(const SampleArgs& a, int row, const Ends& e) {
+#pragma clang fp contract(off)
+        const float t = a.temperature ? a.temperature[row] : 1.0f, top = logit_of(static_cast<uint32_t>(e.best >> 32));
         greedy = !(t > 0.0f) || (a.top_k && a.top_k[row] == 1) || (a.top_p && a.top_p[row] <= 0.0f) ||
                  (a.min_p && a.min_p[row] > 1.0f);
+        infinite = top == INFINITY;
+        m = top;
         c = kLog2eWide / static_cast<double>(t);
+        const double depth = infinite ? 0.0 : fmin((m - static_cast<double>(logit_of(e.low))) * c, kDepth);
+        per_bin = depth > 0.0 ? kBins * (1.0 - 0x1p-30) / depth : 0.0;
     }
-    // log2 of a token's weight, -kDepth or less where it has none (NaN and -inf among them)
+    // log2 of a token's weight; any() is false where it has none (NaN and -inf among them)
     __device__ __forceinline__ double log2w(float x) const {
-        if (x == m) return 0.0;
-        const double d = static_cast<double>(x) - static_cast<double>(m);
-        return x > -INFINITY && d > -INFINITY ? d * c : -2.0 * kDepth;
+#pragma clang fp contract(off)
+        if (infinite) return x == INFINITY ? 0.0 : -2.0 * kDepth;
+        return (static_cast<double>(x) - m) * c;
     }
-    // 2^y in units of 2^-43, y in (-kDepth, 0]: a series of 2^f about 0 for |f| <= 1/2
-    // (its 13th term is below 2^-52), times a power of two; 2^52 + w is rounded to a
-    // whole number as it is added.
+    static __device__ __forceinline__ bool any(double y) { return y > -kDepth; }
+    // 2^y in units of 2^-43 where any(y): 2^n for the nearest whole number n times a
+    // polynomial for 2^f, |f| <= 1/2, through its values at 10 Chebyshev nodes (2^-45
+    // off at most); both sums with 2^52 round to a whole number.
     static __device__ __forceinline__ unsigned long long weight(double y) {
-        const double n = rint(y), f = (y - n) * 0.69314718055994530942;
-        double p = 1.0 / 479001600.0;
-        p = fma(p, f, 1.0 / 39916800.0);
-        p = fma(p, f, 1.0 / 3628800.0);
-        p = fma(p, f, 1.0 / 362880.0);
-        p = fma(p, f, 1.0 / 40320.0);
-        p = fma(p, f, 1.0 / 5040.0);
-        p = fma(p, f, 1.0 / 720.0);
-        p = fma(p, f, 1.0 / 120.0);
-        p = fma(p, f, 1.0 / 24.0);
-        p = fma(p, f, 1.0 / 6.0);
-        p = fma(p, f, 0.5);
-        p = fma(p, f, 1.0);
-        p = fma(p, f, 1.0);
-        const long long e = 1023 + 43 + static_cast<int>(n);
-        const double r = fma(p, __builtin_bit_cast(double, e << 52), 0x1p52);
-        return __builtin_bit_cast(unsigned long long, r) & 0xFFFFFFFFFFFFFull;
+#pragma clang fp contract(off)
+        const double shifted = y + 0x1.8p52;
+        const double f = y - (shifted - 0x1.8p52);
+        double p = 1.0205905686697933e-07;
+        p = fma(p, f, 1.325964524635787e-06);
+        p = fma(p, f, 1.525267292316862e-05);
+        p = fma(p, f, 0.0001540343375124206);
+        p = fma(p, f, 0.0013333558200798077);
+        p = fma(p, f, 0.00961812919393433);
+        p = fma(p, f, 0.05550410866465164);
+        p = fma(p, f, 0.2402265069564034);
+        p = fma(p, f, 0.6931471805599462);
+        p = fma(p, f, 1.0000000000000135);
+        const uint32_t n = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, shifted));
+        const uint64_t power = static_cast<uint64_t>((1023u + 43u + n) << 20) << 32;
+        return __builtin_bit_cast(uint64_t, fma(p, __builtin_bit_cast(double, power), 0x1p52)) & 0xFFFFFFFFFFFFFull;
     }
-    static __device__ __forceinline__ int bin(double y) {  // rising as weights fall
-        return min(static_cast<int>(y * (-kBins / kDepth)), kBins - 1);
+    // 0 .. kBins - 1, rising as weights fall
+    __device__ __forceinline__ int bin(double y) const {
+#pragma clang fp contract(off)
+        return static_cast<int>(y * -per_bin);
     }
 };
 
@@ -126,36 +149,90 @@ __device__ __forceinline__ uint32_t most_kept(const SampleArgs& a, int row) {
     return k > 0 ? static_cast<uint32_t>(k) : 0xFFFFFFFFu;
 }
 
-template <typename T, typename F>
-__device__ __forceinline__ T wave_all(T v, F f) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = f(v, __shfl_xor(v, o, kWave));
-    return v;
+// Running f over the lanes of a wave, all of them here: lane i's takes in lanes 0 ..
+// i.  Within rows of 16 lanes by shifts, then the last lane of a row for the next
+// row or two; moves between registers, some 150 cycles where exchanges through LDS
+// take 700.
+template <int CTRL, int kRows16, typename T>
+__device__ __forceinline__ T moved(T v, T none) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, none);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(static_cast<uint32_t>(b), static_cast<uint32_t>(a), CTRL, kRows16, 0xF, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(static_cast<uint32_t>(b >> 32), static_cast<uint32_t>(a >> 32), CTRL, kRows16,
+                                                        0xF, false);
+        return __builtin_bit_cast(T, (static_cast<uint64_t>(hi) << 32) | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(uint32_t, none),
+                                                                 __builtin_bit_cast(uint32_t, v), CTRL, kRows16, 0xF, false));
+    }
 }
 
-// f(token, logit) for a lane's 4 neighbouring tokens of every step of a slice, and
-// after(tile) by all lanes of a wave behind each; kVec: rows lie in whole 16-byte
-// units.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T v, T none, F f) {
+    constexpr int kRowShr = 0x110, kBcast15 = 0x142, kBcast31 = 0x143;
+    v = f(v, moved<kRowShr + 1, 0xF>(v, none));
+    v = f(v, moved<kRowShr + 2, 0xF>(v, none));
+    v = f(v, moved<kRowShr + 4, 0xF>(v, none));
+    v = f(v, moved<kRowShr + 8, 0xF>(v, none));
+    v = f(v, moved<kBcast15, 0xA>(v, none));
+    return f(v, moved<kBcast31, 0xC>(v, none));
+}
+
+template <typename T>
+__device__ __forceinline__ T last_lane(T v) {
+    if constexpr (sizeof(T) == 8) {
+        const uint64_t a = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(a), kWave - 1);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(a >> 32), kWave - 1);
+        return __builtin_bit_cast(T, (static_cast<uint64_t>(hi) << 32) | lo);
+    } else {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, v), kWave - 1));
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T running_sum(T v) { return wave_scan(v, T(0), [](T p, T q) { return p + q; }); }
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v) { return last_lane(running_sum(v)); }
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) { return last_lane(wave_scan(v, T(0), [](T p, T q) { return p > q ? p : q; })); }
+template <typename T>
+__device__ __forceinline__ T wave_min(T v) { return last_lane(wave_scan(v, static_cast<T>(~T(0)), [](T p, T q) { return p < q ? p : q; })); }
+
+// f(token, 4 logits) for a lane's chunks of 4 neighbouring tokens of a slice, -inf
+// past its end, and after(tile) by all lanes of a wave behind each of its tiles of
+// 4 chunks.  Loads are kAhead chunks ahead; the loop is kept short, since what
+// these kernels run once they also have to fetch as code.  kVec: rows lie in whole
+// 16-byte units.
+constexpr int kChunk = 4 * kWave;
+constexpr int kAhead = 4;
 template <bool kVec, typename F, typename G>
 __device__ __forceinline__ void over_slice(const SampleArgs& a, int row, int slice, F f, G after) {
     const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
-    const int end = min(a.vocab, (slice + 1) * a.slice);
-    for (int v0 = slice * a.slice; v0 < end; v0 += kStep) {
-        const int v = v0 + 4 * static_cast<int>(threadIdx.x);
+    const int end = min(a.vocab, (slice + 1) * a.slice), lane = static_cast<int>(threadIdx.x) % kWave;
+    const int v0 = slice * a.slice + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave) * kTile;
+    const auto at = [&](int c) { return v0 + c / 4 * kStep + c % 4 * kChunk; };
+    const auto load = [&](int c) {
+        const int v = at(c) + 4 * lane;
         if constexpr (kVec) {
-            if (v < end) {
-                const float4 q = *reinterpret_cast<const float4*>(x + v);
-                f(v, q.x); f(v + 1, q.y); f(v + 2, q.z); f(v + 3, q.w);
-            }
+            return v < end ? *reinterpret_cast<const float4*>(x + v)
+                           : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
         } else {
-            float q[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = v + i < end ? x[v + i] : -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (v + i < end) f(v + i, q[i]);
+            return make_float4(v < end ? x[v] : -INFINITY, v + 1 < end ? x[v + 1] : -INFINITY,
+                               v + 2 < end ? x[v + 2] : -INFINITY, v + 3 < end ? x[v + 3] : -INFINITY);
         }
-        after(v0 / kTile + static_cast<int>(threadIdx.x) / kWave);
+    };
+    static_assert(kTile == 4 * kChunk && kAhead == 4, "chunks of a tile, and of the registers below");
+    float4 b0 = load(0), b1 = load(1), b2 = load(2), b3 = load(3);
+#pragma unroll 1
+    for (int c = 0; at(c / 4 * 4) < end; ++c) {
+        const float q[4] = {b0.x, b0.y, b0.z, b0.w};
+        b0 = b1;
+        b1 = b2;
+        b2 = b3;
+        b3 = load(c + kAhead);
+        f(at(c) + 4 * lane, q);
+        if (c % 4 == 3) after(at(c) / kTile);
     }
 }
 
@@ -163,39 +240,52 @@ __device__ __forceinline__ void over_slice(const SampleArgs& a, int row, int sli
 template <bool kVec>
 __global__ __launch_bounds__(kThreads) void sample_best_kernel(const SampleArgs a) {
     __shared__ unsigned long long red[kThreads / kWave];
+    __shared__ uint32_t lows[kThreads / kWave];
     const int row = static_cast<int>(blockIdx.x) / a.slices, slice = static_cast<int>(blockIdx.x) % a.slices;
     unsigned long long best = 0ull;
-    over_slice<kVec>(a, row, slice, [&](int v, float x) {
-        if (x > -INFINITY) {
-            const unsigned long long key = (static_cast<unsigned long long>(order_of(x)) << 32) | (0xFFFFFFFFu - v);
-            best = key > best ? key : best;
-        }
+    uint32_t low = 0xFFFFFFFFu;
+    over_slice<kVec>(a, row, slice, [&](int v, const float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (x[i] > -INFINITY) {
+                const uint32_t o = order_of(x[i]);
+                const unsigned long long key = (static_cast<unsigned long long>(o) << 32) | (0xFFFFFFFFu - v - i);
+                best = key > best ? key : best;
+                low = min(low, o);
+            }
     }, [](int) {});
-    best = wave_all(best, [](auto p, auto q) { return p > q ? p : q; });
-    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = best;
+    best = wave_max(best);
+    low = wave_min(low);
+    if (threadIdx.x % kWave == 0) {
+        red[threadIdx.x / kWave] = best;
+        lows[threadIdx.x / kWave] = low;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kThreads / kWave; ++i) best = red[i] > best ? red[i] : best;
+        for (int i = 1; i < kThreads / kWave; ++i) {
+            best = red[i] > best ? red[i] : best;
+            low = min(low, lows[i]);
+        }
         a.best[blockIdx.x] = best;
-        if (slice == 0) a.listed[row] = 0u;
+        a.low[blockIdx.x] = low;
     }
 }
 
-// The row's largest logit, by every wave for itself (0: nothing to draw from).
-__device__ __forceinline__ unsigned long long row_best(const SampleArgs& a, int row) {
-    const int lane = static_cast<int>(threadIdx.x) % kWave;
-    unsigned long long best = lane < a.slices ? a.best[static_cast<size_t>(row) * a.slices + lane] : 0ull;
+// The row's ends from its slices', by every wave for itself.
+__device__ __forceinline__ Ends row_ends(const SampleArgs& a, int row) {
     static_assert(kMaxSlices <= kWave, "a lane a slice");
-    return wave_all(best, [](auto p, auto q) { return p > q ? p : q; });
-}
-
-__device__ __forceinline__ float logit_of(unsigned long long best) {
-    const uint32_t o = static_cast<uint32_t>(best >> 32);
-    return __builtin_bit_cast(float, (o >> 31) ? o & 0x7FFFFFFFu : ~o);
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    const size_t at = static_cast<size_t>(row) * a.slices + lane;
+    Ends e{0ull, 0xFFFFFFFFu};
+    if (lane < a.slices) e = Ends{a.best[at], a.low[at]};
+    e.best = wave_max(e.best);
+    e.low = wave_min(e.low);
+    return e;
 }
 
 // ------------------------------------------------------- weights by their size
-template <bool kVec>
+// kCount, kMass: what the cuts that the call asks for need (top-k, top-p).
+template <bool kVec, bool kCount, bool kMass>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a) {
     __shared__ unsigned long long mass[kBins];
     __shared__ uint32_t count[kBins];
@@ -203,61 +293,91 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
     static_assert(kBins == kThreads, "a thread a bin");
     mass[threadIdx.x] = 0ull;
     count[threadIdx.x] = 0u;
+    const Ends ends = row_ends(a, row);
+    const Scale s(a, row, ends);
+    if (ends.best == 0ull || s.greedy) return;
     __syncthreads();
-    const unsigned long long best = row_best(a, row);
-    const Scale s(a, row, logit_of(best));
-    if (best == 0ull || s.greedy) return;
-    over_slice<kVec>(a, row, slice, [&](int, float x) {
-        const double y = s.log2w(x);
-        if (y > -kDepth) {
-            const int b = Scale::bin(y);
-            atomicAdd(&mass[b], Scale::weight(y));
-            atomicAdd(&count[b], 1u);
+    over_slice<kVec>(a, row, slice, [&](int, const float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const double y = s.log2w(x[i]);
+            if (Scale::any(y)) {
+                const int b = s.bin(y);
+                if constexpr (kMass) atomicAdd(&mass[b], Scale::weight(y));
+                if constexpr (kCount) atomicAdd(&count[b], 1u);
+            }
         }
     }, [](int) {});
     __syncthreads();
     const size_t at = static_cast<size_t>(blockIdx.x) * kBins + threadIdx.x;
-    a.mass[at] = mass[threadIdx.x];
-    a.count[at] = count[threadIdx.x];
+    if constexpr (kMass) a.mass[at] = mass[threadIdx.x];
+    if constexpr (kCount) a.count[at] = count[threadIdx.x];
 }
 
 // --------------------------------------------- kept weights, and the cut's bins
 struct Bins {
     unsigned long long mass[kBins + 1];  // before bin b
     uint32_t count[kBins + 1];
-    unsigned long long wave_mass[kThreads / kWave];
-    uint32_t wave_count[kThreads / kWave];
+    union {
+        struct {
+            unsigned long long mass[kThreads / kWave][kBins];
+            uint32_t count[kThreads / kWave][kBins];
+        } part;
+        struct {
+            unsigned long long mass[kThreads / kWave];
+            uint32_t count[kThreads / kWave];
+        } wave;
+    };
     int first[3];
 };
 
+// The row's bins from its slices': a wave takes every fourth slice, 4 bins a lane.
+template <bool kCount, bool kMass>
 __device__ __forceinline__ void count_bins(const SampleArgs& a, int row, Bins& s) {
-    const int t = static_cast<int>(threadIdx.x), lane = t % kWave;
-    unsigned long long m = 0ull;
-    uint32_t n = 0u;
-    for (int i = 0; i < a.slices; ++i) {
-        const size_t at = (static_cast<size_t>(row) * a.slices + i) * kBins + t;
-        m += a.mass[at];
-        n += a.count[at];
-    }
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const unsigned long long mo = __shfl_up(m, o, kWave);
-        const uint32_t no = __shfl_up(n, o, kWave);
-        if (lane >= o) {
-            m += mo;
-            n += no;
+    const int t = static_cast<int>(threadIdx.x), lane = t % kWave, wave = t / kWave;
+    unsigned long long ms[4] = {};
+    uint32_t ns[4] = {};
+#pragma unroll 4
+    for (int i = wave; i < a.slices; i += kThreads / kWave) {
+        const size_t at = (static_cast<size_t>(row) * a.slices + i) * kBins + 4 * lane;
+        if constexpr (kMass) {
+            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(a.mass + at);
+            const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(a.mass + at + 2);
+            ms[0] += x.x; ms[1] += x.y; ms[2] += y.x; ms[3] += y.y;
+        }
+        if constexpr (kCount) {
+            const uint4 x = *reinterpret_cast<const uint4*>(a.count + at);
+            ns[0] += x.x; ns[1] += x.y; ns[2] += x.z; ns[3] += x.w;
         }
     }
-    if (lane == kWave - 1) {
-        s.wave_mass[t / kWave] = m;
-        s.wave_count[t / kWave] = n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        s.part.mass[wave][4 * lane + i] = ms[i];
+        s.part.count[wave][4 * lane + i] = ns[i];
     }
     if (t < 3) s.first[t] = kBins;
     __syncthreads();
-    for (int i = 0; i < t / kWave; ++i) {
-        m += s.wave_mass[i];
-        n += s.wave_count[i];
+    unsigned long long m = 0ull;
+    uint32_t n = 0u;
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave; ++i) {
+        m += s.part.mass[i][t];
+        n += s.part.count[i][t];
     }
+    __syncthreads();
+    m = running_sum(m);
+    n = running_sum(n);
+    if (lane == kWave - 1) {
+        s.wave.mass[wave] = m;
+        s.wave.count[wave] = n;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave - 1; ++i)
+        if (i < wave) {
+            m += s.wave.mass[i];
+            n += s.wave.count[i];
+        }
     s.mass[t + 1] = m;
     s.count[t + 1] = n;
     if (t == 0) {
@@ -273,12 +393,12 @@ __device__ __forceinline__ RowState find_bins(const SampleArgs& a, int row, Bins
     const uint32_t k = most_kept(a, row);
     if (s.count[t] < k && s.count[t + 1] >= k) s.first[0] = t;
     __syncthreads();
-    RowState r;
+    RowState r{};
     r.total = s.mass[kBins];
     r.bin_k = k < s.count[kBins] ? s.first[0] : kBins;
     const bool cut = r.bin_k < kBins;
     r.base_k = cut ? s.mass[r.bin_k] : 0ull;
-    r.count_k = cut ? static_cast<int>(s.count[r.bin_k]) : 0;
+    r.count_k = cut ? s.count[r.bin_k] : 0u;
     const float p = a.top_p ? a.top_p[row] : 1.0f;
     const bool part = p < 1.0f;
     const unsigned long long lo = share_of(p, cut ? s.mass[r.bin_k] : r.total);
@@ -292,320 +412,395 @@ __device__ __forceinline__ RowState find_bins(const SampleArgs& a, int row, Bins
     return r;
 }
 
-// Whether a bin's tokens are all kept by the cuts, or the cut may run through it.
-__device__ __forceinline__ bool before_cuts(const RowState& r, int b) { return b < min(r.p_lo, r.bin_k); }
-__device__ __forceinline__ bool in_cut(const RowState& r, int b) {
-    return b == r.bin_k || (b >= r.p_lo && b <= r.p_hi);
-}
+// One wave's tokens on their way to their weights, 64 at a time.
+constexpr int kQueue = 2 * kChunk;
+struct Queue {
+    float x[kQueue];
+    int v[kQueue];
+};
 
-// kCuts: top-k or top-p may cut.
-template <bool kVec, bool kCuts>
+// kCount, kMass: top-k or top-p may cut; kLeast: min_p may drop tokens.  Without
+// any a token goes straight to its weight, else those that a comparison of floats
+// cannot rule out go through a queue, so that the others cost no fp64 work.
+template <bool kVec, bool kCount, bool kMass, bool kLeast>
 __global__ __launch_bounds__(kThreads) void sample_keep_kernel(const SampleArgs a) {
-    __shared__ Bins bins;
+    constexpr bool kCuts = kCount || kMass, kDirect = !kCuts && !kLeast;
+    __shared__ std::conditional_t<kCuts, Bins, char> bins;
+    __shared__ Queue queues[kDirect ? 1 : kThreads / kWave];
+    __shared__ uint2 list[kCuts ? kSliceMost : 1];
+    __shared__ uint32_t listed;
     const int row = static_cast<int>(blockIdx.x) / a.slices, slice = static_cast<int>(blockIdx.x) % a.slices;
-    const unsigned long long best = row_best(a, row);
-    const Scale s(a, row, logit_of(best));
-    if (best == 0ull || s.greedy) return;
+    const int lane = static_cast<int>(threadIdx.x) % kWave, wave = static_cast<int>(threadIdx.x) / kWave;
+    const Ends ends = row_ends(a, row);
+    const Scale s(a, row, ends);
+    if (ends.best == 0ull || s.greedy) return;
     RowState r{};
     r.bin_k = r.p_lo = r.p_hi = kBins;
     if constexpr (kCuts) {
-        count_bins(a, row, bins);
+        if (threadIdx.x == 0) listed = 0u;
+        count_bins<kCount, kMass>(a, row, bins);
         r = find_bins(a, row, bins);
+        if (slice == 0 && threadIdx.x == 0) a.state[row] = r;
     }
-    if (slice == 0 && threadIdx.x == 0) a.state[row] = r;
     const unsigned long long least = least_weight(a, row);
-    const int lane = static_cast<int>(threadIdx.x) % kWave;
     unsigned long long sum = 0ull;
-    over_slice<kVec>(a, row, slice, [&](int v, float x) {
+    const auto store = [&](int tile) {
+        const unsigned long long all = wave_sum(sum);
+        if (lane == 0) a.tile[static_cast<size_t>(row) * a.tiles + tile] = all;
+        sum = 0ull;
+    };
+    if constexpr (kDirect) {
+        over_slice<kVec>(a, row, slice, [&](int, const float (&x)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const double y = s.log2w(x[i]);
+                if (Scale::any(y)) sum += Scale::weight(y);
+            }
+        }, store);
+        return;
+    }
+    // The bins that are kept whatever the cuts, and the last that may be touched by one.
+    const int before = min(r.p_lo, r.bin_k);
+    const int last = before == kBins ? kBins - 1 : max(r.p_lo < kBins ? r.p_hi : -1, r.bin_k < kBins ? r.bin_k : -1);
+    // No logit below `from` is in them: the bin's end, or min_p where nothing cuts, some 2^-22 lower.
+    double reach = s.per_bin > 0.0 ? (last + 1) / s.per_bin : kDepth;
+    if (before == kBins && least > 1ull) reach = fmin(reach, 43.0 - log2(static_cast<double>(least)));
+    const double edge = s.m - (reach + 0x1p-20) / s.c;
+    const float from = s.infinite ? INFINITY
+                                  : static_cast<float>(edge - (fabs(edge) + fabs(s.m)) * 0x1p-22 - 0x1p-140);
+    volatile Queue& queue = queues[wave];
+    int head = 0, held = 0;  // the same in every lane
+    const auto weigh = [&](int n) {
+        if (lane >= n) return;
+        const int at = (head + lane) % kQueue;
+        const float x = queue.x[at];
         const double y = s.log2w(x);
-        if (!(y > -kDepth)) return;
-        const int b = Scale::bin(y);
-        if (before_cuts(r, b)) {
+        if (!Scale::any(y)) return;
+        const int b = s.bin(y);
+        if (b < before) {
             const unsigned long long w = Scale::weight(y);
             if (w >= least) sum += w;
-        } else if (kCuts && in_cut(r, b)) {
-            const uint32_t at = atomicAdd(&a.listed[row], 1u);
-            if (at < static_cast<uint32_t>(a.list_cap))
-                a.list[static_cast<size_t>(row) * a.list_cap + at] = make_uint2(__builtin_bit_cast(uint32_t, x), v);
+        } else if (kCuts && (b == r.bin_k || (b >= r.p_lo && b <= r.p_hi))) {
+            const uint32_t i = atomicAdd(&listed, 1u);
+            if (i < kSliceMost) list[i] = make_uint2(__builtin_bit_cast(uint32_t, x), queue.v[at]);
+        }
+    };
+    over_slice<kVec>(a, row, slice, [&](int v, const float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool take = x[i] >= from;
+            const uint64_t mask = __builtin_amdgcn_ballot_w64(take);
+            if (take) {
+                const int at = (head + held + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0u))) % kQueue;
+                queue.x[at] = x[i];
+                if constexpr (kCuts) queue.v[at] = v + i;
+            }
+            held += __builtin_popcountll(mask);
+        }
+#pragma unroll 1
+        for (; held >= kWave; held -= kWave) {
+            weigh(kWave);
+            head = (head + kWave) % kQueue;
         }
     }, [&](int tile) {
-        const unsigned long long all = wave_all(sum, [](auto p, auto q) { return p + q; });
-        if (lane == 0 && tile < a.tiles) a.tile[static_cast<size_t>(row) * a.tiles + tile] = all;
-        sum = 0ull;
+        weigh(held);
+        head = held = 0;
+        store(tile);
     });
+    if constexpr (kCuts) {
+        __syncthreads();
+        if (threadIdx.x == 0) a.listed[blockIdx.x] = listed;
+        for (int i = static_cast<int>(threadIdx.x); i < static_cast<int>(min(listed, 1u * kSliceMost)); i += kThreads)
+            a.list[static_cast<size_t>(blockIdx.x) * kSliceMost + i] = list[i];
+    }
 }
 
 // ------------------------------------------------------------------ the token
 constexpr int kLast = 1024;   // threads
-constexpr int kSub = 2048;    // bins of one level of a selection
+constexpr int kPartBits = 8;
+constexpr int kParts = 1 << kPartBits;  // of one level of a selection, 4 a lane of one wave
 constexpr int kRankBits = 20;
+static_assert(kTile == kLast && kMaxVocab / kTile <= kLast, "a thread a token, a tile");
 
 // A token's place in the ranking: larger comes first, no two alike.
 __device__ __forceinline__ unsigned long long rank_of(float x, int v) {
     return (static_cast<unsigned long long>(order_of(x)) << kRankBits) | static_cast<unsigned long long>(kMaxVocab - 1 - v);
 }
+__device__ __forceinline__ int token_of(unsigned long long rank) {
+    return kMaxVocab - 1 - static_cast<int>(rank & (kMaxVocab - 1));
+}
 
 struct Last {
-    unsigned long long mass[kSub];
-    uint32_t count[kSub];
+    unsigned long long mass[kParts];
+    uint32_t count[kParts];
     unsigned long long wave_mass[kLast / kWave];
-    uint32_t wave_count[kLast / kWave];
     unsigned long long key[kWave], weight[kWave];
-    unsigned long long found, found_mass, total, target, before;
-    int found_bin;
-    uint32_t few;
-    int tile, token;
+    unsigned long long found, found_mass, total, target, before, low, high;
+    uint32_t found_count, found_held, few, upto[kMaxSlices];
+    int found_part, tile;
     unsigned long long tiles[kMaxVocab / kTile];
-    uint2 list[kListMost];
+    unsigned long long rank[kListMost], held[kListMost];  // held: weight, and the bin above kBinShift
 };
+constexpr int kBinShift = 48;
 
-// Running sums over the block: thread t's inclusive ones.
-__device__ __forceinline__ void block_scan(Last& s, unsigned long long& m, uint32_t& n) {
-    const int t = static_cast<int>(threadIdx.x), lane = t % kWave;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const unsigned long long mo = __shfl_up(m, o, kWave);
-        const uint32_t no = __shfl_up(n, o, kWave);
-        if (lane >= o) {
-            m += mo;
-            n += no;
-        }
-    }
-    if (lane == kWave - 1) {
-        s.wave_mass[t / kWave] = m;
-        s.wave_count[t / kWave] = n;
-    }
+// Running sums over the block: thread t's inclusive one.
+__device__ __forceinline__ unsigned long long block_scan(Last& s, unsigned long long m) {
+    const int t = static_cast<int>(threadIdx.x), wave = t / kWave;
+    m = running_sum(m);
+    if (t % kWave == kWave - 1) s.wave_mass[wave] = m;
     __syncthreads();
-    for (int i = 0; i < t / kWave; ++i) {
-        m += s.wave_mass[i];
-        n += s.wave_count[i];
-    }
+    m += wave_sum(t % kWave < wave ? s.wave_mass[t % kWave] : 0ull);
     __syncthreads();
+    return m;
 }
 
 // The tokens that a cut may fall on: the list, or where it did not hold them all the row.
 struct Source {
     const SampleArgs& a;
-    const RowState& r;
     const Scale& scale;
     Last& s;
     int row, n;
     bool whole;
-    // f(rank, weight) for those of bins [lo, hi]
+    // f(rank, weight) for those of bins [lo, hi] with ranks [low, low + span)
     template <typename F>
-    __device__ __forceinline__ void each(int lo, int hi, F f) const {
-        const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
-        for (int i = static_cast<int>(threadIdx.x); i < n; i += kLast) {
-            const float q = whole ? x[i] : __builtin_bit_cast(float, s.list[i].x);
-            const int v = whole ? i : static_cast<int>(s.list[i].y);
-            const double y = scale.log2w(q);
-            if (!(y > -kDepth)) continue;
-            const int b = Scale::bin(y);
-            if (b >= lo && b <= hi) f(rank_of(q, v), Scale::weight(y));
+    __device__ __forceinline__ void each(int lo, int hi, unsigned long long low, unsigned long long span, F f) const {
+        const int t = static_cast<int>(threadIdx.x);
+        if (whole) {
+            const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
+#pragma unroll 4
+            for (int i = t; i < n; i += kLast) {
+                const float q = x[i];
+                const unsigned long long key = rank_of(q, i);
+                const double y = scale.log2w(q);
+                if (key - low >= span || !Scale::any(y)) continue;
+                const int b = scale.bin(y);
+                if (b >= lo && b <= hi) f(key, Scale::weight(y));
+            }
+        } else {
+            for (int i = t; i < n; i += kLast) {
+                const unsigned long long w = s.held[i], key = s.rank[i];
+                const int b = static_cast<int>(w >> kBinShift);
+                if (key - low < span && b >= lo && b <= hi) f(key, w & ((1ull << kBinShift) - 1));
+            }
         }
     }
 };
 
 // The rank of the last kept token among those of bins [lo, hi], of which `mass` and
 // `count` come before: the first whose running count reaches `want_count` or
-// whose running weight reaches `want_mass`.  Level by level over a range of ranks in
-// kSub equal parts, until a part holds few; returns its rank and, in `mass`, the
-// weight up to and with it.
-__device__ unsigned long long select_rank(const Source& src, int lo, int hi, uint32_t want_count,
-                                          unsigned long long want_mass, uint32_t count, unsigned long long& mass) {
+// whose running weight reaches `want_mass`.  Level by level over a range of ranks
+// [s.low, s.high] in kParts equal parts, until a part holds no more than a wave;
+// returns its rank and, in `mass`, the weight up to and with it.  s.mass, s.count
+// and s.few are zero before and after.
+__device__ __forceinline__ unsigned long long select_rank(const Source& src, int lo, int hi, uint32_t want_count,
+                                                          unsigned long long want_mass, uint32_t count,
+                                                          unsigned long long& mass) {
     Last& s = src.s;
     const int t = static_cast<int>(threadIdx.x);
-    unsigned long long low = 0ull, span = 1ull << (32 + kRankBits);  // ranks [low, low + span) in parts of 2^shift
-    int shift = 32 + kRankBits - 11;
-    static_assert(kSub == 1 << 11, "11 bits a level");
+    const auto reached = [&](uint32_t cn, unsigned long long cm) { return cn >= want_count || cm >= want_mass; };
+    unsigned long long low = s.low, span = s.high - low + 1;
+    int shift = max(0, 64 - __builtin_clzll((span - 1) | 1ull) - kPartBits);
+#pragma unroll 1
     for (;;) {
-        for (int i = t; i < kSub; i += kLast) {
-            s.mass[i] = 0ull;
-            s.count[i] = 0u;
-        }
-        if (t == 0) {
-            s.few = 0u;
-            s.found_bin = 0;
-        }
-        __syncthreads();
-        src.each(lo, hi, [&](unsigned long long key, unsigned long long w) {
-            if (key >= low && key - low < span) {
-                const int at = static_cast<int>((key - low) >> shift);
-                atomicAdd(&s.mass[kSub - 1 - at], w);
-                atomicAdd(&s.count[kSub - 1 - at], 1u);
-            }
+        src.each(lo, hi, low, span, [&](unsigned long long key, unsigned long long w) {
+            const int at = kParts - 1 - static_cast<int>((key - low) >> shift);
+            atomicAdd(&s.mass[at], w);
+            atomicAdd(&s.count[at], 1u);
         });
         __syncthreads();
-        // two neighbouring parts a thread
-        const unsigned long long m0 = s.mass[2 * t], m1 = s.mass[2 * t + 1];
-        const uint32_t n0 = s.count[2 * t], n1 = s.count[2 * t + 1];
-        unsigned long long m = m0 + m1;
-        uint32_t n = n0 + n1;
-        block_scan(s, m, n);
-        m += mass;
-        n += count;
-        const auto reached = [&](uint32_t cn, unsigned long long cm) { return cn >= want_count || cm >= want_mass; };
-        const bool before = reached(n - n0 - n1, m - m0 - m1), after = reached(n, m);
-        if (!before && after) {
-            const bool first = reached(n - n1, m - m1);
-            s.found_bin = first ? 2 * t : 2 * t + 1;
-            s.found_mass = first ? m - m0 - m1 : m - m1;
-            s.wave_count[0] = first ? n - n0 - n1 : n - n1;
-        }
-        __syncthreads();
-        const int part = s.found_bin;
-        mass = s.found_mass;
-        count = s.wave_count[0];
-        const uint32_t held = s.count[part];
-        low += static_cast<unsigned long long>(kSub - 1 - part) << shift;
-        span = 1ull << shift;
-        if (held <= kWave || shift == 0) {
-            src.each(lo, hi, [&](unsigned long long key, unsigned long long w) {
-                if (key >= low && key - low < span) {
-                    const uint32_t i = atomicAdd(&s.few, 1u);
-                    s.key[i] = key;
-                    s.weight[i] = w;
-                }
-            });
-            __syncthreads();
-            if (t < kWave) {
-                const bool mine = t < static_cast<int>(held);
-                const unsigned long long key = mine ? s.key[t] : 0ull, w = mine ? s.weight[t] : 0ull;
-                uint32_t n = count + 1;
-                unsigned long long m = mass + w;
-                for (int i = 0; i < static_cast<int>(held); ++i) {
-                    const unsigned long long ko = s.key[i];
-                    if (ko > key) {
-                        ++n;
-                        m += s.weight[i];
-                    }
-                }
-                if (mine && reached(n, m) && !reached(n - 1, m - w)) {
-                    s.found = key;
-                    s.found_mass = m;
-                }
+        if (t < kWave) {
+            unsigned long long m[4], all = 0ull;
+            uint32_t n[4], held = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                all += m[i] = s.mass[4 * t + i];
+                held += n[i] = s.count[4 * t + i];
+                s.mass[4 * t + i] = 0ull;
+                s.count[4 * t + i] = 0u;
             }
-            __syncthreads();
-            mass = s.found_mass;
-            return s.found;
+            unsigned long long upto = mass + running_sum(all) - all;
+            uint32_t upto_n = count + running_sum(held) - held;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (!reached(upto_n, upto) && reached(upto_n + n[i], upto + m[i])) {
+                    s.found_part = 4 * t + i;
+                    s.found_mass = upto;
+                    s.found_count = upto_n;
+                    s.found_held = n[i];
+                }
+                upto += m[i];
+                upto_n += n[i];
+            }
         }
-        shift = shift > 11 ? shift - 11 : 0;
         __syncthreads();
+        const uint32_t held = s.found_held;
+        mass = s.found_mass;
+        count = s.found_count;
+        low += static_cast<unsigned long long>(kParts - 1 - s.found_part) << shift;
+        span = 1ull << shift;
+        if (held <= kWave || shift == 0) break;
+        shift = shift > kPartBits ? shift - kPartBits : 0;
     }
+    src.each(lo, hi, low, span, [&](unsigned long long key, unsigned long long w) {
+        const uint32_t i = atomicAdd(&s.few, 1u);
+        if (i < kWave) {
+            s.key[i] = key;
+            s.weight[i] = w;
+        }
+    });
+    __syncthreads();
+    if (t < kWave) {
+        const int held = static_cast<int>(min(s.few, 1u * kWave));
+        const bool mine = t < held;
+        const unsigned long long key = mine ? s.key[t] : 0ull, w = mine ? s.weight[t] : 0ull;
+        uint32_t n = count + 1;
+        unsigned long long m = mass + w;
+        for (int i = 0; i < held; ++i)
+            if (s.key[i] > key) {
+                ++n;
+                m += s.weight[i];
+            }
+        if (mine && reached(n, m) && !reached(n - 1, m - w)) {
+            s.found = key;
+            s.found_mass = m;
+        }
+        if (t == 0) s.few = 0u;
+    }
+    __syncthreads();
+    mass = s.found_mass;
+    return s.found;
 }
 
 template <bool kCuts>
 __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a) {
     __shared__ Last s;
     const int row = static_cast<int>(blockIdx.x), t = static_cast<int>(threadIdx.x);
-    const unsigned long long best = row_best(a, row);
-    const Scale scale(a, row, logit_of(best));
-    if (best == 0ull || scale.greedy) {
+    // every load whose place is known, before the first is waited for
+    const int lane = t % kWave;
+    const float u = a.uniform[row], p = a.top_p ? a.top_p[row] : 1.0f;
+    const uint32_t k = most_kept(a, row);
+    const uint32_t own = kCuts && lane < a.slices ? a.listed[static_cast<size_t>(row) * a.slices + lane] : 0u;
+    RowState r{};
+    if (kCuts) r = a.state[row];
+    const unsigned long long weight_here = t < a.tiles ? a.tile[static_cast<size_t>(row) * a.tiles + t] : 0ull;
+    const Ends ends = row_ends(a, row);
+    const Scale scale(a, row, ends);
+    if (ends.best == 0ull || scale.greedy) {
         if (t == 0) {
-            a.tokens[row] = best == 0ull ? -1 : static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-            a.probs[row] = best == 0ull ? 0.0f : 1.0f;
+            a.tokens[row] = ends.best == 0ull ? -1 : static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(ends.best));
+            a.probs[row] = ends.best == 0ull ? 0.0f : 1.0f;
         }
         return;
     }
     const unsigned long long least = least_weight(a, row);
-    const RowState r = a.state[row];
-    for (int i = t; i < a.tiles; i += kLast) s.tiles[i] = a.tile[static_cast<size_t>(row) * a.tiles + i];
+    s.tiles[t] = weight_here;
     unsigned long long cut = 0ull;  // the last kept rank
     if (kCuts && (r.bin_k < kBins || r.p_lo < kBins)) {
-        const uint32_t listed = a.listed[row];
-        const bool whole = listed > static_cast<uint32_t>(a.list_cap);
-        const Source src{a, r, scale, s, row, whole ? a.vocab : static_cast<int>(listed), whole};
-        if (!whole)
-            for (int i = t; i < src.n; i += kLast) s.list[i] = a.list[static_cast<size_t>(row) * a.list_cap + i];
-        __syncthreads();
-        unsigned long long total = r.total;
-        if (r.bin_k < kBins) {
-            total = r.base_k;
-            cut = select_rank(src, r.bin_k, r.bin_k, most_kept(a, row), ~0ull,
-                              static_cast<uint32_t>(r.count_k), total);
+        const uint32_t upto = running_sum(own);
+        const uint32_t listed = last_lane(upto);
+        const bool whole = listed > kListMost || __builtin_amdgcn_ballot_w64(own > kSliceMost) != 0ull;
+        const Source src{a, scale, s, row, whole ? a.vocab : static_cast<int>(listed), whole};
+        if (t < kParts) {
+            s.mass[t] = 0ull;
+            s.count[t] = 0u;
         }
-        if (r.p_lo < kBins) {
-            unsigned long long mass = r.base_p;
-            cut = select_rank(src, r.p_lo, r.p_hi, 0xFFFFFFFFu, share_of(a.top_p[row], total), 0u, mass);
+        if (t < kMaxSlices) s.upto[t] = upto;
+        if (t == 0) {
+            s.low = whole ? 0ull : ~0ull;
+            s.high = whole ? (1ull << (32 + kRankBits)) - 1 : 0ull;
+            s.few = 0u;
+            s.found_part = 0;
+            s.found_held = 0u;
+        }
+        __syncthreads();
+        if (!whole) {
+            unsigned long long low = ~0ull, high = 0ull;
+            // the slices' lists behind each other, an entry a thread
+#pragma unroll 1
+            for (uint32_t i = t; i < listed; i += kLast) {
+                int slice = 0;  // whose entries hold i
+#pragma unroll 1
+                for (int o = kMaxSlices / 2; o >= 1; o >>= 1)
+                    if (s.upto[slice + o - 1] <= i) slice += o;
+                const uint32_t first = slice > 0 ? s.upto[slice - 1] : 0u;
+                const uint2 e = a.list[(static_cast<size_t>(row) * a.slices + slice) * kSliceMost + (i - first)];
+                const float x = __builtin_bit_cast(float, e.x);
+                const double y = scale.log2w(x);
+                const unsigned long long key = rank_of(x, static_cast<int>(e.y));
+                s.rank[i] = key;
+                s.held[i] = Scale::weight(y) | (static_cast<unsigned long long>(scale.bin(y)) << kBinShift);
+                low = key < low ? key : low;
+                high = key > high ? key : high;
+            }
+            low = wave_min(low);
+            high = wave_max(high);
+            if (lane == 0 && high != 0ull) {
+                atomicMin(&s.low, low);
+                atomicMax(&s.high, high);
+            }
+            __syncthreads();
+        }
+        unsigned long long total = r.total;
+#pragma unroll 1
+        for (int by_p = 0; by_p < 2; ++by_p) {  // top-k, then top-p of what it leaves
+            const int lo = by_p ? r.p_lo : r.bin_k, hi = by_p ? r.p_hi : r.bin_k;
+            if (lo == kBins) continue;
+            unsigned long long mass = by_p ? r.base_p : r.base_k;
+            cut = select_rank(src, lo, hi, by_p ? 0xFFFFFFFFu : k, by_p ? share_of(p, total) : ~0ull,
+                              by_p ? 0u : r.count_k, mass);
+            total = mass;
         }
         // the kept ones of the cut's bins join their tiles
-        const int lo = min(r.p_lo, r.bin_k);
-        src.each(lo, kBins - 1, [&](unsigned long long key, unsigned long long w) {
-            if (key >= cut && w >= least)
-                atomicAdd(&s.tiles[(kMaxVocab - 1 - static_cast<int>(key & (kMaxVocab - 1))) / kTile], w);
+        src.each(min(r.p_lo, r.bin_k), kBins - 1, cut, ~0ull, [&](unsigned long long key, unsigned long long w) {
+            if (key >= cut && w >= least) atomicAdd(&s.tiles[token_of(key) / kTile], w);
         });
+        __syncthreads();
     }
-    __syncthreads();
-    // the tile that the random number falls into, a thread a run of tiles
-    const int per = (a.tiles + kLast - 1) / kLast;
-    unsigned long long m = 0ull;
-    uint32_t none = 0u;
-    for (int i = t * per; i < min(a.tiles, (t + 1) * per); ++i) m += s.tiles[i];
-    const unsigned long long own = m;
-    block_scan(s, m, none);
+    // the tile that the random number falls into
+    const unsigned long long here = s.tiles[t];
+    unsigned long long m = block_scan(s, here);
     if (t == kLast - 1) {
-        const float u = a.uniform[row];
         const double at = u > 0.0f ? static_cast<double>(u) * static_cast<double>(m) : 0.0;
         s.total = m;
         s.target = at < static_cast<double>(m) ? min(static_cast<unsigned long long>(at), m - 1) : m - 1;
     }
     __syncthreads();
     const unsigned long long target = s.target;
-    if (m > target && m - own <= target) {
-        unsigned long long before = m - own;
-        int i = t * per;
-        while (before + s.tiles[i] <= target) before += s.tiles[i++];
-        s.tile = i;
-        s.before = before;
+    if (m > target && m - here <= target) {
+        s.tile = t;
+        s.before = m - here;
     }
     __syncthreads();
-    // and its token, 4 of a lane of one wave
-    if (t >= kWave) return;
-    const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
-    unsigned long long w[4], sum = 0ull;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int v = s.tile * kTile + 4 * t + i;
-        const float q = v < a.vocab ? x[v] : -INFINITY;
-        const double y = scale.log2w(q);
-        w[i] = y > -kDepth ? Scale::weight(y) : 0ull;
-        if (w[i] < least || rank_of(q, v) < cut) w[i] = 0ull;
-        sum += w[i];
-    }
-    unsigned long long upto = sum;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const unsigned long long other = __shfl_up(upto, o, kWave);
-        if (t >= o) upto += other;
-    }
-    unsigned long long run = s.before + upto - sum;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (run <= target && run + w[i] > target) {
-            a.tokens[row] = s.tile * kTile + 4 * t + i;
-            a.probs[row] = static_cast<float>(static_cast<double>(w[i]) / static_cast<double>(s.total));
-        }
-        run += w[i];
+    // and its token
+    const int v = s.tile * kTile + t;
+    const float x = v < a.vocab ? a.logits[static_cast<size_t>(row) * a.vocab + v] : -INFINITY;
+    const double y = scale.log2w(x);
+    unsigned long long w = Scale::any(y) ? Scale::weight(y) : 0ull;
+    if (w < least || (kCuts && rank_of(x, v) < cut)) w = 0ull;
+    m = s.before + block_scan(s, w);
+    if (m > target && m - w <= target) {
+        a.tokens[row] = v;
+        a.probs[row] = static_cast<float>(static_cast<double>(w) / static_cast<double>(s.total));
     }
 }
 
 // ----------------------------------------------------------------------- host
 // Slices of a row: so many that the launch fills the chip, of whole steps.
 struct Plan {
-    int slices, slice, tiles, list_cap;
-    size_t best, mass, count, tile, state, listed, list, bytes;  // where each begins
+    int slices, slice, tiles;
+    size_t best, low, mass, count, tile, state, listed, list, bytes;  // where each begins
 };
 
 Plan plan_for(int n_rows, int vocab) {
     Plan p;
     const int steps = (vocab + kStep - 1) / kStep;
-    int want = (512 + n_rows - 1) / n_rows;
+    int want = (1024 + n_rows - 1) / n_rows;
     want = want < kMaxSlices ? want : kMaxSlices;
     const int per = (steps + want - 1) / want;
     p.slice = per * kStep;
     p.slices = (steps + per - 1) / per;
     p.tiles = (vocab + kTile - 1) / kTile;
-    p.list_cap = vocab < kListMost ? vocab : kListMost;
     size_t at = 0;
     auto place = [&](size_t& field, size_t bytes) {
         field = at;
@@ -613,12 +808,13 @@ Plan plan_for(int n_rows, int vocab) {
     };
     const size_t rows = static_cast<size_t>(n_rows), pieces = rows * p.slices;
     place(p.best, pieces * sizeof(unsigned long long));
+    place(p.low, pieces * sizeof(uint32_t));
     place(p.mass, pieces * kBins * sizeof(unsigned long long));
     place(p.count, pieces * kBins * sizeof(uint32_t));
     place(p.tile, rows * p.tiles * sizeof(unsigned long long));
     place(p.state, rows * sizeof(RowState));
-    place(p.listed, rows * sizeof(uint32_t));
-    place(p.list, rows * p.list_cap * sizeof(uint2));
+    place(p.listed, pieces * sizeof(uint32_t));
+    place(p.list, pieces * kSliceMost * sizeof(uint2));
     p.bytes = at;
     return p;
 }
@@ -651,26 +847,37 @@ extern "C" asdsl_status asdsl_sample_logits(const float* logits, const float* un
     char* at = static_cast<char*>(ws);
     const SampleArgs a{logits, uniform, temperature, top_k, top_p, min_p, tokens, probs,
                        reinterpret_cast<unsigned long long*>(at + p.best),
+                       reinterpret_cast<uint32_t*>(at + p.low),
                        reinterpret_cast<unsigned long long*>(at + p.mass),
                        reinterpret_cast<uint32_t*>(at + p.count),
                        reinterpret_cast<unsigned long long*>(at + p.tile),
                        reinterpret_cast<RowState*>(at + p.state),
                        reinterpret_cast<uint32_t*>(at + p.listed),
                        reinterpret_cast<uint2*>(at + p.list),
-                       vocab, p.slices, p.slice, p.tiles, p.list_cap};
+                       vocab, p.slices, p.slice, p.tiles};
     const bool vec = vocab % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0;
-    const bool cuts = top_k || top_p;
     const dim3 grid(static_cast<unsigned>(n_rows * p.slices)), block(kThreads);
     const hipStream_t hs = as_hip(stream);
-    st = launch("sample_best_kernel", vec ? sample_best_kernel<true> : sample_best_kernel<false>, grid, block, 0, hs, a);
-    if (st == ASDSL_OK && cuts)
-        st = launch("sample_bins_kernel", vec ? sample_bins_kernel<true> : sample_bins_kernel<false>, grid, block, 0, hs,
-                    a);
-    if (st == ASDSL_OK)
-        st = launch("sample_keep_kernel",
-                    cuts ? (vec ? sample_keep_kernel<true, true> : sample_keep_kernel<false, true>)
-                         : (vec ? sample_keep_kernel<true, false> : sample_keep_kernel<false, false>),
-                    grid, block, 0, hs, a);
+    const bool cuts = top_k || top_p;
+    auto with = [&](auto is_vec, auto count, auto mass, auto drops) {
+        constexpr bool kVec = decltype(is_vec)::value, kCount = decltype(count)::value, kMass = decltype(mass)::value;
+        asdsl_status res = launch("sample_best_kernel", sample_best_kernel<kVec>, grid, block, 0, hs, a);
+        if constexpr (kCount || kMass)
+            if (res == ASDSL_OK)
+                res = launch("sample_bins_kernel", sample_bins_kernel<kVec, kCount, kMass>, grid, block, 0, hs, a);
+        if (res != ASDSL_OK) return res;
+        return launch("sample_keep_kernel", sample_keep_kernel<kVec, kCount, kMass, decltype(drops)::value>, grid, block,
+                      0, hs, a);
+    };
+    const std::true_type yes{};
+    const std::false_type no{};
+    auto by_cuts = [&](auto is_vec) {
+        return top_k   ? top_p ? with(is_vec, yes, yes, yes) : with(is_vec, yes, no, yes)
+               : top_p ? with(is_vec, no, yes, yes)
+               : min_p ? with(is_vec, no, no, yes)
+                       : with(is_vec, no, no, no);
+    };
+    st = vec ? by_cuts(yes) : by_cuts(no);
     if (st != ASDSL_OK) return st;
     return launch("sample_token_kernel", cuts ? sample_token_kernel<true> : sample_token_kernel<false>, dim3(n_rows),
                   dim3(kLast), 0, hs, a);

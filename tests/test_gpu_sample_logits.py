@@ -153,6 +153,13 @@ def test_odd_values(gpu):
     check(x[2:7], u[2:7])
     nan = np.full(12, np.nan, np.float32)
     assert np.array_equal(run(x, u, top_p=nan, min_p=nan)[0], got)
+    # NaN beside a cut: of both signs, in rows whose first bin is cut
+    y = (np.arange(4 * 300).reshape(4, 300) % 7 * -1e-3).astype(np.float32)
+    y[:, 5::9], y[:, 6::9] = np.nan, -np.float32(np.nan)
+    y[1:, 7] = 2.0
+    cuts = {"top_k": np.array([100, 100, 3, 250], np.int32), "top_p": np.array([.5, .9, .3, 1], np.float32)}
+    for use in (("top_k",), ("top_p",), ("top_k", "top_p")):
+        check(y, u[:4], **{n: cuts[n] for n in use})
     for t in (0.0, -1.0, np.nan):  # the first of the ranking
         first = run(x, u, temperature=np.full(12, t, np.float32))
         assert first[0].tolist() == [-1, -1, 5, 33, 0, 7, 69, 0, 0, 0, 0, 0]
