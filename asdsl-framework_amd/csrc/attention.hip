@@ -740,6 +740,42 @@ struct Step {
         else
             v_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
     }
+    // 4-bit step t whose rows follow each other: one scalar address a tensor, one offset a
+    // lane, constants.
+    __device__ __forceinline__ void load_k4(const Keys& K, int t, int lane) {
+        const uint32_t r = lane & 15, gq = lane >> 4;
+        const size_t row = static_cast<size_t>(cache_row(K, t * kKeys));
+        const char* codes = static_cast<const char*>(K.k) + row * (D / 2);
+        const char* words = static_cast<const char*>(K.ks) + row * (D / 16);
+        const uint32_t at = r * (D / 2) + gq * (D / 8), word = r * (D / 16) + D / 4 * gq / kGroup4 * 2;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            if constexpr (D == 128) {
+                const uint4 c = *reinterpret_cast<const uint4*>(codes + at + 16 * kt * (D / 2));
+                k4[kt][0] = c.x; k4[kt][1] = c.y; k4[kt][2] = c.z; k4[kt][3] = c.w;
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2*>(codes + at + 16 * kt * (D / 2));
+                k4[kt][0] = c.x; k4[kt][1] = c.y;
+            }
+            kw[kt] = *reinterpret_cast<const uint16_t*>(words + word + 16 * kt * (D / 16));
+        }
+    }
+    __device__ __forceinline__ void load_v4(const Keys& K, int t, int lane) {
+        const uint32_t r = lane & 15, gq = lane >> 4;
+        const size_t row = static_cast<size_t>(cache_row(K, t * kKeys));
+        const char* codes = static_cast<const char*>(K.v) + row * (D / 2);
+        const char* words = static_cast<const char*>(K.vs) + row * (D / 16);
+        const uint32_t at = 4 * gq * (D / 2) + r * (D / 32), word = 4 * gq * (D / 16) + D / 16 * r / kGroup4 * 2;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int key = (i & 4) * 4 + (i & 3);
+            if constexpr (D == 128)
+                v.w[i] = *reinterpret_cast<const uint32_t*>(codes + at + key * (D / 2));
+            else
+                v.w[i] = *reinterpret_cast<const uint16_t*>(codes + at + key * (D / 2));
+            v.words[i] = *reinterpret_cast<const uint16_t*>(words + word + key * (D / 16));
+        }
+    }
     __device__ __forceinline__ half8 k_operand(int kt, int s) const {
         if constexpr (F == kI4)
             return codes4_half8(k4[kt][s], Step4(both4(kw[kt])));
@@ -789,13 +825,11 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, F == 
     if (t0 >= t1) return;
     const int gq = lane >> 4;
     Step<D, F> x;
-    x.load_k(K, t0, lane);
-    x.load_v(K, t0, lane);
-    for (int t = t0; t < t1; t += stride) {
+    // One step in x; after_k and after_v load what comes next as its registers get free.
+    const auto step = [&](int t, auto after_k, auto after_v) {
         float s[8];
         x.scores(q, s);
-        const int next = t + stride;
-        if (next < t1) x.load_k(K, next, lane);
+        after_k();
         const bool all = all_seen(K, t * kKeys, kKeys);  // the same in every lane
         uint32_t seen = 0xFFu;
         if (!all) seen = mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
@@ -806,7 +840,40 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, F == 
         w.cut(s, x.vs, all, seen, ev);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
-        if (next < t1) x.load_v(K, next, lane);
+        after_v();
+    };
+    if constexpr (F == kI4) {
+        // Steps whose rows follow each other, then the one or two that do not (at a range's
+        // end).  In one loop the compiler merges the loads of both kinds and forms 64-bit
+        // addresses for each, some 90 of 435 vector instructions, which this form is short of.
+        const auto following = [&](int t) {
+            while (t < t1 && !rows_follow(K, t * kKeys)) t += stride;
+            return t;
+        };
+        int t = following(t0);
+        if (t < t1) {
+            x.load_k4(K, t, lane);
+            x.load_v4(K, t, lane);
+        }
+        while (t < t1) {
+            const int next = following(t + stride), load = next < t1 ? next : t;
+            step(t, [&] { x.load_k4(K, load, lane); }, [&] { x.load_v4(K, load, lane); });
+            t = next;
+        }
+#pragma unroll 1
+        for (t = t0; t < t1; t += stride) {
+            if (rows_follow(K, t * kKeys)) continue;
+            x.load_k(K, t, lane);
+            x.load_v(K, t, lane);
+            step(t, [] {}, [] {});
+        }
+    } else {
+        x.load_k(K, t0, lane);
+        x.load_v(K, t0, lane);
+        for (int t = t0; t < t1; t += stride) {
+            const int next = t + stride;
+            step(t, [&] { if (next < t1) x.load_k(K, next, lane); }, [&] { if (next < t1) x.load_v(K, next, lane); });
+        }
     }
 }
 
@@ -1009,9 +1076,9 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
                 const int n1 = row0 + 4 * wave + i;
                 const long long at1 = map.at(n1);
                 strict_row<D, F>(K, g.q + at1 * D, g.scale, sight(K, p0 + n1 / map.g, rows, g.window), split * per,
-                              min(steps, (split + 1) * per), 1, lane,
-                              g.slots == 1 ? g.out + at1 * D : g.part + (at1 * g.slots + slot) * D,
-                              g.slots == 1 ? nullptr : g.ml + at1 * g.slots + slot);
+                                 min(steps, (split + 1) * per), 1, lane,
+                                 g.slots == 1 ? g.out + at1 * D : g.part + (at1 * g.slots + slot) * D,
+                                 g.slots == 1 ? nullptr : g.ml + at1 * g.slots + slot);
             }
             if (again) return;
         }
@@ -1121,32 +1188,62 @@ struct Bring {
     }
     // 4-bit codes: the key of which a lane brings dims D / 4 * (lane % 4) ..
     static __device__ __forceinline__ int k4_key(int wave, int lane) { return 16 * (wave - 2) + (lane >> 2); }
+    // Both ways end with w[0]: where they end with a store to the same array elsewhere,
+    // the compiler makes one store of the two, to an index in a register, keeps the
+    // array in memory for it and waits there for the load.
+    __device__ __forceinline__ void keep_k4(const char* codes, uint32_t word) {
+        static_assert(F == kI4, "codes and words");
+        w[8] = word;
+        if constexpr (D == 128) {
+            const uint4 c = *reinterpret_cast<const uint4*>(codes);
+            w[3] = c.w; w[2] = c.z; w[1] = c.y; w[0] = c.x;
+        } else {
+            const uint2 c = *reinterpret_cast<const uint2*>(codes);
+            w[1] = c.y; w[0] = c.x;
+        }
+    }
     template <typename At>
-    __device__ __forceinline__ void load4_rows(const Keys& K, size_t first, At at, int wave, int lane) {
+    __device__ __forceinline__ void load4_rows(const Keys& K, At at, int wave, int lane) {
         if (wave < 2) {
             if (wave < D / 64) {
                 const int d = 64 * wave + 4 * (lane & 15);
-                const char* src = static_cast<const char*>(K.v) + first * (D / 2) + d / 2;
-                const uint16_t* words = static_cast<const uint16_t*>(K.vs) + first * (D / kGroup4) + d / kGroup4;
+                const char* codes = static_cast<const char*>(K.v) + d / 2;
+                const uint16_t* words = static_cast<const uint16_t*>(K.vs) + d / kGroup4;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 7; i >= 0; --i) {
                     const auto key = at(v_key(i, lane >> 4));
-                    w[i] = *reinterpret_cast<const uint16_t*>(src + key * (D / 2));
                     w[8 + i] = words[key * (D / kGroup4)];
+                    w[i] = *reinterpret_cast<const uint16_t*>(codes + key * (D / 2));
                 }
             }
         } else {
             const auto key = at(k4_key(wave, lane));
-            const char* x = static_cast<const char*>(K.k) + first * (D / 2) + (key * (D / 2) + D / 8 * (lane & 3));
-            if constexpr (D == 128) {
-                const uint4 c = *reinterpret_cast<const uint4*>(x);
-                w[0] = c.x; w[1] = c.y; w[2] = c.z; w[3] = c.w;
-            } else {
-                const uint2 c = *reinterpret_cast<const uint2*>(x);
-                w[0] = c.x; w[1] = c.y;
+            const int part = lane & 3;
+            keep_k4(static_cast<const char*>(K.k) + key * (D / 2) + D / 8 * part,
+                    static_cast<const uint16_t*>(K.ks)[key * (D / kGroup4) + D / 4 * part / kGroup4]);
+        }
+    }
+    // The same where the rows follow each other from `row` on: one scalar address a
+    // tensor, one offset a lane, constants.
+    __device__ __forceinline__ void load4_following(const Keys& K, size_t row, int wave, int lane) {
+        if (wave < 2) {
+            if (wave < D / 64) {
+                const char* codes = static_cast<const char*>(K.v) + row * (D / 2);
+                const char* words = static_cast<const char*>(K.vs) + row * (D / 16);
+                const uint32_t d = 64 * wave + 4 * (lane & 15), key = v_key(0, lane >> 4);
+                const uint32_t at = key * (D / 2) + d / 2, word = key * (D / 16) + d / kGroup4 * 2;
+#pragma unroll
+                for (int i = 7; i >= 0; --i) {
+                    w[8 + i] = *reinterpret_cast<const uint16_t*>(words + word + v_key(i, 0) * (D / 16));
+                    w[i] = *reinterpret_cast<const uint16_t*>(codes + at + v_key(i, 0) * (D / 2));
+                }
             }
-            w[8] = static_cast<const uint16_t*>(K.ks)[first * (D / kGroup4) + key * (D / kGroup4) +
-                                                      D / 4 * (lane & 3) / kGroup4];
+        } else {
+            const uint32_t key = k4_key(wave, lane), part = lane & 3;
+            const char* codes = static_cast<const char*>(K.k) + row * (D / 2);
+            const char* words = static_cast<const char*>(K.ks) + row * (D / 16);
+            keep_k4(codes + (key * (D / 2) + part * (D / 8)),
+                    *reinterpret_cast<const uint16_t*>(words + (key * (D / 16) + D / 4 * part / kGroup4 * 2)));
         }
     }
     __device__ __forceinline__ void store4(Stage<D, false>& s, int wave, int lane) {
@@ -1175,10 +1272,6 @@ struct Bring {
     // Key i's row is at(i) rows past `first`.
     template <typename At>
     __device__ __forceinline__ void load_rows(const Keys& K, size_t first, At at, int wave, int lane) {
-        if constexpr (F == kI4) {
-            load4_rows(K, first, at, wave, lane);
-            return;
-        }
         constexpr int kBytes = Q8 ? 1 : 2;
         if (wave < 2) {
             if (wave < D / 64) {
@@ -1228,16 +1321,27 @@ struct Bring {
     // constants; at a range's end every row is looked up by itself.
     __device__ __forceinline__ void load(const Keys& K, int t, int wave, int lane) {
         const int i0 = t * kKeys;
-        if (rows_follow(K, i0))
-            load_rows(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, wave, lane);
-        else
-            load_rows(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, wave, lane);
+        const bool follow = rows_follow(K, i0);
+        const auto row = [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); };
+        if constexpr (F == kI4) {
+            if (follow)
+                load4_following(K, static_cast<size_t>(cache_row(K, i0)), wave, lane);
+            else
+                load4_rows(K, row, wave, lane);
+        } else {
+            if (follow)
+                load_rows(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, wave, lane);
+            else
+                load_rows(K, 0, row, wave, lane);
+        }
     }
     __device__ __forceinline__ void store(Stage<D, Q8>& s, int wave, int lane) {
-        if constexpr (F == kI4) {
+        if constexpr (F == kI4)
             store4(s, wave, lane);
-            return;
-        }
+        else
+            store_rows(s, wave, lane);
+    }
+    __device__ __forceinline__ void store_rows(Stage<D, Q8>& s, int wave, int lane) {
         if (wave < 2) {
             if (wave < D / 64) {
                 const int q = lane >> 4;
@@ -1725,6 +1829,18 @@ long long fill_many(long long jobs, long long rows, long long heads, long long n
     return rows * splits * 4 <= heads * n ? kFillFew : kFillFew / 2;
 }
 
+// Over 4-bit keys three workgroups fit a compute unit, and ragged sequences fare better
+// in more pieces, as long as these are long.  us with 512 / 768 / 1024 / 2048
+// workgroups, 24 heads of 128, 8 KV heads, caches of 16384: 32 sequences of up to
+// 16000 rows 111 / 97 / 89 / 89, all of 16000 143 / 137 / 137 / 136, of 4100 43 / 40 /
+// 46 / 48; 8 of up to 8000 23.4 / 23.9 / 26.0 / 28.0.  Equal shares of all keys for every
+// workgroup, whatever the sequences' ends, was no better: 83 / 90 / 89 and 28 / 34 / 35.
+int splits_four(long long jobs, long long n) {
+    const int most = splits_for(1024, jobs, n, kMaxSlots), least = splits_for(768, jobs, n, kMaxSlots);
+    const long long whole = n / 2048;
+    return whole < least ? least : whole < most ? static_cast<int>(whole) : most;
+}
+
 // Values of a KV head's keys that few rows take in one piece: a second launch
 // for the join costs more than the pieces save.  us a call in a graph (queued
 // one by one), whole / in pieces of 128 keys, 8 KV heads of 128 dims: 200 keys
@@ -1772,6 +1888,8 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, K
     p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
     if (!p.many && n * head_dim <= kAlone)
         p.splits = 1;
+    else if (!p.many && form == kI4)
+        p.splits = splits_four(p.jobs, n);
     else
         p.splits = splits_for(p.many ? fill_many(p.jobs, p.rows, static_cast<long long>(n_seq) * n_kv, n, head_dim)
                                      : kFillFew,

@@ -22,12 +22,19 @@ struct Step4 {
     half2_4 scale, zero;  // zero: 1024 + z
     __device__ __forceinline__ explicit Step4(uint32_t words)
         : scale(__builtin_bit_cast(half2_4, words & 0xFFF0FFF0u)),
-          zero(__builtin_bit_cast(half2_4, (words & 0x000F000Fu) | 0x64006400u)) {}
+          zero(__builtin_bit_cast(half2_4, with_1024(words))) {}
     // The codes at bits 4 * i .. and 16 + 4 * i .. of w: 0x6400 | c is 1024 + c, the
     // difference is exact, and so is the product.
     __device__ __forceinline__ uint32_t values(uint32_t w, int i) const {
-        const half2_4 c = __builtin_bit_cast(half2_4, ((w >> (4 * i)) & 0x000F000Fu) | 0x64006400u);
-        return __builtin_bit_cast(uint32_t, (c - zero) * scale);
+        return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(half2_4, with_1024(w >> (4 * i))) - zero) * scale);
+    }
+    // The low 4 bits of both halves of w as fp16 numbers 1024 + c.  One instruction, which
+    // takes one constant from a scalar register and the other from a vector one; left
+    // to itself the compiler takes two with a literal each.
+    static __device__ __forceinline__ uint32_t with_1024(uint32_t w) {
+        uint32_t r;
+        asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(w), "s"(0x000F000Fu), "v"(0x64006400u));
+        return r;
     }
 };
 
