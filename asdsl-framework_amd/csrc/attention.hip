@@ -1801,12 +1801,23 @@ int splits_for(long long fill, long long jobs, long long n, int most) {
 //                  25.6 / 72.9, p 8192 x 2048 82 / 107, p 16384 x 4096 269 / 235
 // One rule by steps does not fit all: 4 s 4096 rows of 64 dims over int8 caches with
 // a window of 256 take 74 in the form for few, 54 in the other.
-bool takes_many(long long total, long long heads, long long keys, int head_dim, Kv form) {
+//
+// 4-bit keys (`seen`: every row sees all of them, a prefix) are turned into fp16 in
+// both forms, once per 16 rows or once per 128; the few bytes leave the form for few
+// rows ahead for longer, with one rule for both head dims, by steps less four of the
+// others.  us few / many, 24 heads, 8 KV heads, 128 dims (64 dims):
+//   p 1024 x 1024 39 / 51 (26 / 37), p 1500 x 1500 65 / 76 (44 / 53), p 1024 x 2048
+//   75 / 71 (50 / 49), p 2048 x 2048 104 / 100 (69 / 68), p 1024 x 3000 113 / 95
+//   (76 / 68), with a window of 256 p 4096 85 / 59 (55 / 34)
+//   prefix of 16000: 144 rows 48 / 57 (34 / 38), 384 rows 114 / 91 (79 / 52); of 16384
+//   and 192 rows 67 / 64, 256 rows of 64 dims 47 / 41; of 8000 and 192 rows 38 / 38
+bool takes_many(long long total, long long heads, long long keys, int head_dim, Kv form, bool seen) {
     const bool q8 = form == kI8;
     if (total <= kRows) return false;
     const int wide = kManyWaves * kWideRows;
     const long long pieces = heads * ((keys + kLeastKeys - 1) / kLeastKeys);
     const long long few = (total + kRows - 1) / kRows * pieces, many = (total + wide - 1) / wide * pieces;
+    if (form == kI4) return few - 4 * many > (seen ? 2000 : 8500);
     const int worth = head_dim == 128 ? (q8 ? 3 : 2) : (q8 ? 5 : 3);
     const int margin = head_dim == 128 ? (q8 ? 1900 : 300) : (q8 ? 40000 : 3900);
     return few - worth * many > margin;
@@ -1883,7 +1894,7 @@ Plan plan_window(int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, K
         const long long near = static_cast<long long>(window) + sinks + kManyWaves * kWideRows / (n_heads / n_kv);
         keys = near < keys ? near : keys;
     }
-    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, keys, head_dim, form);
+    p.many = takes_many(total, static_cast<long long>(n_seq) * n_kv, keys, head_dim, form, false);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.jobs = n_seq * ((total + p.wg_rows - 1) / p.wg_rows) * n_kv;
     if (!p.many && n * head_dim <= kAlone)
@@ -1904,7 +1915,7 @@ Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, Kv form, int pr
     p.rows = static_cast<size_t>(n_seq) * n_heads;
     const int group = n_heads / n_kv;
     const long long total = static_cast<long long>(n_seq) * group;
-    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, form);
+    p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, form, true);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
     const int own_splits = splits_for(kFillFew, p.own_jobs, own_rows, kMaxSlots / 4);
