@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "device_common.hpp"
+
 namespace asdsl {
 
 constexpr int kGroup4 = 32;  // dims per scale word
@@ -68,8 +70,20 @@ __device__ __forceinline__ double scale4(double range) {
     return fmax(ceil(q * 0x1p20), 1.0) * 0x1p-20;
 }
 
+// The value of another lane of the same 8: lane ^ 1, lane ^ 2, the mirrored one.
+template <int CTRL>
+__device__ __forceinline__ double moved8(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, 0xF, 0xF, false);
+    return __builtin_bit_cast(double, (static_cast<uint64_t>(hi) << 32) | lo);
+}
+
 // Four neighbouring dims of a lane, a group's 32 in 8 neighbouring lanes, all of
-// them here: the lane's codes (16 bits) and the group's word.
+// them here: the lane's codes (16 bits) and the group's word.  A quotient is formed
+// in fp32, within 2^-18 of itself, and in fp64 only where that leaves its rounding
+// open, some 4 in 10^5; with fp64 divisions throughout an append of 2045 tokens (8
+// KV heads of 128) took 2 us more.
 __device__ __forceinline__ uint32_t quantize4(const double (&x)[4], uint32_t& word) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const bool bad = !(isfinite(x[0]) && isfinite(x[1]) && isfinite(x[2]) && isfinite(x[3]));
@@ -81,21 +95,29 @@ __device__ __forceinline__ uint32_t quantize4(const double (&x)[4], uint32_t& wo
         lo = fmin(lo, y[i]);
         hi = fmax(hi, y[i]);
     }
-#pragma unroll
-    for (int o = 4; o >= 1; o >>= 1) {
-        lo = fmin(lo, __shfl_xor(lo, o, 64));
-        hi = fmax(hi, __shfl_xor(hi, o, 64));
-    }
+    lo = fmin(lo, moved8<kDppQuadXor1>(lo));
+    hi = fmax(hi, moved8<kDppQuadXor1>(hi));
+    lo = fmin(lo, moved8<kDppQuadXor2>(lo));
+    hi = fmax(hi, moved8<kDppQuadXor2>(hi));
+    lo = fmin(lo, moved8<kDppRowHalfMirror>(lo));
+    hi = fmax(hi, moved8<kDppRowHalfMirror>(hi));
     if (((any >> (lane & 56)) & 0xFFull) != 0ull) {
         word = kNaN4;
         return 0u;
     }
     const double scale = scale4(hi - lo);
-    const double zero = rint(-lo / scale);
+    const float inv = 1.0f / static_cast<float>(scale);  // the scale is an fp32 number
+    const auto rounded = [&](double v) {
+        const float t = static_cast<float>(v) * inv;  // |t| < 17: off by less than 2^-18
+        float r = __builtin_rintf(t);
+        if (fabsf(fabsf(t - r) - 0.5f) < 0x1p-16f) r = static_cast<float>(rint(v / scale));
+        return r;
+    };
+    const float zero = rounded(-lo);
     uint32_t codes = 0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        codes |= static_cast<uint32_t>(fmin(fmax(rint(y[i] / scale) + zero, 0.0), 15.0)) << (4 * i);
+        codes |= static_cast<uint32_t>(fminf(fmaxf(rounded(y[i]) + zero, 0.0f), 15.0f)) << (4 * i);
     const _Float16 h = static_cast<_Float16>(static_cast<float>(scale));  // exactly
     word = __builtin_bit_cast(uint16_t, h) | static_cast<uint32_t>(zero);
     return codes;

@@ -254,3 +254,72 @@ def test_more_than_2_31_logits(gpu):
     want, share, room = reference(x[at].cpu().numpy(), u[at].cpu().numpy(), top_p=p[at].cpu().numpy())
     assert (room > vocab * 2.0 ** -42).all() and np.array_equal(tokens[at].cpu().numpy(), want)
     assert np.allclose(probs[at].cpu().numpy(), share, rtol=2.0 ** -23)
+
+
+def test_a_chat_over_4_bits_drawn_token_by_token(gpu):
+    """A step as a program runs it: new rows into a 4-bit cache, attention over it, logits, a mask and penalties, the
+    token drawn; captured twice and replayed in turn, against eager steps, and each token against its logits in 64 bits."""
+    import torch
+
+    from asdsl.kernels import attention_window, control_logits, kv_append, sample_logits
+
+    rng = np.random.default_rng(11)
+    n, h, kvh, d, rows, vocab, steps = 3, 8, 2, 64, 40, 5003, 7
+    width = (h + 2 * kvh) * d
+    embed = dev(rng.standard_normal((vocab, width)).astype(np.float32))
+    head = dev((rng.standard_normal((h * d, vocab)) / 8).astype(np.float32))
+    angle = np.arange(rows)[:, None] * 100.0 ** (-np.arange(16) / 16)
+    cos, sin = dev(np.cos(angle).astype(np.float32)), dev(np.sin(angle).astype(np.float32))
+    may = rng.random((n, (vocab + 31) // 32 * 32)) < 0.8
+    words = dev(np.packbits(may, axis=1, bitorder="little").view(np.int32))
+    kw = {"temperature": dev(np.array([.8, 1.0, .5], np.float32)), "top_k": dev(np.array([40, 0, 500], np.int32)),
+          "top_p": dev(np.array([.95, .9, 1], np.float32)), "min_p": dev(np.array([0, .01, .001], np.float32))}
+    uniform = dev(rng.random((steps, n), dtype=np.float32))
+    penalty = torch.full((n,), 1.2, device="cuda")
+
+    def chat():
+        return {"k": torch.zeros((n, kvh, rows, d // 2), dtype=torch.uint8, device="cuda"),
+                "ks": torch.zeros((n, kvh, rows, d // 32), dtype=torch.int16, device="cuda"),
+                "v": torch.zeros((n, kvh, rows, d // 2), dtype=torch.uint8, device="cuda"),
+                "vs": torch.zeros((n, kvh, rows, d // 32), dtype=torch.int16, device="cuda"),
+                "pos": torch.zeros(n, dtype=torch.int32, device="cuda"),
+                "tokens": torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda"),
+                "history": torch.full((n, steps + 1), -1, dtype=torch.int32, device="cuda")}
+
+    def step(c, u):
+        q = kv_append(embed[c["tokens"].long()], c["k"], c["v"], cos, sin, c["pos"], n_heads=h, k_scale=c["ks"],
+                      v_scale=c["vs"])
+        out = attention_window(q, c["k"], c["v"], c["pos"], n_heads=h, k_scale=c["ks"], v_scale=c["vs"])
+        y, _ = control_logits(torch.mm(out, head), history=c["history"], repetition=penalty, allowed=words, pick=False)
+        tokens, probs = sample_logits(y, u, **kw)
+        c["history"].scatter_(1, c["pos"].long()[:, None], tokens[:, None])
+        c["tokens"].copy_(tokens)
+        c["pos"].add_(1)
+        return y, tokens, probs
+
+    eager, other = chat(), chat()
+    u = torch.empty(n, device="cuda")
+    spare = chat()
+    graphs = []
+    for _ in range(2):
+        step(spare, u.zero_())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(other, u)
+        graphs.append((g, out))
+    for name, t in chat().items():
+        other[name].copy_(t)
+    for i in range(steps):
+        want = step(eager, uniform[i])
+        u.copy_(uniform[i])
+        graphs[i % 2][0].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, graphs[i % 2][1]):
+            assert torch.equal(a, b)
+        assert all(torch.equal(eager[name], other[name]) for name in eager)
+        token, share, room = reference(want[0].cpu().numpy(), uniform[i].cpu().numpy(),
+                                       **{name: t.cpu().numpy() for name, t in kw.items()})
+        sure = room > vocab * 2.0 ** -42
+        assert sure.any() and np.array_equal(want[1].cpu().numpy()[sure], token[sure])
+        assert may[np.arange(n), want[1].cpu().numpy()].all()
