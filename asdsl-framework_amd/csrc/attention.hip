@@ -223,6 +223,7 @@ struct AttnArgs {
     int window, sinks;
     int splits, slots;  // key splits of this launch's jobs, partials kept per row
     float scale;        // log2(e) / sqrt(D)
+    bool longest_first; // workgroups take the sequences in order of their positions
 };
 
 // f over the lanes that hold one row: lane % kStep is the same (16: four lanes,
@@ -819,17 +820,19 @@ struct Step {
 };
 
 template <int D, int F>
-__device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, F == kI4>& q, const RowSight& see, int t0,
-                                         int t1, int stride, int lane, State<D, F == kI8>& st) {
+__device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, false>& q, const RowSight& see, int t0, int t1,
+                                         int stride, int lane, State<D, F == kI8>& st) {
     constexpr bool Q8 = F == kI8;
     if (t0 >= t1) return;
     const int gq = lane >> 4;
     Step<D, F> x;
-    // One step in x; after_k and after_v load what comes next as its registers get free.
-    const auto step = [&](int t, auto after_k, auto after_v) {
+    x.load_k(K, t0, lane);
+    x.load_v(K, t0, lane);
+    for (int t = t0; t < t1; t += stride) {
         float s[8];
         x.scores(q, s);
-        after_k();
+        const int next = t + stride;
+        if (next < t1) x.load_k(K, next, lane);
         const bool all = all_seen(K, t * kKeys, kKeys);  // the same in every lane
         uint32_t seen = 0xFFu;
         if (!all) seen = mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
@@ -840,40 +843,58 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, F == 
         w.cut(s, x.vs, all, seen, ev);
 #pragma unroll
         for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
+        if (next < t1) x.load_v(K, next, lane);
+    }
+}
+
+// The same over 4-bit keys, as their fp16 values.  Bound by vector instructions and
+// memory about alike: of some 380 a step 230 turn 32 rows of K and V into fp16 (an
+// and-or, a subtraction and a product for two values, a shift for three in four), so
+// what else there is counts.  Steps whose rows follow each other are taken first,
+// then the one or two that do not (at a range's end): in one loop the compiler merges
+// the loads of both kinds and forms 64-bit addresses for each, 90 instructions more.
+// A whole step loaded ahead leaves two waves a SIMD instead of three and is slower.
+// 32 sequences of 16000 rows (24 heads of 128, 8 KV heads, 590 MB) take 136 us, 4.3
+// TB/s, ragged ones of up to 16000 (281 MB) 71; fp16 caches, 3.6 times the bytes, 276.
+template <int D>
+__device__ __forceinline__ void few_rows4(const Keys& K, const Query<D, 32, true>& q, const RowSight& see, int t0, int t1,
+                                          int stride, int lane, State<D, false>& st) {
+    const int gq = lane >> 4;
+    Step<D, kI4> x;
+    // One step in x; after_k and after_v load what comes next as its registers get free.
+    const auto step = [&](int t, auto after_k, auto after_v) {
+        float s[8];
+        x.scores(q, s);
+        after_k();
+        if (!all_seen(K, t * kKeys, kKeys))
+            mask_keys<8>(K, see, s, [&](int i) { return t * kKeys + (i & 4) * 4 + 4 * gq + (i & 3); });
+        st.step(s, q.c, x.vs);
+        Weights<D, false> w;
+        w.cut(s, x.vs, true, 0u, 0);
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) st.acc[j] = w.add(x.v.operand(j), j >> 2, st.acc[j]);
         after_v();
     };
-    if constexpr (F == kI4) {
-        // Steps whose rows follow each other, then the one or two that do not (at a range's
-        // end).  In one loop the compiler merges the loads of both kinds and forms 64-bit
-        // addresses for each, some 90 of 435 vector instructions, which this form is short of.
-        const auto following = [&](int t) {
-            while (t < t1 && !rows_follow(K, t * kKeys)) t += stride;
-            return t;
-        };
-        int t = following(t0);
-        if (t < t1) {
-            x.load_k4(K, t, lane);
-            x.load_v4(K, t, lane);
-        }
-        while (t < t1) {
-            const int next = following(t + stride), load = next < t1 ? next : t;
-            step(t, [&] { x.load_k4(K, load, lane); }, [&] { x.load_v4(K, load, lane); });
-            t = next;
-        }
+    const auto following = [&](int t) {
+        while (t < t1 && !rows_follow(K, t * kKeys)) t += stride;
+        return t;
+    };
+    int t = following(t0);
+    if (t < t1) {
+        x.load_k4(K, t, lane);
+        x.load_v4(K, t, lane);
+    }
+    while (t < t1) {
+        const int next = following(t + stride), load = next < t1 ? next : t;
+        step(t, [&] { x.load_k4(K, load, lane); }, [&] { x.load_v4(K, load, lane); });
+        t = next;
+    }
 #pragma unroll 1
-        for (t = t0; t < t1; t += stride) {
-            if (rows_follow(K, t * kKeys)) continue;
-            x.load_k(K, t, lane);
-            x.load_v(K, t, lane);
-            step(t, [] {}, [] {});
-        }
-    } else {
-        x.load_k(K, t0, lane);
-        x.load_v(K, t0, lane);
-        for (int t = t0; t < t1; t += stride) {
-            const int next = t + stride;
-            step(t, [&] { if (next < t1) x.load_k(K, next, lane); }, [&] { if (next < t1) x.load_v(K, next, lane); });
-        }
+    for (t = t0; t < t1; t += stride) {
+        if (rows_follow(K, t * kKeys)) continue;
+        x.load_k(K, t, lane);
+        x.load_v(K, t, lane);
+        step(t, [] {}, [] {});
     }
 }
 
@@ -1036,7 +1057,11 @@ __device__ __forceinline__ void few_job(const AttnArgs& g, const Keys& K, const 
     const int steps = (K.n + kKeys - 1) / kKeys;
     // a split's steps, a multiple of the waves'
     const int per = ((steps + splits - 1) / splits + kFewWaves - 1) / kFewWaves * kFewWaves;
-    few_rows<D, F>(K, q, see, split * per + wave, min(steps, (split + 1) * per), kFewWaves, lane, st);
+    const int t0 = split * per + wave, t1 = min(steps, (split + 1) * per);
+    if constexpr (F == kI4)
+        few_rows4<D>(K, q, see, t0, t1, kFewWaves, lane, st);
+    else
+        few_rows<D, F>(K, q, see, t0, t1, kFewWaves, lane, st);
     st.l = lanes_sum<16>(st.l);
     store_row<D, Q8>(area.acc[wave][lane & 15], st, gq);
     if (gq == 0) area.ml[wave][lane & 15] = make_float2(st.m, st.l);
@@ -1588,6 +1613,27 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const A
 }
 
 // ------------------------------------------------------- few rows: kernels
+// The sequence of the place-th largest position, by its 8 leading bits of a cache's
+// rows and then by index; for up to 64 sequences.  Bit by bit, those that have it
+// before those that have not: scalar work, a quarter of what ranking every lane takes.
+constexpr int kOrdered = kWave;
+__device__ __forceinline__ int sequence_at(const AttnArgs& g, int place) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int p = lane < g.n_seq ? min(max(g.pos[lane], 0), g.rows_b - 1) : 0;
+    const int key = p >> max(0, 24 - __builtin_clz(g.rows_b));
+    uint64_t left = g.n_seq < kWave ? (1ull << g.n_seq) - 1 : ~0ull;
+#pragma unroll
+    for (int bit = 7; bit >= 0; --bit) {
+        const uint64_t ones = __builtin_amdgcn_ballot_w64((key >> bit) & 1) & left;
+        const int n = __builtin_popcountll(ones);
+        left = place < n ? ones : left & ~ones;
+        place = place < n ? place : place - n;
+    }
+    const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(left >> 32),
+                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(left), 0u));
+    return uniform(__builtin_ctzll(__builtin_amdgcn_ballot_w64(before == place) & left));
+}
+
 // blockIdx.x = ((sequence * row tiles + tile) * splits + split) * n_kv + kv head:
 // with 8 KV heads one head's workgroups share an XCD's L2.
 template <int D, int F>
@@ -1602,7 +1648,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void window_few_kernel(const Att
     const int split = b % g.splits;
     b /= g.splits;
     const int row0 = b % tiles * kRows;
-    const int seq = b / tiles;
+    const int seq = F == kI4 && g.longest_first ? sequence_at(g, b / tiles) : b / tiles;
     const RowMap map{static_cast<long long>(seq) * g.n_tokens * g.n_heads + static_cast<long long>(kvh) * group, group,
                      g.n_heads, total};
     const Keys K = window_keys<D, F>(g, seq, kvh, row0 / group, (min(row0 + kRows, total) - 1) / group + 1);
@@ -1979,6 +2025,9 @@ asdsl_status window(const char* what, Kv form, const float* q, const Cache& c, c
     AttnArgs g{q, out, nullptr, nullptr, c, c, pos, n_seq, n_tokens, n_heads, n_kv_heads, rows, rows, -1, window,
                sinks, p.splits, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
+    // Where the workgroups come one after the other, ragged sequences take 12 to 15 % less
+    // with the longest first: 32 of up to 16000 rows 82 -> 71 us, 64 of up to 4000 48 -> 41.
+    g.longest_first = form == kI4 && n_seq > 1 && n_seq <= kOrdered && p.jobs > kFillFew;
     const dim3 grid(static_cast<unsigned>(p.jobs));
     auto with = [&](auto dim, auto codes) {
         constexpr int kD = decltype(dim)::value, kF = decltype(codes)::value;

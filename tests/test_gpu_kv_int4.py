@@ -162,6 +162,25 @@ def test_window(gpu, case):
     assert np.array_equal(again.cpu().numpy().reshape(q.shape), got.cpu().numpy())
 
 
+@pytest.mark.parametrize("n,kvh,d,rows,win", [(40, 16, 128, 700, 0), (64, 16, 64, 1100, 200), (65, 16, 64, 1100, 0),
+                                              (2, 300, 64, 530, 0)])
+def test_window_of_many_ragged_sequences(gpu, n, kvh, d, rows, win):
+    """More workgroups than run at once, which take the longest sequences first; equal positions, padded sequences."""
+    from asdsl.kernels import attention_window
+
+    rng = np.random.default_rng(n)
+    pos = rng.integers(-1, rows, n)
+    pos[rng.integers(0, n, n // 3)] = rows - 1
+    pos[1] = rows  # outside
+    q = rng.standard_normal((n, 1, kvh, d)).astype(np.float32)
+    k, ks, kw = cache4(rng, n, kvh, rows, d)
+    v, vs, vw = cache4(rng, n, kvh, rows, d)
+    want, bound = ref.window(q, kw, vw, pos, win, 2 if win else 0)
+    got = attention_window(dev(q), k, v, dev(pos.astype(np.int32)), window=win, sinks=2 if win else 0, k_scale=ks,
+                           v_scale=vs)
+    check(got, want, bound)
+
+
 @pytest.mark.parametrize("case", [c[:4] + c[5:] for c in PREFIX], ids=lambda c: str(c[:7]))
 def test_prefix(gpu, case):
     from asdsl.kernels import attention_prefix
