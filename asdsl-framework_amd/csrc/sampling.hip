@@ -624,33 +624,66 @@ __device__ __forceinline__ unsigned long long block_scan(Last& s, unsigned long 
     return m;
 }
 
-// The tokens that a cut may fall on: the list, or where it did not hold them all the row.
+// The tokens that a cut may fall on: the list, or where it did not hold them all the
+// row.
 struct Source {
     const SampleArgs& a;
     const Scale& scale;
     Last& s;
     int row, n;
     bool whole;
-    // f(rank, weight) for those of bins [lo, hi] with ranks [low, low + span)
-    template <typename F>
+
+    // f(rank, weight, is it one) for the tokens of bins [lo, hi] with ranks [low, low +
+    // span), by whole waves that hold any.  kRanksOnly: whatever their bins, no weights.
+    template <bool kRanksOnly, typename F>
     __device__ __forceinline__ void each(int lo, int hi, unsigned long long low, unsigned long long span, F f) const {
         const int t = static_cast<int>(threadIdx.x);
-        if (whole) {
-            const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
-#pragma unroll 4
-            for (int i = t; i < n; i += kLast) {
-                const float q = x[i];
-                const unsigned long long key = rank_of(q, i);
-                const double y = scale.log2w(q);
-                if (key - low >= span || !Scale::any(y)) continue;
-                const int b = scale.bin(y);
-                if (b >= lo && b <= hi) f(key, Scale::weight(y));
-            }
-        } else {
-            for (int i = t; i < n; i += kLast) {
-                const unsigned long long w = s.held[i], key = s.rank[i];
+        if (!whole) {
+#pragma unroll 1
+            for (int i = t; i - t % kWave < n; i += kLast) {
+                const unsigned long long w = i < n ? s.held[i] : 0ull, key = i < n ? s.rank[i] : 0ull;
                 const int b = static_cast<int>(w >> kBinShift);
-                if (key - low < span && b >= lo && b <= hi) f(key, w & ((1ull << kBinShift) - 1));
+                const bool mine = i < n && b >= lo && b <= hi && key - low < span;
+                if (__builtin_amdgcn_ballot_w64(mine) != 0ull) f(key, w & ((1ull << kBinShift) - 1), mine);
+            }
+            return;
+        }
+        // A comparison of floats first, and of one logit's equals only those in range: a
+        // vector instruction a token is 1.3 us of a row of 200064 by one workgroup.
+        const uint32_t o0 = static_cast<uint32_t>(low >> kRankBits);
+        const uint32_t o1 = min(static_cast<uint32_t>((low + span - 1) >> kRankBits), order_of(INFINITY));
+        const float x0 = logit_of(o0), x1 = logit_of(o1);
+        const int v0 = o0 == o1 ? token_of(low + span - 1) & ~3 : 0, v1 = o0 == o1 ? min(n, token_of(low) + 1) : n;
+        // four neighbouring tokens a thread, the next four on their way
+        const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
+        const auto load = [&](int v) {
+            return make_float4(v < v1 ? x[v] : -INFINITY, v + 1 < v1 ? x[v + 1] : -INFINITY,
+                               v + 2 < v1 ? x[v + 2] : -INFINITY, v + 3 < v1 ? x[v + 3] : -INFINITY);
+        };
+        float4 next = load(v0 + 4 * t);
+#pragma unroll 1
+        for (int v = v0 + 4 * t; v - 4 * (t % kWave) < v1; v += 4 * kLast) {
+            float4 q = next;
+            next = load(v + 4 * kLast);
+            const bool none = !((q.x >= x0 && q.x <= x1) || (q.y >= x0 && q.y <= x1) || (q.z >= x0 && q.z <= x1) ||
+                                (q.w >= x0 && q.w <= x1));
+            if (__builtin_amdgcn_ballot_w64(!none) == 0ull) continue;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+                const float z = q.x;
+                q = make_float4(q.y, q.z, q.w, 0.0f);
+                const unsigned long long key = rank_of(z, v + j);
+                bool mine = z >= x0 && z <= x1 && key - low < span;
+                if (__builtin_amdgcn_ballot_w64(mine) == 0ull) continue;
+                unsigned long long w = 0ull;
+                if constexpr (!kRanksOnly) {
+                    const double y = scale.log2w(z);
+                    const int b = scale.bin(y);
+                    mine = mine && Scale::any(y) && b >= lo && b <= hi;
+                    if (__builtin_amdgcn_ballot_w64(mine) == 0ull) continue;
+                    w = Scale::weight_or_none(y);
+                }
+                f(key, w, mine);
             }
         }
     }
@@ -666,16 +699,27 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
                                                           unsigned long long want_mass, uint32_t count,
                                                           unsigned long long& mass) {
     Last& s = src.s;
-    const int t = static_cast<int>(threadIdx.x);
+    const int t = static_cast<int>(threadIdx.x), lane = t % kWave;
     const auto reached = [&](uint32_t cn, unsigned long long cm) { return cn >= want_count || cm >= want_mass; };
     unsigned long long low = s.low, span = s.high - low + 1;
     int shift = max(0, 64 - __builtin_clzll((span - 1) | 1ull) - kPartBits);
 #pragma unroll 1
     for (;;) {
-        src.each(lo, hi, low, span, [&](unsigned long long key, unsigned long long w) {
+        src.each<false>(lo, hi, low, span, [&](unsigned long long key, unsigned long long w, bool mine) {
             const int at = kParts - 1 - static_cast<int>((key - low) >> shift);
-            atomicAdd(&s.mass[at], w);
-            atomicAdd(&s.count[at], 1u);
+            // equal logits lie in one part, lane by lane: their sum goes there as one
+            const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
+            const int first = __builtin_ctzll(all), there = __builtin_amdgcn_readlane(at, first);
+            if (__builtin_amdgcn_ballot_w64(mine && at == there) == all) {
+                const unsigned long long sum = wave_sum(mine ? w : 0ull);
+                if (lane == first) {
+                    atomicAdd(&s.mass[there], sum);
+                    atomicAdd(&s.count[there], static_cast<uint32_t>(__builtin_popcountll(all)));
+                }
+            } else if (mine) {
+                atomicAdd(&s.mass[at], w);
+                atomicAdd(&s.count[at], 1u);
+            }
         });
         __syncthreads();
         if (t < kWave) {
@@ -711,7 +755,8 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
         if (held <= kWave || shift == 0) break;
         shift = shift > kPartBits ? shift - kPartBits : 0;
     }
-    src.each(lo, hi, low, span, [&](unsigned long long key, unsigned long long w) {
+    src.each<false>(lo, hi, low, span, [&](unsigned long long key, unsigned long long w, bool mine) {
+        if (!mine) return;
         const uint32_t i = atomicAdd(&s.few, 1u);
         if (i < kWave) {
             s.key[i] = key;
@@ -776,53 +821,81 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
         }
         if (t < kMaxSlices) s.upto[t] = upto;
         if (t == 0) {
-            s.low = whole ? 0ull : ~0ull;
-            s.high = whole ? (1ull << (32 + kRankBits)) - 1 : 0ull;
+            s.low = ~0ull;
+            s.high = 0ull;
             s.few = 0u;
             s.found_part = 0;
             s.found_held = 0u;
         }
         __syncthreads();
         if (!whole) {
-            unsigned long long low = ~0ull, high = 0ull;
             // the slices' lists behind each other, an entry a thread
-#pragma unroll 1
             for (uint32_t i = t; i < listed; i += kLast) {
                 int slice = 0;  // whose entries hold i
-#pragma unroll 1
+#pragma unroll
                 for (int o = kMaxSlices / 2; o >= 1; o >>= 1)
                     if (s.upto[slice + o - 1] <= i) slice += o;
                 const uint32_t first = slice > 0 ? s.upto[slice - 1] : 0u;
                 const uint2 e = a.list[(static_cast<size_t>(row) * a.slices + slice) * kSliceMost + (i - first)];
                 const float x = __builtin_bit_cast(float, e.x);
                 const double y = scale.log2w(x);
-                const unsigned long long key = rank_of(x, static_cast<int>(e.y));
-                s.rank[i] = key;
+                s.rank[i] = rank_of(x, static_cast<int>(e.y));
                 s.held[i] = Scale::weight(y) | (static_cast<unsigned long long>(scale.bin(y)) << kBinShift);
-                low = key < low ? key : low;
-                high = key > high ? key : high;
-            }
-            low = wave_min(low);
-            high = wave_max(high);
-            if (lane == 0 && high != 0ull) {
-                atomicMin(&s.low, low);
-                atomicMax(&s.high, high);
             }
             __syncthreads();
         }
+        // The range of their ranks: by the ends of the bins and of the row, some 2^-22 wider
+        // than the bins; of a whole row, where levels are dear, then by its tokens in it.
+        const int lo = min(r.p_lo, r.bin_k), hi = max(r.p_lo < kBins ? r.p_hi : 0, r.bin_k < kBins ? r.bin_k : 0);
+        const float top = logit_of(static_cast<uint32_t>(ends.best >> 32)), least_logit = logit_of(ends.low);
+        float x0 = least_logit, x1 = top;
+        if (scale.per_bin > 0.0) {
+            const double wide = 1.0 / (scale.per_bin * scale.c), e0 = scale.m - (hi + 1) * wide, e1 = scale.m - (lo - 1) * wide;
+            const double more = fabs(scale.m) * 0x1p-22 + 0x1p-140;
+            x0 = fmaxf(static_cast<float>(e0 - fabs(e0) * 0x1p-22 - more), x0);
+            x1 = fminf(static_cast<float>(e1 + fabs(e1) * 0x1p-22 + more), x1);
+        }
+        unsigned long long low = static_cast<unsigned long long>(order_of(x0)) << kRankBits;
+        unsigned long long high = (static_cast<unsigned long long>(order_of(x1)) << kRankBits) | (kMaxVocab - 1);
+        if (whole && x0 != x1) {
+            const unsigned long long from = low, span = high - low + 1;
+            low = ~0ull;
+            high = 0ull;
+            src.each<true>(lo, hi, from, span, [&](unsigned long long key, unsigned long long, bool mine) {
+                low = mine && key < low ? key : low;
+                high = mine && key > high ? key : high;
+            });
+            low = wave_min(low);
+            high = wave_max(high);
+        }
+        if (lane == 0 && high != 0ull) {
+            atomicMin(&s.low, low);
+            atomicMax(&s.high, high);
+        }
+        __syncthreads();
         unsigned long long total = r.total;
 #pragma unroll 1
         for (int by_p = 0; by_p < 2; ++by_p) {  // top-k, then top-p of what it leaves
-            const int lo = by_p ? r.p_lo : r.bin_k, hi = by_p ? r.p_hi : r.bin_k;
-            if (lo == kBins) continue;
+            const int from = by_p ? r.p_lo : r.bin_k, upto = by_p ? r.p_hi : r.bin_k;
+            if (from == kBins) continue;
             unsigned long long mass = by_p ? r.base_p : r.base_k;
-            cut = select_rank(src, lo, hi, by_p ? 0xFFFFFFFFu : k, by_p ? share_of(p, total) : ~0ull,
+            cut = select_rank(src, from, upto, by_p ? 0xFFFFFFFFu : k, by_p ? share_of(p, total) : ~0ull,
                               by_p ? 0u : r.count_k, mass);
             total = mass;
         }
         // the kept ones of the cut's bins join their tiles
-        src.each(min(r.p_lo, r.bin_k), kBins - 1, cut, ~0ull, [&](unsigned long long key, unsigned long long w) {
-            if (key >= cut && w >= least) atomicAdd(&s.tiles[token_of(key) / kTile], w);
+        src.each<false>(lo, kBins - 1, cut, (1ull << (32 + kRankBits)) - cut, [&](unsigned long long key, unsigned long long w, bool mine) {
+            const bool keep = mine && w >= least;
+            const int tile = token_of(key) / kTile;
+            const uint64_t all = __builtin_amdgcn_ballot_w64(keep);
+            if (all == 0ull) return;
+            const int first = __builtin_ctzll(all), there = __builtin_amdgcn_readlane(tile, first);
+            if (__builtin_amdgcn_ballot_w64(keep && tile == there) == all) {
+                const unsigned long long sum = wave_sum(keep ? w : 0ull);
+                if (lane == first) atomicAdd(&s.tiles[there], sum);
+            } else if (keep) {
+                atomicAdd(&s.tiles[tile], w);
+            }
         });
         __syncthreads();
     }
@@ -855,6 +928,11 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
 }
 
 // ----------------------------------------------------------------------- host
+// Tiles of a slice at most, so that the tokens of the bin that a cut runs through,
+// some 1.4 % of a row of normally distributed logits whatever their spread, stay
+// within the slice's list: without a list the token's workgroup looks the row through.
+constexpr int kSliceTiles = 48;
+
 // Slices of a row: so many that the launch fills the chip, of whole steps.
 struct Plan {
     int slices, slice, tiles;
@@ -865,7 +943,7 @@ Plan plan_for(int n_rows, int vocab) {
     Plan p;
     p.tiles = (vocab + kTile - 1) / kTile;
     const int want = std::min((1024 + n_rows - 1) / n_rows, kMaxSlices);
-    const int per = (p.tiles + want - 1) / want;
+    const int per = std::min((p.tiles + want - 1) / want, kSliceTiles);
     p.slice = per * kTile;
     p.slices = (p.tiles + per - 1) / per;
     size_t at = 0;

@@ -119,6 +119,22 @@ def test_flat_and_tied_logits(gpu, vocab):
             assert (got[0] == 1).all() and (got[1] == 0.5).all()
 
 
+@pytest.mark.parametrize("vocab", [70001, 200064])
+def test_a_far_logit_leaves_the_others_in_one_bin(gpu, vocab):
+    """Bins reach from the largest logit to the smallest: one far below makes them wide, and more tokens of different
+    logits lie in the cut's bin than its lists hold."""
+    rng = np.random.default_rng(vocab)
+    rows = 6
+    x = (rng.standard_normal((rows, vocab)) * np.array([.02, .1, .3, .02, .1, .3])[:, None]).astype(np.float32)
+    x[:, 17] = -500.0
+    x[3:, 5] = 3.0
+    kw = {"top_k": rng.integers(1, vocab, rows).astype(np.int32), "top_p": rng.uniform(0.05, 1, rows).astype(np.float32),
+          "min_p": np.array([0, .8, .3, 0, .04, .04], np.float32)}
+    u = rng.random(rows, dtype=np.float32)
+    for use in (("top_k",), ("top_p",), ("top_k", "top_p"), ("top_p", "min_p"), tuple(kw)):
+        check(x, u, **{n: kw[n] for n in use})
+
+
 def test_every_kept_token_by_its_share(gpu):
     """u over a grid draws each kept token as often as its share, in index order, and no other."""
     rng = np.random.default_rng(1)
