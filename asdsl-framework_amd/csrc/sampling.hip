@@ -14,6 +14,7 @@
 // (full rate here): 2^-43 a weight, against some 2^-24 in fp32, which over a flat
 // vocabulary of 200000 would move the token in some of every thousand draws.
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 #include "abi_util.hpp"
@@ -52,7 +53,7 @@ struct SampleArgs {
     int* tokens;
     float* probs;
     unsigned long long* best;  // [rows][slices] largest logit and its first token
-    uint32_t* low;             // [rows][slices] smallest logit above -inf
+    uint32_t* low;             // [rows][slices] a small logit that may have a weight
     unsigned long long* mass;  // [rows][slices][kBins]
     uint32_t* count;           // [rows][slices][kBins]
     unsigned long long* tile;  // [rows][tiles]
@@ -75,8 +76,13 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 // What a row's slices found.
 struct Ends {
     unsigned long long best;  // order_of the largest logit, and below it ~ its first token; 0: nothing to draw from
-    uint32_t low;             // order_of the smallest logit above -inf
+    uint32_t low;             // order_of the logit at which the last bin ends, or of a smaller one
 };
+
+// Logits so far below another have no weight.
+__device__ __forceinline__ float reach_of(const SampleArgs& a, int row) {
+    return static_cast<float>(kDepth / kLog2eWide) * (a.temperature ? a.temperature[row] : 1.0f);
+}
 
 // A row's weights.  Every kernel forms them with the same roundings (none is
 // contracted), so that what one counts is what the next one finds.
@@ -132,9 +138,9 @@ struct Scale {
         return any(y) ? w : 0ull;
     }
     // 0 .. kBins - 1, rising as weights fall, where any(y); the sum with 2^52 rounds to a
-    // whole number
+    // whole number.  The last bin takes in all that is smaller.
     __device__ __forceinline__ int bin(double y) const {
-        return static_cast<int>(__builtin_bit_cast(uint64_t, fma(y, -per_bin, 0x1p52)));
+        return min(static_cast<int>(__builtin_bit_cast(uint64_t, fma(y, -per_bin, 0x1p52))), kBins - 1);
     }
 };
 
@@ -260,37 +266,47 @@ struct Stream {
 };
 
 // ------------------------------------------------------------- largest logit
-template <bool kVec>
+// And, for the bins, the smallest of those that may have a weight beside it, about:
+// logits of -10000 for tokens that do not exist or are not allowed would leave the
+// others few bins.  A lane forgets a small one when one out of its reach comes, lanes
+// and slices out of the largest one's reach do not count.
+//
+// Bound by memory: 64 rows of 200064 (51 MB) 10.8 us, 4.7 TB/s; one row 3.6.
+template <bool kVec, bool kLow>
 __global__ __launch_bounds__(kThreads) void sample_best_kernel(const SampleArgs a) {
     __shared__ unsigned long long red[kThreads / kWave];
     __shared__ uint32_t lows[kThreads / kWave];
     const int row = static_cast<int>(blockIdx.x) / a.slices, slice = static_cast<int>(blockIdx.x) % a.slices;
-    unsigned long long best = 0ull;
-    uint32_t low = 0xFFFFFFFFu;
+    const float reach = reach_of(a, row);
+    float top = -INFINITY, low = INFINITY, from = INFINITY;  // from: the smallest in reach
+    int token = 0;
     Stream<kVec, false>(a, row, slice).each([&](int v, const float (&x)[4]) {
+        const float most = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));  // of numbers, whatever NaN are beside them
+        if (most > top) {
+            top = most;
+            token = v + (x[0] == most ? 0 : x[1] == most ? 1 : x[2] == most ? 2 : 3);
+            from = fmaxf(top - reach, -FLT_MAX);
+            if (low < from) low = top;
+        }
+        if constexpr (kLow) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (x[i] > -INFINITY) {
-                const uint32_t o = order_of(x[i]);
-                const unsigned long long key = (static_cast<unsigned long long>(o) << 32) | (0xFFFFFFFFu - v - i);
-                best = key > best ? key : best;
-                low = min(low, o);
-            }
+            for (int i = 0; i < 4; ++i) low = fminf(low, x[i] >= from ? x[i] : INFINITY);
+        }
     }, [](int) {});
+    unsigned long long best =
+        top > -INFINITY ? (static_cast<unsigned long long>(order_of(top)) << 32) | (0xFFFFFFFFu - token) : 0ull;
     best = wave_max(best);
-    low = wave_min(low);
-    if (threadIdx.x % kWave == 0) {
-        red[threadIdx.x / kWave] = best;
-        lows[threadIdx.x / kWave] = low;
-    }
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / kWave; ++i) best = red[i] > best ? red[i] : best;
+    const float most = logit_of(static_cast<uint32_t>(best >> 32));
+    const uint32_t mine = wave_min(best != 0ull && low < INFINITY && !(low < most - reach) ? order_of(low) : 0xFFFFFFFFu);
+    if (threadIdx.x % kWave == 0) lows[threadIdx.x / kWave] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kThreads / kWave; ++i) {
-            best = red[i] > best ? red[i] : best;
-            low = min(low, lows[i]);
-        }
         a.best[blockIdx.x] = best;
-        a.low[blockIdx.x] = low;
+        a.low[blockIdx.x] = min(min(lows[0], lows[1]), min(lows[2], lows[3]));
     }
 }
 
@@ -302,12 +318,18 @@ __device__ __forceinline__ Ends row_ends(const SampleArgs& a, int row) {
     Ends e{0ull, 0xFFFFFFFFu};
     if (lane < a.slices) e = Ends{a.best[at], a.low[at]};
     e.best = wave_max(e.best);
-    e.low = wave_min(e.low);
+    const float most = logit_of(static_cast<uint32_t>(e.best >> 32));
+    const bool near = e.low != 0xFFFFFFFFu && !(logit_of(e.low) < most - reach_of(a, row));
+    e.low = min(wave_min(near ? e.low : 0xFFFFFFFFu), static_cast<uint32_t>(e.best >> 32));
     return e;
 }
 
 // ------------------------------------------------------- weights by their size
-// kCount, kMass: what the cuts that the call asks for need (top-k, top-p).
+// kCount, kMass: what the cuts that the call asks for need (top-k, top-p).  Bound by
+// the weights, some 25 instructions in fp64 each, and their sums in LDS: 64 rows of
+// 200064 with top-p 22.6 us (19.0 go to the weights alone), with top-k, which asks for
+// none, 12.3; one row with both 6.1.  kCopies: of the bins, for the lanes in turn, so
+// that fewer of a wave's meet in one (24.7 us with one).
 constexpr int kCopies = 4;
 template <bool kVec, bool kCount, bool kMass>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a) {
@@ -468,7 +490,10 @@ struct Queue {
 
 // kCount, kMass: top-k or top-p may cut; kLeast: min_p may drop tokens.  Without
 // any a token goes straight to its weight, else those that a comparison of floats
-// cannot rule out go through a queue, so that the others cost no fp64 work.
+// cannot rule out go through a queue, so that the others cost no fp64 work.  64 rows
+// of 200064 take 19.0 us without cuts, with top-p of 0.5 / 0.9 / 0.999 18.7 / 23.8 /
+// 33.1, of which the row's bins, summed by every workgroup for itself, are some 5; one
+// row 8.3 with every filter.
 template <bool kVec, bool kCount, bool kMass, bool kLeast>
 __global__ __launch_bounds__(kThreads) void sample_keep_kernel(const SampleArgs a) {
     constexpr bool kCuts = kCount || kMass, kDirect = !kCuts && !kLeast;
@@ -508,7 +533,7 @@ __global__ __launch_bounds__(kThreads) void sample_keep_kernel(const SampleArgs 
     const int before = min(r.p_lo, r.bin_k);
     const int last = before == kBins ? kBins - 1 : max(r.p_lo < kBins ? r.p_hi : -1, r.bin_k < kBins ? r.bin_k : -1);
     // No logit below `from` is in them: the bin's end, or min_p where nothing cuts, some 2^-22 lower.
-    double reach = s.per_bin > 0.0 ? (last + 1) / s.per_bin : kDepth;
+    double reach = s.per_bin > 0.0 && last < kBins - 1 ? (last + 1) / s.per_bin : kDepth;
     if (before == kBins && least > 1ull) reach = fmin(reach, 43.0 - log2(static_cast<double>(least)));
     const double edge = s.m - (reach + 0x1p-20) / s.c;
     const float from = s.infinite ? INFINITY
@@ -786,6 +811,11 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
     return s.found;
 }
 
+// One workgroup a row.  A chain of loads (the slices' ends, their lists, the token's
+// tile), scans and barriers: 4.0 us without cuts, 9.5 with both, for one row as for 64.
+// Where the lists did not hold the cut's bins it goes through the row for each level of
+// a selection, at some 60 to 130 us a pass over 200064: equal logits throughout take
+// 300 to 400 us.
 template <bool kCuts>
 __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a) {
     __shared__ Last s;
@@ -844,20 +874,20 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
             }
             __syncthreads();
         }
-        // The range of their ranks: by the ends of the bins and of the row, some 2^-22 wider
-        // than the bins; of a whole row, where levels are dear, then by its tokens in it.
+        // The range of their ranks: by the ends of the bins, some 2^-22 wider; of the last bin
+        // and of a whole row, where levels are dear, by the tokens.
         const int lo = min(r.p_lo, r.bin_k), hi = max(r.p_lo < kBins ? r.p_hi : 0, r.bin_k < kBins ? r.bin_k : 0);
-        const float top = logit_of(static_cast<uint32_t>(ends.best >> 32)), least_logit = logit_of(ends.low);
-        float x0 = least_logit, x1 = top;
+        const float top = logit_of(static_cast<uint32_t>(ends.best >> 32));
+        float x0 = -FLT_MAX, x1 = top;
         if (scale.per_bin > 0.0) {
             const double wide = 1.0 / (scale.per_bin * scale.c), e0 = scale.m - (hi + 1) * wide, e1 = scale.m - (lo - 1) * wide;
             const double more = fabs(scale.m) * 0x1p-22 + 0x1p-140;
-            x0 = fmaxf(static_cast<float>(e0 - fabs(e0) * 0x1p-22 - more), x0);
+            if (hi < kBins - 1) x0 = fmaxf(static_cast<float>(e0 - fabs(e0) * 0x1p-22 - more), x0);
             x1 = fminf(static_cast<float>(e1 + fabs(e1) * 0x1p-22 + more), x1);
         }
         unsigned long long low = static_cast<unsigned long long>(order_of(x0)) << kRankBits;
         unsigned long long high = (static_cast<unsigned long long>(order_of(x1)) << kRankBits) | (kMaxVocab - 1);
-        if (whole && x0 != x1) {
+        if (whole || x0 == -FLT_MAX) {
             const unsigned long long from = low, span = high - low + 1;
             low = ~0ull;
             high = 0ull;
@@ -1006,7 +1036,7 @@ extern "C" asdsl_status asdsl_sample_logits(const float* logits, const float* un
     const bool cuts = top_k || top_p;
     auto with = [&](auto is_vec, auto count, auto mass, auto drops) {
         constexpr bool kVec = decltype(is_vec)::value, kCount = decltype(count)::value, kMass = decltype(mass)::value;
-        asdsl_status res = launch("sample_best_kernel", sample_best_kernel<kVec>, grid, block, 0, hs, a);
+        asdsl_status res = launch("sample_best_kernel", sample_best_kernel<kVec, kCount || kMass>, grid, block, 0, hs, a);
         if constexpr (kCount || kMass)
             if (res == ASDSL_OK)
                 res = launch("sample_bins_kernel", sample_bins_kernel<kVec, kCount, kMass>, grid, block, 0, hs, a);

@@ -121,18 +121,34 @@ def test_flat_and_tied_logits(gpu, vocab):
 
 @pytest.mark.parametrize("vocab", [70001, 200064])
 def test_a_far_logit_leaves_the_others_in_one_bin(gpu, vocab):
-    """Bins reach from the largest logit to the smallest: one far below makes them wide, and more tokens of different
-    logits lie in the cut's bin than its lists hold."""
+    """Bins reach from the largest logit to the smallest: one below the others makes them wide, and more tokens of
+    different logits lie in the cut's bin than its lists hold."""
     rng = np.random.default_rng(vocab)
     rows = 6
     x = (rng.standard_normal((rows, vocab)) * np.array([.02, .1, .3, .02, .1, .3])[:, None]).astype(np.float32)
-    x[:, 17] = -500.0
+    x[:, 17] = -5.0
     x[3:, 5] = 3.0
     kw = {"top_k": rng.integers(1, vocab, rows).astype(np.int32), "top_p": rng.uniform(0.05, 1, rows).astype(np.float32),
           "min_p": np.array([0, .8, .3, 0, .04, .04], np.float32)}
     u = rng.random(rows, dtype=np.float32)
     for use in (("top_k",), ("top_p",), ("top_k", "top_p"), ("top_p", "min_p"), tuple(kw)):
         check(x, u, **{n: kw[n] for n in use})
+
+
+def test_logits_for_tokens_that_do_not_exist(gpu):
+    """-10000 for many tokens, a far one, and cuts that fall among the smallest that have a weight."""
+    rng = np.random.default_rng(4)
+    rows, vocab = 8, 40000
+    x = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    x[:, 33000:] = -10000.0
+    x[1::2, rng.permutation(vocab)[:30000]] = -65504.0
+    x[2, 77] = -31.0 + x[2].max()  # nearly no weight
+    x[3, 0] = -1e30
+    for t, p in ((1.0, .999999), (.5, .9), (2.0, .95), (30.0, .99), (1e4, .5), (1e-3, .9)):
+        check(x, rng.random(rows, dtype=np.float32), temperature=np.full(rows, t, np.float32),
+              top_p=np.full(rows, p, np.float32))
+        check(x, rng.random(rows, dtype=np.float32), temperature=np.full(rows, t, np.float32),
+              top_k=np.array([5, 100, 9000, 3, 32999, 33001, 39999, 1], np.int32))
 
 
 def test_every_kept_token_by_its_share(gpu):
