@@ -10,9 +10,9 @@
 // their sum.
 //
 // Where a running sum stands beside uniform * total, or beside top_p * total, the
-// last bits of the weights decide a whole number, so exponents are formed in fp64
-// (full rate here): 2^-43 a weight, against some 2^-24 in fp32, which over a flat
-// vocabulary of 200000 would move the token in some of every thousand draws.
+// last bits of the weights decide a whole number, so they are formed in fp64: 2^-43
+// a weight, against some 2^-24 in fp32, which over a flat vocabulary of 200000 would
+// move the token in some of every thousand draws.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -326,24 +326,18 @@ __device__ __forceinline__ Ends row_ends(const SampleArgs& a, int row) {
 
 // ------------------------------------------------------- weights by their size
 // kCount, kMass: what the cuts that the call asks for need (top-k, top-p).  Bound by
-// the weights, some 25 instructions in fp64 each, and their sums in LDS: 64 rows of
-// 200064 with top-p 22.6 us (19.0 go to the weights alone), with top-k, which asks for
-// none, 12.3; one row with both 6.1.  kCopies: of the bins, for the lanes in turn, so
-// that fewer of a wave's meet in one (24.7 us with one).
-constexpr int kCopies = 4;
+// the weights, some 25 instructions in fp64 each: 64 rows of 200064 with top-p 21.6 us
+// (19.0 go to the weights' sum alone), with top-k, which asks for none, 11.3; one row
+// with both 6.1.
 template <bool kVec, bool kCount, bool kMass>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a) {
-    __shared__ unsigned long long mass[kCopies][kBins];
-    __shared__ uint32_t count[kCopies][kBins];
+    __shared__ unsigned long long mass[kBins];
+    __shared__ uint32_t count[kBins];
     const int row = static_cast<int>(blockIdx.x) / a.slices, slice = static_cast<int>(blockIdx.x) % a.slices;
     Stream<kVec, false> in(a, row, slice);
     static_assert(kBins == kThreads, "a thread a bin");
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-        mass[i][threadIdx.x] = 0ull;
-        count[i][threadIdx.x] = 0u;
-    }
-    const int copy = static_cast<int>(threadIdx.x) % kCopies;
+    mass[threadIdx.x] = 0ull;
+    count[threadIdx.x] = 0u;
     const Ends ends = row_ends(a, row);
     const Scale s(a, row, ends);
     if (ends.best == 0ull || s.greedy) return;
@@ -357,26 +351,19 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
             const double y = s.log2w(x[i]);
             any[i] = Scale::any(y);
             b[i] = s.bin(y);
-            if constexpr (kMass) w[i] = Scale::weight_or_none(y);
+            if constexpr (kMass) w[i] = Scale::weight(y);  // of any(y) only is used
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (!any[i]) continue;
-            if constexpr (kMass) atomicAdd(&mass[copy][b[i]], w[i]);
-            if constexpr (kCount) atomicAdd(&count[copy][b[i]], 1u);
+            if constexpr (kMass) atomicAdd(&mass[b[i]], w[i]);
+            if constexpr (kCount) atomicAdd(&count[b[i]], 1u);
         }
     }, [](int) {});
     __syncthreads();
     const size_t at = static_cast<size_t>(blockIdx.x) * kBins + threadIdx.x;
-    unsigned long long m = 0ull;
-    uint32_t n = 0u;
-#pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-        m += mass[i][threadIdx.x];
-        n += count[i][threadIdx.x];
-    }
-    if constexpr (kMass) a.mass[at] = m;
-    if constexpr (kCount) a.count[at] = n;
+    if constexpr (kMass) a.mass[at] = mass[threadIdx.x];
+    if constexpr (kCount) a.count[at] = count[threadIdx.x];
 }
 
 // --------------------------------------------- kept weights, and the cut's bins
