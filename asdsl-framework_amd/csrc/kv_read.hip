@@ -108,6 +108,7 @@ asdsl_status read_rows(const char* what, bool four, const void* k, const void* v
     const long long chunks = (static_cast<long long>(n_rows) + per - 1) / per, heads = static_cast<long long>(n_seq) * n_kv_heads;
     ASDSL_CHECK_ARG(heads <= (1LL << 31) && fits_launch(2 * heads * chunks, kReadThreads),
                     "%s: too many rows: more than 2^32 work items", what);
+    ASDSL_CHECK_ARG(k_out != v_out, "%s: keys and values need an output each", what);
     const ReadArgs a{{k, v}, {ks, vs}, {k_out, v_out}, pos, n_kv_heads, rows, n_rows, static_cast<int>(chunks)};
     auto with = [&](auto dim, auto is_four) {
         constexpr int kD = decltype(dim)::value;

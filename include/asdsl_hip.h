@@ -685,7 +685,8 @@ asdsl_status asdsl_kv_append_q4(const float* qkv, uint8_t* k_cache, uint8_t* v_c
  * every KV head of sequence s (pos null: from row 0) to k_out and v_out
  * [n_seq][n_kv_heads][n_rows][head_dim], fp32 or (out_fp32 0) fp16: int8 codes
  * times their scale in fp32, rounded once more to fp16; 4-bit values exactly.
- * Rows outside [0, rows) read as zero.  Caches and outputs 16-byte aligned. */
+ * Rows outside [0, rows) read as zero.  Caches and outputs 16-byte aligned; the
+ * outputs must overlap neither each other nor the caches. */
 asdsl_status asdsl_kv_read_q8(const int8_t* k_cache, const int8_t* v_cache, const float* k_scale, const float* v_scale,
                               const int* pos, void* k_out, void* v_out, int out_fp32, int n_seq, int n_kv_heads,
                               int head_dim, int rows, int n_rows, asdsl_stream_t stream);

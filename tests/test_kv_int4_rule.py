@@ -75,6 +75,15 @@ def test_read_refusals():
             refused(f(dims=dims), text)
 
 
+def test_read_refuses_one_output_for_keys_and_values():
+    from asdsl import _hip
+
+    lib = _hip.LIB
+    for read in (lib.asdsl_kv_read_q8, lib.asdsl_kv_read_q4):
+        for out_fp32 in (0, 1):
+            refused(read(*(ONE,) * 7, out_fp32, 2, 4, 128, 64, 10, None), "an output each")
+
+
 def test_wrappers_refuse_what_does_not_fit():
     import torch
 
