@@ -48,7 +48,7 @@ struct Cache {
 // copy of 1 GiB gets 5.15) and in 14.8 where the last call's are; into int8 caches
 // 18.8 and 15.1.  A head per workgroup of scalar lanes took 47.  16 tokens take 3.0
 // us (int8 3.1), of which the launch and one chain of loads (position, then
-// tables) are nearly all.
+// tables) are nearly all.  Into 4-bit caches 2045 tokens take 18.6 us and 16 take 3.6.
 struct AppendArgs {
     const float* qkv;
     void* k;
@@ -854,8 +854,8 @@ __device__ __forceinline__ void few_rows(const Keys& K, const Query<D, 32, false
 // then the one or two that do not (at a range's end): in one loop the compiler merges
 // the loads of both kinds and forms 64-bit addresses for each, 90 instructions more.
 // A whole step loaded ahead leaves two waves a SIMD instead of three and is slower.
-// 32 sequences of 16000 rows (24 heads of 128, 8 KV heads, 590 MB) take 136 us, 4.3
-// TB/s, ragged ones of up to 16000 (281 MB) 71; fp16 caches, 3.6 times the bytes, 276.
+// 32 sequences of 16000 rows (24 heads of 128, 8 KV heads, 590 MB) take 146 us, 4.0
+// TB/s, ragged ones of up to 16000 72; fp16 caches, 3.6 times the bytes, 344 and 245.
 template <int D>
 __device__ __forceinline__ void few_rows4(const Keys& K, const Query<D, 32, true>& q, const RowSight& see, int t0, int t1,
                                           int stride, int lane, State<D, false>& st) {
@@ -1174,7 +1174,9 @@ __device__ __forceinline__ Keys window_keys(const AttnArgs& g, int seq, int kvh,
 // run, without the tiles' loads 198 were left, without their stores to LDS 211,
 // without the softmax 213, without all three 174: none alone bounds it.  Two
 // buffers and a barrier a tile took 260 us, the form for few rows 816.  Over int8
-// caches 4096 tokens take 253 us with all of 4096 rows to see.
+// caches 4096 tokens take 253 us with all of 4096 rows to see; over 4-bit ones the
+// first call takes 230 where fp16 takes 223 in the same run, and 2048 tokens over as
+// many rows 100 where fp16 takes 86: codes are turned into fp16 once per 128 rows.
 //
 // A lane holds one row n = lane % 32 and, with h = lane / 32, the keys
 // wide_key(i, h) of a tile's score registers i = 0..15; operand step s of the
