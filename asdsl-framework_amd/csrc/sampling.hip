@@ -636,6 +636,48 @@ __device__ __forceinline__ unsigned long long block_scan(Last& s, unsigned long 
     return m;
 }
 
+// Tokens of a step: one a lane, or (N = 4) four neighbouring ones a lane, all of the
+// wave's `mine` of one logit and so of one weight w.
+template <int N>
+struct Some {
+    unsigned long long key[N], w;
+    bool mine[N];
+
+    // Their weights, and with kCount their number, to mass[place] and count[place], place =
+    // f(key): as one sum where a wave's lie in one place, or lane by lane.
+    template <bool kCount, typename F>
+    __device__ __forceinline__ void add(unsigned long long* mass, uint32_t* count, F f) const {
+        int at[N], here = -1;
+        bool alike = true;  // this lane's
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            at[i] = f(key[i]);
+            alike = alike && (!mine[i] || here < 0 || at[i] == here);
+            here = mine[i] ? at[i] : here;
+        }
+        const uint64_t any = __builtin_amdgcn_ballot_w64(here >= 0);
+        if (any == 0ull) return;
+        const int first = __builtin_ctzll(any), there = __builtin_amdgcn_readlane(here, first);
+        if (__builtin_amdgcn_ballot_w64(!alike || (here >= 0 && here != there)) == 0ull) {
+            uint32_t n = 0u;
+#pragma unroll
+            for (int i = 0; i < N; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(mine[i]));
+            const unsigned long long sum = N > 1 ? w * n : wave_sum(mine[0] ? w : 0ull);
+            if (static_cast<int>(threadIdx.x) % kWave == first) {
+                atomicAdd(&mass[there], sum);
+                if constexpr (kCount) atomicAdd(&count[there], n);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (mine[i]) {
+                    atomicAdd(&mass[at[i]], w);
+                    if constexpr (kCount) atomicAdd(&count[at[i]], 1u);
+                }
+        }
+    }
+};
+
 // The tokens that a cut may fall on: the list, or where it did not hold them all the
 // row.
 struct Source {
@@ -645,8 +687,8 @@ struct Source {
     int row, n;
     bool whole;
 
-    // f(rank, weight, is it one) for the tokens of bins [lo, hi] with ranks [low, low +
-    // span), by whole waves that hold any.  kRanksOnly: whatever their bins, no weights.
+    // f(Some) of the tokens of bins [lo, hi] with ranks [low, low + span), by whole waves
+    // that hold any.  kRanksOnly: whatever their bins, no weights.
     template <bool kRanksOnly, typename F>
     __device__ __forceinline__ void each(int lo, int hi, unsigned long long low, unsigned long long span, F f) const {
         const int t = static_cast<int>(threadIdx.x);
@@ -656,7 +698,8 @@ struct Source {
                 const unsigned long long w = i < n ? s.held[i] : 0ull, key = i < n ? s.rank[i] : 0ull;
                 const int b = static_cast<int>(w >> kBinShift);
                 const bool mine = i < n && b >= lo && b <= hi && key - low < span;
-                if (__builtin_amdgcn_ballot_w64(mine) != 0ull) f(key, w & ((1ull << kBinShift) - 1), mine);
+                if (__builtin_amdgcn_ballot_w64(mine) != 0ull)
+                    f(Some<1>{{key}, w & ((1ull << kBinShift) - 1), {mine}});
             }
             return;
         }
@@ -666,36 +709,68 @@ struct Source {
         const uint32_t o1 = min(static_cast<uint32_t>((low + span - 1) >> kRankBits), order_of(INFINITY));
         const float x0 = logit_of(o0), x1 = logit_of(o1);
         const int v0 = o0 == o1 ? token_of(low + span - 1) & ~3 : 0, v1 = o0 == o1 ? min(n, token_of(low) + 1) : n;
-        // four neighbouring tokens a thread, the next four on their way
+        // four neighbouring tokens a thread, the next ones on their way
         const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
         const auto load = [&](int v) {
             return make_float4(v < v1 ? x[v] : -INFINITY, v + 1 < v1 ? x[v + 1] : -INFINITY,
                                v + 2 < v1 ? x[v + 2] : -INFINITY, v + 3 < v1 ? x[v + 3] : -INFINITY);
         };
-        float4 next = load(v0 + 4 * t);
+        constexpr int kStep = 4 * kLast;
+        float4 next = load(v0 + 4 * t), then = load(v0 + 4 * t + kStep), last = load(v0 + 4 * t + 2 * kStep);
 #pragma unroll 1
-        for (int v = v0 + 4 * t; v - 4 * (t % kWave) < v1; v += 4 * kLast) {
+        for (int v = v0 + 4 * t; v - 4 * (t % kWave) < v1; v += kStep) {
             float4 q = next;
-            next = load(v + 4 * kLast);
-            const bool none = !((q.x >= x0 && q.x <= x1) || (q.y >= x0 && q.y <= x1) || (q.z >= x0 && q.z <= x1) ||
-                                (q.w >= x0 && q.w <= x1));
-            if (__builtin_amdgcn_ballot_w64(!none) == 0ull) continue;
+            next = then;
+            then = last;
+            last = load(v + 3 * kStep);
+            const float z[4] = {q.x, q.y, q.z, q.w};
+            float here = 0.0f;  // a logit of this lane's that is in range
+            bool in[4], alike = true, any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                in[i] = z[i] >= x0 && z[i] <= x1;
+                alike = alike && (!in[i] || !any || z[i] == here);
+                here = in[i] ? z[i] : here;
+                any = any || in[i];
+            }
+            const uint64_t lanes = __builtin_amdgcn_ballot_w64(any);
+            if (lanes == 0ull) continue;
+            const float there = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(uint32_t, here), __builtin_ctzll(lanes)));
+            if (__builtin_amdgcn_ballot_w64(!alike || (any && here != there)) == 0ull) {
+                Some<4> some;
+                some.w = 0ull;
+                if constexpr (!kRanksOnly) {
+                    const double y = scale.log2w(there);
+                    const int b = scale.bin(y);
+                    if (!Scale::any(y) || b < lo || b > hi) continue;
+                    some.w = Scale::weight(y);
+                }
+                const unsigned long long top = rank_of(there, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    some.key[i] = top - static_cast<uint32_t>(v + i);
+                    some.mine[i] = in[i] && some.key[i] - low < span;
+                }
+                f(some);
+                continue;
+            }
 #pragma unroll 1
             for (int j = 0; j < 4; ++j) {
-                const float z = q.x;
+                const float x = q.x;
                 q = make_float4(q.y, q.z, q.w, 0.0f);
-                const unsigned long long key = rank_of(z, v + j);
-                bool mine = z >= x0 && z <= x1 && key - low < span;
+                const unsigned long long key = rank_of(x, v + j);
+                bool mine = x >= x0 && x <= x1 && key - low < span;
                 if (__builtin_amdgcn_ballot_w64(mine) == 0ull) continue;
                 unsigned long long w = 0ull;
                 if constexpr (!kRanksOnly) {
-                    const double y = scale.log2w(z);
+                    const double y = scale.log2w(x);
                     const int b = scale.bin(y);
                     mine = mine && Scale::any(y) && b >= lo && b <= hi;
                     if (__builtin_amdgcn_ballot_w64(mine) == 0ull) continue;
                     w = Scale::weight_or_none(y);
                 }
-                f(key, w, mine);
+                f(Some<1>{{key}, w, {mine}});
             }
         }
     }
@@ -717,21 +792,10 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
     int shift = max(0, 64 - __builtin_clzll((span - 1) | 1ull) - kPartBits);
 #pragma unroll 1
     for (;;) {
-        src.each<false>(lo, hi, low, span, [&](unsigned long long key, unsigned long long w, bool mine) {
-            const int at = kParts - 1 - static_cast<int>((key - low) >> shift);
-            // equal logits lie in one part, lane by lane: their sum goes there as one
-            const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
-            const int first = __builtin_ctzll(all), there = __builtin_amdgcn_readlane(at, first);
-            if (__builtin_amdgcn_ballot_w64(mine && at == there) == all) {
-                const unsigned long long sum = wave_sum(mine ? w : 0ull);
-                if (lane == first) {
-                    atomicAdd(&s.mass[there], sum);
-                    atomicAdd(&s.count[there], static_cast<uint32_t>(__builtin_popcountll(all)));
-                }
-            } else if (mine) {
-                atomicAdd(&s.mass[at], w);
-                atomicAdd(&s.count[at], 1u);
-            }
+        src.each<false>(lo, hi, low, span, [&](const auto& some) {
+            some.template add<true>(s.mass, s.count, [&](unsigned long long key) {
+                return kParts - 1 - static_cast<int>((key - low) >> shift);
+            });
         });
         __syncthreads();
         if (t < kWave) {
@@ -767,12 +831,15 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
         if (held <= kWave || shift == 0) break;
         shift = shift > kPartBits ? shift - kPartBits : 0;
     }
-    src.each<false>(lo, hi, low, span, [&](unsigned long long key, unsigned long long w, bool mine) {
-        if (!mine) return;
-        const uint32_t i = atomicAdd(&s.few, 1u);
-        if (i < kWave) {
-            s.key[i] = key;
-            s.weight[i] = w;
+    src.each<false>(lo, hi, low, span, [&](const auto& some) {
+#pragma unroll
+        for (size_t j = 0; j < sizeof(some.mine); ++j) {
+            if (!some.mine[j]) continue;
+            const uint32_t i = atomicAdd(&s.few, 1u);
+            if (i < kWave) {
+                s.key[i] = some.key[j];
+                s.weight[i] = some.w;
+            }
         }
     });
     __syncthreads();
@@ -801,8 +868,9 @@ __device__ __forceinline__ unsigned long long select_rank(const Source& src, int
 // One workgroup a row.  A chain of loads (the slices' ends, their lists, the token's
 // tile), scans and barriers: 4.0 us without cuts, 9.5 with both, for one row as for 64.
 // Where the lists did not hold the cut's bins it goes through the row for each level of
-// a selection, at some 60 to 130 us a pass over 200064: equal logits throughout take
-// 300 to 400 us.
+// a selection, bound by the vector instructions of one compute unit: a call for one row of
+// 200064 equal logits takes 172 us with top-k and 229 with top-p, with a weight and a sum
+// for each token instead of one for a wave's 299 and 411.
 template <bool kCuts>
 __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a) {
     __shared__ Last s;
@@ -878,9 +946,12 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
             const unsigned long long from = low, span = high - low + 1;
             low = ~0ull;
             high = 0ull;
-            src.each<true>(lo, hi, from, span, [&](unsigned long long key, unsigned long long, bool mine) {
-                low = mine && key < low ? key : low;
-                high = mine && key > high ? key : high;
+            src.each<true>(lo, hi, from, span, [&](const auto& some) {
+#pragma unroll
+                for (size_t j = 0; j < sizeof(some.mine); ++j) {
+                    low = some.mine[j] && some.key[j] < low ? some.key[j] : low;
+                    high = some.mine[j] && some.key[j] > high ? some.key[j] : high;
+                }
             });
             low = wave_min(low);
             high = wave_max(high);
@@ -901,18 +972,10 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
             total = mass;
         }
         // the kept ones of the cut's bins join their tiles
-        src.each<false>(lo, kBins - 1, cut, (1ull << (32 + kRankBits)) - cut, [&](unsigned long long key, unsigned long long w, bool mine) {
-            const bool keep = mine && w >= least;
-            const int tile = token_of(key) / kTile;
-            const uint64_t all = __builtin_amdgcn_ballot_w64(keep);
-            if (all == 0ull) return;
-            const int first = __builtin_ctzll(all), there = __builtin_amdgcn_readlane(tile, first);
-            if (__builtin_amdgcn_ballot_w64(keep && tile == there) == all) {
-                const unsigned long long sum = wave_sum(keep ? w : 0ull);
-                if (lane == first) atomicAdd(&s.tiles[there], sum);
-            } else if (keep) {
-                atomicAdd(&s.tiles[tile], w);
-            }
+        src.each<false>(lo, kBins - 1, cut, s.high - cut + 1, [&](auto some) {
+#pragma unroll
+            for (size_t j = 0; j < sizeof(some.mine); ++j) some.mine[j] = some.mine[j] && some.w >= least;
+            some.template add<false>(s.tiles, nullptr, [&](unsigned long long key) { return token_of(key) / kTile; });
         });
         __syncthreads();
     }
