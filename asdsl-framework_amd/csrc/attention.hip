@@ -1615,25 +1615,50 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const A
 }
 
 // ------------------------------------------------------- few rows: kernels
-// The sequence of the place-th largest position, by its 8 leading bits of a cache's
-// rows and then by index; for up to 64 sequences.  Bit by bit, those that have it
-// before those that have not: scalar work, a quarter of what ranking every lane takes.
-constexpr int kOrdered = kWave;
-__device__ __forceinline__ int sequence_at(const AttnArgs& g, int place) {
+// The sequence of the place-th largest position, by its kBits leading bits of a cache's
+// rows and then by index; for up to 64 * kGroups sequences.  Bit by bit, those that
+// have it before those that have not: scalar work, a quarter of what ranking every
+// lane takes.
+constexpr int kOrdered = 4 * kWave;
+template <int kGroups, int kBits>
+__device__ __forceinline__ int sequence_of(const AttnArgs& g, int place) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
-    const int p = lane < g.n_seq ? min(max(g.pos[lane], 0), g.rows_b - 1) : 0;
-    const int key = p >> max(0, 24 - __builtin_clz(g.rows_b));
-    uint64_t left = g.n_seq < kWave ? (1ull << g.n_seq) - 1 : ~0ull;
+    int key[kGroups];
+    uint64_t left[kGroups];
 #pragma unroll
-    for (int bit = 7; bit >= 0; --bit) {
-        const uint64_t ones = __builtin_amdgcn_ballot_w64((key >> bit) & 1) & left;
-        const int n = __builtin_popcountll(ones);
-        left = place < n ? ones : left & ~ones;
-        place = place < n ? place : place - n;
+    for (int i = 0; i < kGroups; ++i) {
+        const int seq = kWave * i + lane;
+        const int p = seq < g.n_seq ? min(max(g.pos[seq], 0), g.rows_b - 1) : 0;
+        key[i] = p >> max(0, 32 - kBits - __builtin_clz(g.rows_b));
+        left[i] = __builtin_amdgcn_ballot_w64(seq < g.n_seq);
     }
-    const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(left >> 32),
-                                                 __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(left), 0u));
-    return uniform(__builtin_ctzll(__builtin_amdgcn_ballot_w64(before == place) & left));
+#pragma unroll
+    for (int bit = kBits - 1; bit >= 0; --bit) {
+        uint64_t ones[kGroups];
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+            ones[i] = __builtin_amdgcn_ballot_w64((key[i] >> bit) & 1) & left[i];
+            n += __builtin_popcountll(ones[i]);
+        }
+        const bool one = place < n;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) left[i] = one ? ones[i] : left[i] & ~ones[i];
+        place = one ? place : place - n;
+    }
+    int seq = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        const int n = __builtin_popcountll(left[i]);
+        const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(left[i] >> 32),
+                                                     __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(left[i]), 0u));
+        if (place >= 0 && place < n) seq = kWave * i + __builtin_ctzll(__builtin_amdgcn_ballot_w64(before == place) & left[i]);
+        place -= n;
+    }
+    return uniform(seq);
+}
+__device__ __forceinline__ int sequence_at(const AttnArgs& g, int place) {
+    return g.n_seq <= kWave ? sequence_of<1, 8>(g, place) : sequence_of<4, 5>(g, place);
 }
 
 // blockIdx.x = ((sequence * row tiles + tile) * splits + split) * n_kv + kv head:
@@ -2027,8 +2052,9 @@ asdsl_status window(const char* what, Kv form, const float* q, const Cache& c, c
     AttnArgs g{q, out, nullptr, nullptr, c, c, pos, n_seq, n_tokens, n_heads, n_kv_heads, rows, rows, -1, window,
                sinks, p.splits, p.slots, kLog2e / sqrtf(static_cast<float>(head_dim))};
     place_work(g, p, work, head_dim);
-    // Where the workgroups come one after the other, ragged sequences take 12 to 15 % less
-    // with the longest first: 32 of up to 16000 rows 82 -> 71 us, 64 of up to 4000 48 -> 41.
+    // Where the workgroups come one after the other, ragged sequences take 6 to 25 % less
+    // with the longest first: 32 of up to 16000 rows 82 -> 71 us, 64 of up to 4000 48 -> 41;
+    // 128 of up to 8000 182 -> 136, 128 of up to 4000 87 -> 69, 256 of up to 500 33 -> 31.
     g.longest_first = form == kI4 && n_seq > 1 && n_seq <= kOrdered && p.jobs > kFillFew;
     const dim3 grid(static_cast<unsigned>(p.jobs));
     auto with = [&](auto dim, auto codes) {

@@ -163,7 +163,9 @@ def test_window(gpu, case):
 
 
 @pytest.mark.parametrize("n,kvh,d,rows,win", [(40, 16, 128, 700, 0), (64, 16, 64, 1100, 200), (65, 16, 64, 1100, 0),
-                                              (2, 300, 64, 530, 0)])
+                                              (2, 300, 64, 530, 0), (127, 8, 64, 530, 0), (128, 8, 128, 300, 40),
+                                              (129, 8, 64, 300, 0), (193, 4, 64, 530, 0), (256, 4, 128, 270, 0),
+                                              (257, 4, 64, 300, 0)])
 def test_window_of_many_ragged_sequences(gpu, n, kvh, d, rows, win):
     """More workgroups than run at once, which take the longest sequences first; equal positions, padded sequences."""
     from asdsl.kernels import attention_window
