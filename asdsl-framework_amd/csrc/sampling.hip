@@ -76,7 +76,7 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 // What a row's slices found.
 struct Ends {
     unsigned long long best;  // order_of the largest logit, and below it ~ its first token; 0: nothing to draw from
-    uint32_t low;             // order_of the logit at which the last bin ends, or of a smaller one
+    uint32_t low;             // order_of the logit at which the last bin begins; smaller ones may have weights
 };
 
 // Logits so far below another have no weight.
@@ -137,10 +137,12 @@ struct Scale {
         const unsigned long long w = weight(fmax(y, -2.0 * kDepth));
         return any(y) ? w : 0ull;
     }
-    // 0 .. kBins - 1, rising as weights fall, where any(y); the sum with 2^52 rounds to a
-    // whole number.  The last bin takes in all that is smaller.
+    // 0 .. kBins - 1, rising as weights fall; the sum with 2^52 rounds to a whole number.
+    // The last bin takes in all that is smaller.  Held to it before the bits are taken:
+    // the bins may end a bit of a float below the largest logit (Ends::low), and 44
+    // doublings in units of such bins are past 32 bits and past 2^52.
     __device__ __forceinline__ int bin(double y) const {
-        return min(static_cast<int>(__builtin_bit_cast(uint64_t, fma(y, -per_bin, 0x1p52))), kBins - 1);
+        return static_cast<int>(__builtin_bit_cast(uint64_t, fmin(fma(y, -per_bin, 0x1p52), 0x1p52 + (kBins - 1))));
     }
 };
 
@@ -266,10 +268,12 @@ struct Stream {
 };
 
 // ------------------------------------------------------------- largest logit
-// And, for the bins, the smallest of those that may have a weight beside it, about:
-// logits of -10000 for tokens that do not exist or are not allowed would leave the
-// others few bins.  A lane forgets a small one when one out of its reach comes, lanes
-// and slices out of the largest one's reach do not count.
+// And, for the bins, a small one of those that may have a weight beside it: logits of
+// -10000 for tokens that do not exist or are not allowed would leave the others few
+// bins.  It is some such logit, not the least: a lane forgets what it has when its
+// largest one rises out of reach of it, and lanes and slices whose small one is out of
+// the largest one's reach do not count, also where others of theirs are in it.  What
+// lies below goes into the last bin.
 //
 // Bound by memory: 64 rows of 200064 (51 MB) 10.8 us, 4.7 TB/s; one row 3.6.
 template <bool kVec, bool kLow>

@@ -151,6 +151,31 @@ def test_logits_for_tokens_that_do_not_exist(gpu):
               top_k=np.array([5, 100, 9000, 3, 32999, 33001, 39999, 1], np.int32))
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 8), (3, 1021), (2, 4096), (600, 3000), (2, 70000)])
+def test_bins_that_end_beside_the_largest_logit(gpu, rows, vocab):
+    """Four neighbouring tokens without weight but for the two largest logits, a bit of fp32 apart, and -31 among all
+    others, which is out of the largest one's reach but not of theirs: the bins' range is that bit, and tokens with
+    weights lie some 10^10 of its 255th parts below it.  Others of a lane and of its later steps alike."""
+    top = np.float32(0.3)
+    x = np.full((rows, vocab), -0.7, np.float32)
+    x[:, 1::4] = -31.0
+    for i in range(rows):
+        at = (4 * 307 * i + (i % 2) * 2048) % max(4, (vocab - 4) // 4 * 4)  # in a lane's first steps and in later ones
+        x[i, at:at + 4] = top, np.nextafter(top, np.float32(0)), -np.inf, -np.inf
+    rng = np.random.default_rng(vocab)
+    k = rng.integers(3, vocab // 2 + 1, rows).astype(np.int32)
+    k[0] = 3
+    p = rng.uniform(0.5, 0.99, rows).astype(np.float32)
+    u = rng.random(rows, dtype=np.float32)
+    for kw in ({"top_k": k}, {"top_p": p}, {"top_k": k, "top_p": p},
+               {"top_k": k, "temperature": np.full(rows, 1e-3, np.float32)},
+               {"top_p": p, "min_p": np.full(rows, 0.3, np.float32)}):
+        check(x, u, **kw)
+    if rows == 1:  # the share of the third token is that of three kept ones
+        got, probs = run(x, [0.999], top_k=k)
+        assert got[0] == 4 and abs(probs[0] - np.exp(-1) / (2 + np.exp(-1))) < 1e-6
+
+
 def test_every_kept_token_by_its_share(gpu):
     """u over a grid draws each kept token as often as its share, in index order, and no other."""
     rng = np.random.default_rng(1)
