@@ -709,10 +709,13 @@ struct Source {
         }
         // A comparison of floats first, and of one logit's equals only those in range: a
         // vector instruction a token is 1.3 us of a row of 200064 by one workgroup.
-        const uint32_t o0 = static_cast<uint32_t>(low >> kRankBits);
-        const uint32_t o1 = min(static_cast<uint32_t>((low + span - 1) >> kRankBits), order_of(INFINITY));
+        // The range's end is held to the first token of +inf: the topmost of a selection's
+        // equal parts may reach past it, into ranks of no logit.
+        const unsigned long long first = (static_cast<unsigned long long>(order_of(INFINITY)) << kRankBits) | (kMaxVocab - 1);
+        const unsigned long long end = low + span - 1 < first ? low + span - 1 : first;
+        const uint32_t o0 = static_cast<uint32_t>(low >> kRankBits), o1 = static_cast<uint32_t>(end >> kRankBits);
         const float x0 = logit_of(o0), x1 = logit_of(o1);
-        const int v0 = o0 == o1 ? token_of(low + span - 1) & ~3 : 0, v1 = o0 == o1 ? min(n, token_of(low) + 1) : n;
+        const int v0 = o0 == o1 ? token_of(end) & ~3 : 0, v1 = o0 == o1 ? min(n, token_of(low) + 1) : n;
         // four neighbouring tokens a thread, the next ones on their way
         const float* x = a.logits + static_cast<size_t>(row) * a.vocab;
         const auto load = [&](int v) {

@@ -176,6 +176,27 @@ def test_bins_that_end_beside_the_largest_logit(gpu, rows, vocab):
         assert got[0] == 4 and abs(probs[0] - np.exp(-1) / (2 + np.exp(-1))) < 1e-6
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 5000), (5, 5003), (3, 70001), (2, 200064), (1, 1 << 20)])
+@pytest.mark.parametrize("others", [False, True])
+def test_more_infinite_logits_than_the_lists_hold(gpu, rows, vocab, others):
+    """Rows of +inf, all or (others) three of four of them, share evenly: cuts among the first of them, where the
+    topmost part of a selection reaches past the largest rank that there is."""
+    rng = np.random.default_rng(rows + vocab)
+    x = np.full((rows, vocab), np.inf, np.float32)
+    if others:
+        away = rng.random((rows, vocab)) < 0.25
+        x[away] = rng.choice(np.array([3e38, 0, -np.inf, np.nan], np.float32), int(away.sum()))
+    u = rng.random(rows, dtype=np.float32)
+    for k in (2, 3, 4, 100, 385, 1025, vocab // 2, vocab):
+        check(x, u, top_k=np.full(rows, k, np.int32))
+    for p in (1e-6, 3.3 / vocab, 70.7 / vocab, 0.4):
+        check(x, u, top_p=np.full(rows, p, np.float32))
+    check(x, u, top_k=np.full(rows, 400, np.int32), top_p=np.full(rows, 0.011, np.float32))
+    if not others:  # the last of four
+        got, probs = run(x, np.full(rows, 0.8, np.float32), top_k=np.full(rows, 4, np.int32))
+        assert (got == 3).all() and (probs == 0.25).all()
+
+
 def test_every_kept_token_by_its_share(gpu):
     """u over a grid draws each kept token as often as its share, in index order, and no other."""
     rng = np.random.default_rng(1)
