@@ -542,7 +542,7 @@ __global__ __launch_bounds__(kThreads) void sample_keep_kernel(const SampleArgs 
         const float x = queue.x[at];
         const double y = s.log2w(x);
         if (!Scale::any(y)) return;
-        const int b = s.bin(y);
+        const int b = kCuts ? s.bin(y) : 0;
         const unsigned long long w = Scale::weight(y);
         sum += (b < before && w >= least) ? w : 0ull;
         if (b >= before && in_cut(b)) note(x, kCuts ? queue.v[at] : 0);
@@ -561,7 +561,7 @@ __global__ __launch_bounds__(kThreads) void sample_keep_kernel(const SampleArgs 
             for (int i = 0; i < 4; ++i) {
                 const double y = s.log2w(x[i]);
                 const unsigned long long w = Scale::weight_or_none(y);
-                const int b = s.bin(y);
+                const int b = kCuts ? s.bin(y) : 0;
                 const bool any = Scale::any(y);
                 sum += (any & (b < before) & (w >= least)) ? w : 0ull;
                 cut |= (any & (b >= before) & in_cut(b)) ? 1u << i : 0u;
