@@ -108,10 +108,16 @@ SIGNATURES: dict[str, list] = {
     "asdsl_kv_append_q4": [_P] * 9 + [_I] * 9 + [_P],
     "asdsl_kv_read_q8": [_P] * 7 + [_I] * 6 + [_P],
     "asdsl_kv_read_q4": [_P] * 7 + [_I] * 6 + [_P],
+    "asdsl_attention_window_f16kv_work_bytes": [_I] * 8,
+    "asdsl_attention_window_q8kv_work_bytes": [_I] * 8,
+    "asdsl_attention_window_q4kv_work_bytes": [_I] * 8,
     "asdsl_attention_window_work_bytes": [_I] * 8,
     "asdsl_attention_window_f16kv": [_P] * 5 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_window_q8kv": [_P] * 7 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_window_q4kv": [_P] * 7 + [_I] * 8 + [_P, ctypes.c_size_t, _P],
+    "asdsl_attention_prefix_f16kv_work_bytes": [_I] * 6,
+    "asdsl_attention_prefix_q8kv_work_bytes": [_I] * 6,
+    "asdsl_attention_prefix_q4kv_work_bytes": [_I] * 6,
     "asdsl_attention_prefix_work_bytes": [_I] * 6,
     "asdsl_attention_prefix_f16kv": [_P] * 7 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
     "asdsl_attention_prefix_q8kv": [_P] * 11 + [_I] * 7 + [_P, ctypes.c_size_t, _P],
@@ -142,7 +148,13 @@ _RESTYPE = {"asdsl_last_error": ctypes.c_char_p, "asdsl_attention_work_floats": 
             "asdsl_gemv_preq2_fused_batch_work_bytes_n": ctypes.c_size_t,
             "asdsl_affine_batch_work_bytes": ctypes.c_size_t,
             "asdsl_decode_branches_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_window_f16kv_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_window_q8kv_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_window_q4kv_work_bytes": ctypes.c_size_t,
             "asdsl_attention_window_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_prefix_f16kv_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_prefix_q8kv_work_bytes": ctypes.c_size_t,
+            "asdsl_attention_prefix_q4kv_work_bytes": ctypes.c_size_t,
             "asdsl_attention_prefix_work_bytes": ctypes.c_size_t,
             "asdsl_logits_control_work_bytes": ctypes.c_size_t,
             "asdsl_sample_logits_work_bytes": ctypes.c_size_t}

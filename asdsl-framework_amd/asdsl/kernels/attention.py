@@ -137,13 +137,9 @@ def _work(nbytes: int, like):
 
 
 @functools.lru_cache(maxsize=4096)
-def _window_bytes(*dims) -> int:
-    return _hip.LIB.asdsl_attention_window_work_bytes(*dims)
-
-
-@functools.lru_cache(maxsize=4096)
-def _prefix_bytes(*dims) -> int:
-    return _hip.LIB.asdsl_attention_prefix_work_bytes(*dims)
+def _work_bytes(entry: str, *dims) -> int:
+    """Bytes of work that a call of an entry point, and so over its form of caches, needs."""
+    return getattr(_hip.LIB, entry + "_work_bytes")(*dims)
 
 
 def kv_append(qkv, k_cache, v_cache, rope_cos, rope_sin, pos, *, n_heads: int, pos_offset: int = 0, k_scale=None,
@@ -261,9 +257,10 @@ def attention_window(q, k_cache, v_cache, pos, *, n_heads: int | None = None, wi
           _addr(fn, dev, "pos", pos, _i32, n_seq))
     if out is None:
         out = _empty_like(q)
-    nbytes = _window_bytes(*dims)
+    entry = _WINDOW[k_cache.dtype]
+    nbytes = _work_bytes(entry, *dims)
     work = _work(nbytes, q)
-    _hip.call(_WINDOW[k_cache.dtype], *at,
+    _hip.call(entry, *at,
               _addr(fn, dev, "out", out, _f32, n), *dims, None if work is None else work.data_ptr(), nbytes,
               _stream(dev))
     return out
@@ -299,9 +296,10 @@ def attention_prefix(q, k_prefix, v_prefix, k_own, v_own, own_pos, *, prefix_len
           *_caches(fn, dev, "own", k_own, v_own, k_scale, v_scale, d), _addr(fn, dev, "own_pos", own_pos, _i32, n_seq))
     if out is None:
         out = _empty_like(q)
-    nbytes = _prefix_bytes(n_seq, n_heads, n_kv, d, prefix_len, rows)
+    entry = _PREFIX[k_own.dtype]
+    nbytes = _work_bytes(entry, n_seq, n_heads, n_kv, d, prefix_len, rows)
     work = _work(nbytes, q)
-    _hip.call(_PREFIX[k_own.dtype], *at,
+    _hip.call(entry, *at,
               _addr(fn, dev, "out", out, _f32, n), n_seq, n_heads, n_kv, d, prefix_len, prefix_rows, rows,
               None if work is None else work.data_ptr(), nbytes, _stream(dev))
     return out

@@ -8,6 +8,7 @@
 // 16-bit word per 32 dims (kv_int4.hpp); queries and outputs are fp32.
 #include <hip/hip_fp16.h>
 
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -2002,6 +2003,22 @@ Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, Kv form, int pr
     return finish(p, head_dim);
 }
 
+// What the work queries give for a form: 0 for sizes that the call refuses.
+size_t window_bytes(Kv form, int n_seq, int n_tokens, int n_heads, int n_kv, int head_dim, int rows, int window,
+                    int sinks) {
+    if (check_heads("attention_window", n_seq, n_tokens, n_heads, n_kv, head_dim) != ASDSL_OK || rows <= 0 ||
+        rows > kMaxRows || window < 0 || sinks < 0)
+        return 0;
+    return plan_window(n_seq, n_tokens, n_heads, n_kv, head_dim, form, rows, window, sinks).work;
+}
+
+size_t prefix_bytes(Kv form, int n_seq, int n_heads, int n_kv, int head_dim, int prefix_len, int own_rows) {
+    if (check_heads("attention_prefix", n_seq, 1, n_heads, n_kv, head_dim) != ASDSL_OK || prefix_len < 0 ||
+        prefix_len > kMaxRows || own_rows <= 0 || own_rows > kMaxRows)
+        return 0;
+    return plan_prefix(n_seq, n_heads, n_kv, head_dim, form, prefix_len, own_rows).work;
+}
+
 // The grids of the call's launches: the keys' pieces, and the join's.
 asdsl_status check_launches(const char* what, const Plan& p) {
     static_assert(kFewWaves == kManyWaves, "one workgroup size");
@@ -2135,16 +2152,26 @@ extern "C" asdsl_status asdsl_kv_append_q4(const float* qkv, uint8_t* k_cache, u
                   n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, rows, pos_offset, rope_rows, stream);
 }
 
+extern "C" size_t asdsl_attention_window_f16kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads,
+                                                          int head_dim, int rows, int window_size, int sinks) {
+    return window_bytes(kF16, n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks);
+}
+
+extern "C" size_t asdsl_attention_window_q8kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads,
+                                                         int head_dim, int rows, int window_size, int sinks) {
+    return window_bytes(kI8, n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks);
+}
+
+extern "C" size_t asdsl_attention_window_q4kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads,
+                                                         int head_dim, int rows, int window_size, int sinks) {
+    return window_bytes(kI4, n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks);
+}
+
 extern "C" size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
                                                     int rows, int window_size, int sinks) {
-    if (check_heads("attention_window", n_seq, n_tokens, n_heads, n_kv_heads, head_dim) != ASDSL_OK || rows <= 0 ||
-        rows > kMaxRows || window_size < 0 || sinks < 0)
-        return 0;
-    size_t most = 0;  // of the cache types
-    for (const Kv form : {kF16, kI8, kI4}) {
-        const Plan p = plan_window(n_seq, n_tokens, n_heads, n_kv_heads, head_dim, form, rows, window_size, sinks);
-        most = p.work > most ? p.work : most;
-    }
+    size_t most = 0;
+    for (const Kv form : {kF16, kI8, kI4})
+        most = std::max(most, window_bytes(form, n_seq, n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks));
     return most;
 }
 
@@ -2175,16 +2202,26 @@ extern "C" asdsl_status asdsl_attention_window_q4kv(const float* q, const uint8_
                   n_tokens, n_heads, n_kv_heads, head_dim, rows, window_size, sinks, work, work_bytes, stream);
 }
 
+extern "C" size_t asdsl_attention_prefix_f16kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim,
+                                                          int prefix_len, int own_rows) {
+    return prefix_bytes(kF16, n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows);
+}
+
+extern "C" size_t asdsl_attention_prefix_q8kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim,
+                                                         int prefix_len, int own_rows) {
+    return prefix_bytes(kI8, n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows);
+}
+
+extern "C" size_t asdsl_attention_prefix_q4kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim,
+                                                         int prefix_len, int own_rows) {
+    return prefix_bytes(kI4, n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows);
+}
+
 extern "C" size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim,
                                                     int prefix_len, int own_rows) {
-    if (check_heads("attention_prefix", n_seq, 1, n_heads, n_kv_heads, head_dim) != ASDSL_OK || prefix_len < 0 ||
-        prefix_len > kMaxRows || own_rows <= 0 || own_rows > kMaxRows)
-        return 0;
-    size_t most = 0;  // of the cache types
-    for (const Kv form : {kF16, kI8, kI4}) {
-        const Plan p = plan_prefix(n_seq, n_heads, n_kv_heads, head_dim, form, prefix_len, own_rows);
-        most = p.work > most ? p.work : most;
-    }
+    size_t most = 0;
+    for (const Kv form : {kF16, kI8, kI4})
+        most = std::max(most, prefix_bytes(form, n_seq, n_heads, n_kv_heads, head_dim, prefix_len, own_rows));
     return most;
 }
 

@@ -704,7 +704,15 @@ asdsl_status asdsl_kv_read_q4(const uint8_t* k_cache, const uint8_t* v_cache, co
  * it, as the definition has it: a score of +inf or NaN makes their outputs NaN, a
  * key of score -inf has no weight (out is zero where all have none), and an
  * infinite value is its dim's output at any weight (NaN at none).  Such tokens are
- * taken again one by one, at up to sixty times the cost. */
+ * taken again one by one, at up to sixty times the cost.  The query of a
+ * cache's form gives what calls over such caches need; the one without a form
+ * the most of the three. */
+size_t asdsl_attention_window_f16kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                               int rows, int window, int sinks);
+size_t asdsl_attention_window_q8kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                              int rows, int window, int sinks);
+size_t asdsl_attention_window_q4kv_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim,
+                                              int rows, int window, int sinks);
 size_t asdsl_attention_window_work_bytes(int n_seq, int n_tokens, int n_heads, int n_kv_heads, int head_dim, int rows,
                                          int window, int sinks);
 asdsl_status asdsl_attention_window_f16kv(const float* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -726,7 +734,13 @@ asdsl_status asdsl_attention_window_q4kv(const float* q, const uint8_t* k_cache,
  * its own caches [n_seq][n_kv_heads][own_rows][head_dim] (own_pos[s] = -1:
  * none); its token follows them all.  A sequence that sees nothing, or whose
  * own_pos is outside [-1, own_rows), gets zero.  With prefix_len 0 the prefix
- * pointers may be null. */
+ * pointers may be null.  Queries as those of asdsl_attention_window. */
+size_t asdsl_attention_prefix_f16kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
+                                               int own_rows);
+size_t asdsl_attention_prefix_q8kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
+                                              int own_rows);
+size_t asdsl_attention_prefix_q4kv_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
+                                              int own_rows);
 size_t asdsl_attention_prefix_work_bytes(int n_seq, int n_heads, int n_kv_heads, int head_dim, int prefix_len,
                                          int own_rows);
 asdsl_status asdsl_attention_prefix_f16kv(const float* q, const uint16_t* k_prefix, const uint16_t* v_prefix,

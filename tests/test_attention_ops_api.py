@@ -162,3 +162,34 @@ def test_sizes_past_the_kernels_ints():
                 call(x)
     with pytest.raises(ValueError, match=r"2\^30"):
         control_logits(torch.zeros(1, 40), history=torch.zeros(1, dtype=torch.int32).expand((1 << 30) + 1))
+
+
+def test_work_bytes_by_the_caches_form():
+    """A form's query is what a call over such caches needs: fp16 and int8 calls that take no work buffer get none
+    where the 4-bit form takes one, and the query without a form is the most of the three."""
+    import random
+
+    from asdsl import _hip
+
+    lib = _hip.LIB
+    window = [getattr(lib, f"asdsl_attention_window_{f}_work_bytes") for f in ("f16kv", "q8kv", "q4kv")]
+    prefix = [getattr(lib, f"asdsl_attention_prefix_{f}_work_bytes") for f in ("f16kv", "q8kv", "q4kv")]
+    # 99 sequences of 16 tokens: the wide form with one piece of keys over fp16 and int8, pieces over 4 bits
+    rows = 99 * 16 * 8  # query rows, each with head_dim + 2 floats a piece
+    assert [f(99, 16, 8, 4, 128, 12139, 0, 0) for f in window] == [0, 0, rows * 2 * (128 + 2) * 4]
+    call = lib.asdsl_attention_window_q4kv
+    refused(call(*(ONE,) * 7, 99, 16, 8, 4, 128, 12139, 0, 0, ONE, rows * 2 * 130 * 4 - 1, None), "work buffer")
+    rng, less = random.Random(5), 0
+    for _ in range(2000):
+        kv = rng.choice([1, 2, 4, 8])
+        n, t, h, d = rng.randint(1, 128), rng.choice([1, 1, rng.randint(2, 4096)]), kv * rng.randint(1, 8), rng.choice([64, 128])
+        dims = (n, t, h, kv, d, rng.randint(1, 20000), rng.choice([0, 256, 4096]), rng.choice([0, 4]))
+        each = [f(*dims) for f in window]
+        assert lib.asdsl_attention_window_work_bytes(*dims) == max(each), dims
+        less += max(each[:2]) < each[2]
+        dims = (n, h, kv, d, rng.randint(0, 20000), rng.randint(1, 2000))
+        assert lib.asdsl_attention_prefix_work_bytes(*dims) == max(f(*dims) for f in prefix), dims
+    assert less > 100  # such calls are no rarity
+    big = (1 << 30) + 1
+    assert not any(f(1, 1, 8, 2, 64, big, 0, 0) or f(1, 1, 9, 2, 64, 9, 0, 0) or f(1, 1, 8, 2, 64, 9, -1, 0) for f in window)
+    assert not any(f(1, 8, 2, 64, big, 1) or f(1, 8, 2, 64, 1, big) or f(1, 8, 2, 80, 1, 1) for f in prefix)

@@ -376,3 +376,38 @@ def test_refusals_on_the_device(gpu):
         assert lib.asdsl_attention_window_f16kv(one, one, one, one, one, 1, 1, 24, 8, 128, 4096, 0, 0, one, need - 1,
                                                 None) == gpu.ASDSL_ERR_INVALID_ARGUMENT
         assert "work buffer" in gpu.last_error()
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8"])
+def test_calls_that_need_no_work_buffer_allocate_none(gpu, kv):
+    """With its output given a call whose keys are taken in one piece allocates nothing, and one in pieces the bytes
+    of its own form, not those of another."""
+    import torch
+
+    from asdsl.kernels import attention_prefix, attention_window
+
+    rng = np.random.default_rng(1)
+    form = "f16kv" if kv == "fp16" else "q8kv"
+
+    def taken(call, *args, **kw):
+        out = torch.empty_like(args[0])
+        before = torch.cuda.memory_stats()["requested_bytes.all.allocated"]
+        call(*args, out=out, **kw)
+        return torch.cuda.memory_stats()["requested_bytes.all.allocated"] - before
+
+    for n, t, h, kvh, d, rows in ((99, 16, 8, 4, 128, 12139), (60, 24, 16, 4, 64, 5000), (1, 1, 24, 8, 128, 4352)):
+        k, ks, _ = make_cache(rng, kv, n, kvh, 1, d)
+        k = k.expand(n, kvh, rows, d).contiguous()
+        ks = None if ks is None else ks.expand(n, kvh, rows, d // 64).contiguous()
+        pos = dev(rng.integers(0, 300, n).astype(np.int32))
+        q = torch.randn((n, t, h, d), device="cuda")
+        need = getattr(gpu.LIB, f"asdsl_attention_window_{form}_work_bytes")(n, t, h, kvh, d, rows, 0, 0)
+        got = taken(attention_window, q, k, k, pos, k_scale=ks, v_scale=ks)
+        assert got == need
+    own, own_s, _ = make_cache(rng, kv, 3, 8, 100, 128)
+    q, pos = torch.randn((3, 24, 128), device="cuda"), dev(np.array([5, -1, 99], np.int32))
+    pre, pre_s, _ = make_cache(rng, kv, 8, 3000, 128)
+    need = getattr(gpu.LIB, f"asdsl_attention_prefix_{form}_work_bytes")(3, 24, 8, 128, 3000, 100)
+    got = taken(attention_prefix, q, pre, pre, own, own, pos, k_prefix_scale=pre_s, v_prefix_scale=pre_s, k_scale=own_s,
+                v_scale=own_s)
+    assert got == need
