@@ -125,6 +125,7 @@ SIGNATURES: dict[str, list] = {
     "asdsl_logits_control_work_bytes": [_I, _I],
     "asdsl_logits_control": [_P] * 6 + [_I] + [_P] * 4 + [ctypes.c_longlong, _P, ctypes.c_longlong, _I, _I, _P,
                                                          ctypes.c_size_t, _P],
+    "asdsl_sample_logits_work_bytes_cuts": [_I, _I, _I],
     "asdsl_sample_logits_work_bytes": [_I, _I],
     "asdsl_sample_logits": [_P] * 8 + [_I, _I, _P, ctypes.c_size_t, _P],
     "asdsl_decode_branches_work_bytes": [_P, _I, _I, _I],
@@ -157,6 +158,7 @@ _RESTYPE = {"asdsl_last_error": ctypes.c_char_p, "asdsl_attention_work_floats": 
             "asdsl_attention_prefix_q4kv_work_bytes": ctypes.c_size_t,
             "asdsl_attention_prefix_work_bytes": ctypes.c_size_t,
             "asdsl_logits_control_work_bytes": ctypes.c_size_t,
+            "asdsl_sample_logits_work_bytes_cuts": ctypes.c_size_t,
             "asdsl_sample_logits_work_bytes": ctypes.c_size_t}
 
 

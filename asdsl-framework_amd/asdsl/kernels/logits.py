@@ -102,8 +102,8 @@ def control_logits(logits, *, history=None, prompt_len=None, history_len=None, r
 
 
 @functools.lru_cache(maxsize=4096)
-def _sample_bytes(rows: int, vocab: int) -> int:
-    return _hip.LIB.asdsl_sample_logits_work_bytes(rows, vocab)
+def _sample_bytes(rows: int, vocab: int, cuts: bool) -> int:
+    return _hip.LIB.asdsl_sample_logits_work_bytes_cuts(rows, vocab, cuts)
 
 
 def sample_logits(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None):
@@ -143,7 +143,7 @@ def sample_logits(logits, uniform, *, temperature=None, top_k=None, top_p=None, 
           None if top_p is None else _addr(fn, dev, "top_p", top_p, _f32, rows),
           None if min_p is None else _addr(fn, dev, "min_p", min_p, _f32, rows))
     tokens, probs = logits.new_empty(rows, dtype=_i32), logits.new_empty(rows)
-    nbytes = _sample_bytes(rows, vocab)
+    nbytes = _sample_bytes(rows, vocab, top_k is not None or top_p is not None)
     work = _work(nbytes, logits)
     _hip.call("asdsl_sample_logits", *at, tokens.data_ptr(), probs.data_ptr(), rows, vocab,
               None if work is None else work.data_ptr(), nbytes, _stream(dev))

@@ -1020,13 +1020,14 @@ __global__ __launch_bounds__(kLast) void sample_token_kernel(const SampleArgs a)
 // within the slice's list: without a list the token's workgroup looks the row through.
 constexpr int kSliceTiles = 48;
 
-// Slices of a row: so many that the launch fills the chip, of whole steps.
+// Slices of a row: so many that the launch fills the chip, of whole steps.  What only
+// top-k and top-p use (bins and lists, 11 KB a slice) has no place without them.
 struct Plan {
     int slices, slice, tiles;
-    size_t best, low, mass, count, tile, state, listed, list, bytes;  // where each begins
+    size_t best, low, tile, mass, count, state, listed, list, bytes;  // where each begins
 };
 
-Plan plan_for(int n_rows, int vocab) {
+Plan plan_for(int n_rows, int vocab, bool cuts) {
     Plan p;
     p.tiles = (vocab + kTile - 1) / kTile;
     const int want = std::min((1024 + n_rows - 1) / n_rows, kMaxSlices);
@@ -1041,12 +1042,13 @@ Plan plan_for(int n_rows, int vocab) {
     const size_t rows = static_cast<size_t>(n_rows), pieces = rows * p.slices;
     place(p.best, pieces * sizeof(unsigned long long));
     place(p.low, pieces * sizeof(uint32_t));
-    place(p.mass, pieces * kBins * sizeof(unsigned long long));
-    place(p.count, pieces * kBins * sizeof(uint32_t));
     place(p.tile, rows * p.tiles * sizeof(unsigned long long));
-    place(p.state, rows * sizeof(RowState));
-    place(p.listed, pieces * sizeof(uint32_t));
-    place(p.list, pieces * kSliceMost * sizeof(uint2));
+    const size_t cut = cuts ? pieces : 0;
+    place(p.mass, cut * kBins * sizeof(unsigned long long));
+    place(p.count, cut * kBins * sizeof(uint32_t));
+    place(p.state, cuts ? rows * sizeof(RowState) : 0);
+    place(p.listed, cut * sizeof(uint32_t));
+    place(p.list, cut * kSliceMost * sizeof(uint2));
     p.bytes = at;
     return p;
 }
@@ -1056,9 +1058,13 @@ Plan plan_for(int n_rows, int vocab) {
 
 using namespace asdsl;
 
-extern "C" size_t asdsl_sample_logits_work_bytes(int n_rows, int vocab) {
+extern "C" size_t asdsl_sample_logits_work_bytes_cuts(int n_rows, int vocab, int cuts) {
     if (n_rows <= 0 || vocab <= 0 || vocab > kMaxVocab) return 0;
-    return plan_for(n_rows, vocab).bytes;
+    return plan_for(n_rows, vocab, cuts != 0).bytes;
+}
+
+extern "C" size_t asdsl_sample_logits_work_bytes(int n_rows, int vocab) {
+    return asdsl_sample_logits_work_bytes_cuts(n_rows, vocab, 1);
 }
 
 extern "C" asdsl_status asdsl_sample_logits(const float* logits, const float* uniform, const float* temperature,
@@ -1069,7 +1075,8 @@ extern "C" asdsl_status asdsl_sample_logits(const float* logits, const float* un
     ASDSL_CHECK_ARG(logits && uniform && tokens && probs, "%s: null pointer", what);
     ASDSL_CHECK_ARG(n_rows > 0 && vocab > 0, "%s: n_rows and vocab must be positive", what);
     ASDSL_CHECK_ARG(vocab <= kMaxVocab, "%s: vocab must be at most 2^20", what);
-    const Plan p = plan_for(n_rows, vocab);
+    const bool cuts = top_k || top_p;
+    const Plan p = plan_for(n_rows, vocab, cuts);
     ASDSL_CHECK_ARG(fits_launch(static_cast<long long>(n_rows) * p.slices, kThreads) && fits_launch(n_rows, kLast),
                     "%s: too many rows: more than 2^32 work items", what);
     ASDSL_CHECK_ARG(work, "%s: needs a work buffer of %zu bytes", what, p.bytes);
@@ -1090,7 +1097,6 @@ extern "C" asdsl_status asdsl_sample_logits(const float* logits, const float* un
     const bool vec = vocab % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % 16 == 0;
     const dim3 grid(static_cast<unsigned>(n_rows * p.slices)), block(kThreads);
     const hipStream_t hs = as_hip(stream);
-    const bool cuts = top_k || top_p;
     auto with = [&](auto is_vec, auto count, auto mass, auto drops) {
         constexpr bool kVec = decltype(is_vec)::value, kCount = decltype(count)::value, kMass = decltype(mass)::value;
         asdsl_status res = launch("sample_best_kernel", sample_best_kernel<kVec, kCount || kMass>, grid, block, 0, hs, a);

@@ -795,7 +795,10 @@ asdsl_status asdsl_logits_control(const float* logits, float* out, int* tokens, 
  * whose running sum of kept weights exceeds uniform * their sum, probs[row] = its
  * share of that sum; -1 and 0 where no token has a weight.  A temperature that is
  * not above 0 takes the first of the ranking.  temperature, top_k, top_p and min_p
- * [n_rows] may each be null: 1, all, all, all. */
+ * [n_rows] may each be null: 1, all, all, all.  The query with cuts gives what a
+ * call with top_k or top_p needs (cuts not 0) or one without either (0, some
+ * hundredth of it); the one without gives the first. */
+size_t asdsl_sample_logits_work_bytes_cuts(int n_rows, int vocab, int cuts);
 size_t asdsl_sample_logits_work_bytes(int n_rows, int vocab);
 asdsl_status asdsl_sample_logits(const float* logits, const float* uniform, const float* temperature,
                                  const int* top_k, const float* top_p, const float* min_p, int* tokens, float* probs,

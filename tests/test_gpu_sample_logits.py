@@ -316,6 +316,28 @@ def test_two_streams_at_once_and_the_same_each_time(gpu):
             assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 200064), (600, 300), (40, 5003)])
+def test_work_of_the_filters_that_a_call_has(gpu, rows, vocab):
+    """Without top-k and top-p a call allocates its outputs and a weight for 1024 tokens, no bins and lists; its
+    results in a buffer of that size alone are those beside all filters that keep everything."""
+    import torch
+
+    from asdsl.kernels import sample_logits
+
+    rng = np.random.default_rng(vocab)
+    x, u = dev((rng.standard_normal((rows, vocab)) * 3).astype(np.float32)), dev(rng.random(rows, dtype=np.float32))
+    t, m = dev(rng.uniform(0.3, 2, rows).astype(np.float32)), dev(rng.uniform(0, 0.1, rows).astype(np.float32))
+    k, p = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.ones(rows, device="cuda")
+    size = gpu.LIB.asdsl_sample_logits_work_bytes_cuts
+    for kw in ({}, {"temperature": t}, {"min_p": m}, {"temperature": t, "min_p": m}, {"top_k": k}, {"top_p": p}):
+        before = torch.cuda.memory_stats()["requested_bytes.all.allocated"]
+        got = sample_logits(x, u, **kw)
+        taken = torch.cuda.memory_stats()["requested_bytes.all.allocated"] - before
+        assert taken == size(rows, vocab, "top_k" in kw or "top_p" in kw) + 8 * rows
+        want = sample_logits(x, u, **{**kw, "top_k": k, "top_p": p})
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_more_than_2_31_logits(gpu):
     import torch
 

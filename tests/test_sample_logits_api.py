@@ -27,6 +27,27 @@ def test_abi_refusals():
     assert size(0, 5) == 0 and size(5, 0) == 0 and size(1, (1 << 20) + 1) == 0 and size(3, 200064) % 256 == 0
 
 
+def test_work_bytes_without_cuts():
+    """Calls without top-k and top-p need no bins and no lists, and are not refused for want of them."""
+    from asdsl import _hip
+
+    lib = _hip.LIB
+    size, most = lib.asdsl_sample_logits_work_bytes_cuts, lib.asdsl_sample_logits_work_bytes
+    for rows, vocab in ((1, 1), (1, 200064), (600, 300), (64, 200064), (11000, 200064)):
+        assert size(rows, vocab, 1) == size(rows, vocab, -3) == most(rows, vocab)
+        slices, tiles = most(rows, vocab) // (256 * 12 + 1024 * 8), rows * ((vocab + 1023) // 1024)
+        # a largest and a small logit a slice, a weight for 1024 tokens
+        assert tiles * 8 <= size(rows, vocab, 0) <= slices * 12 + tiles * 8 + 3 * 256 < most(rows, vocab)
+    assert not any(size(rows, vocab, c) for c in (0, 1) for rows, vocab in ((0, 5), (5, 0), (1, (1 << 20) + 1)))
+
+    def f(k, p, rows, vocab, nbytes):
+        return lib.asdsl_sample_logits(ONE, ONE, ONE, k, p, ONE, ONE, ONE, rows, vocab, ONE, nbytes, None)
+    for rows, vocab in ((1, 200064), (600, 300)):
+        refused(f(None, None, rows, vocab, size(rows, vocab, 0) - 1), "work buffer")
+        refused(f(ONE, None, rows, vocab, most(rows, vocab) - 1), "work buffer")
+        refused(f(None, ONE, rows, vocab, most(rows, vocab) - 1), "work buffer")
+
+
 def test_wrapper_refusals():
     import torch
 
