@@ -727,17 +727,17 @@ struct Step {
         }
     }
     // Step t: where its rows do not follow each other (at a range's end) every
-    // row is looked up by itself.
+    // row is looked up by itself.  4-bit steps come here only then (few_rows4).
     __device__ __forceinline__ void load_k(const Keys& K, int t, int lane) {
         const int i0 = t * kKeys;
-        if (rows_follow(K, i0))
+        if (F != kI4 && rows_follow(K, i0))
             k_rows<true>(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, lane);
         else
             k_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
     }
     __device__ __forceinline__ void load_v(const Keys& K, int t, int lane) {
         const int i0 = t * kKeys;
-        if (rows_follow(K, i0))
+        if (F != kI4 && rows_follow(K, i0))
             v_rows<true>(K, static_cast<size_t>(cache_row(K, i0)), [](int i) { return i; }, lane);
         else
             v_rows<false>(K, 0, [&](int i) { return static_cast<long long>(cache_row(K, min(i0 + i, K.n - 1))); }, lane);
