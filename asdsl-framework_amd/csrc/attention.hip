@@ -1619,7 +1619,9 @@ __global__ __launch_bounds__(kManyWaves * 64, 2) void window_many_kernel(const A
 // The sequence of the place-th largest position, by its kBits leading bits of a cache's
 // rows and then by index; for up to 64 * kGroups sequences.  Bit by bit, those that
 // have it before those that have not: scalar work, a quarter of what ranking every
-// lane takes.
+// lane takes.  More sequences are taken as they come, at a loss: us as they come / with
+// the longest first, 257 of up to 4000 rows 151 / 124, 300 173 / 149, 512 272 / 241,
+// 1000 of up to 2000 272 / 252, 512 of up to 500 59 / 55.
 constexpr int kOrdered = 4 * kWave;
 template <int kGroups, int kBits>
 __device__ __forceinline__ int sequence_of(const AttnArgs& g, int place) {
@@ -1992,6 +1994,10 @@ Plan plan_prefix(int n_seq, int n_heads, int n_kv, int head_dim, Kv form, int pr
     p.many = prefix_len > 0 && takes_many(total, n_kv, prefix_len, head_dim, form, true);
     p.wg_rows = p.many ? kManyWaves * kWideRows : kRows;
     p.own_jobs = static_cast<long long>(n_seq) * ((group + kRows - 1) / kRows) * n_kv;
+    // Over 4-bit keys this leaves long own rows in fewer pieces than splits_four would.  us
+    // with 512 / 768 / 1024 workgroups, 24 heads of 128: 32 sequences of up to 16384 own rows
+    // 145 / 100 / 87, 16 of them 67 / 53 / 51, 64 of up to 4352 85 / 61 / 62, 32 38 / 34 / 31,
+    // 8 16.8 / 17.7 / 18.6; 64 of up to 512 behind 16384 58 with each.
     const int own_splits = splits_for(kFillFew, p.own_jobs, own_rows, kMaxSlots / 4);
     const long long jobs = (total + p.wg_rows - 1) / p.wg_rows * n_kv;
     if (prefix_len > 0)

@@ -28,9 +28,10 @@ struct ReadArgs {
 // lane takes kPer rows, whose loads it requests together.
 //
 // Bound by memory and, for small calls, by the chain of position, codes and stores:
-// 4001 rows of 8 KV heads of 128 dims from 4 bits to fp16 (21 MB) take 6.4 us, 701
-// rows of 12 sequences of 8 heads of 64 dims from int8 to fp32 (44 MB) 9.8 (4.4
-// TB/s); a row a lane took 8.0 and 11.2.
+// 4001 rows of 8 KV heads of 128 dims from 4 bits to fp16 (21 MB) take 6.6 us and to
+// fp32 (37 MB) 8.9 (4.2 TB/s), from int8 to fp16 (25 MB) 7.2; 701 rows of 12 sequences
+// of 8 heads of 64 dims from int8 to fp32 (44 MB) 10.2 (4.3 TB/s).  A row a lane took
+// 1.5 us more at the first and the last of these.
 constexpr int kPer = 4;
 template <int D, bool kFour, typename T>
 __global__ __launch_bounds__(kReadThreads) void kv_read_kernel(const ReadArgs a) {
